@@ -60,6 +60,33 @@ typedef struct ttsp_fast_layer {
  * the count of barrier waits that gave up (sticky until the caller clears it). */
 enum { TTSP_FAST_SYNC_WORDS = 192, TTSP_FAST_SYNC_FAILED = 128 };
 
+/* A paged key-value cache as the ttsp_paged_* entries take it (no counterpart
+ * in the reference, whose cache is one contiguous sequence). K and V are pools
+ * of `pages` pages; element (page, kv head, row, d) of K is at
+ * K + page*k_page + head*k_head + row*k_row + d, V likewise: strides in
+ * elements, non-negative multiples of 8, bases 16-byte aligned, the pages' rows
+ * not overlapping. Row b of `table` (int32, at table + b*table_stride, `cols`
+ * entries) names the pages of sequence b, and slot j of the sequence is row
+ * j % page_size of its page j / page_size; an entry outside [0, pages) is a
+ * hole, through which nothing is read or written. page_size is a power of two
+ * from 16 to 4096, cols * page_size at most TTSP_PAGED_MAX_SLOTS, head_dim 64
+ * or 128, dtype TTSP_F16 or TTSP_BF16, seqs at most 65535.
+ * scores (fp32) and slot_pos (int32), each optional, hold per sequence, kv head
+ * and slot the attention weight the slot has gathered and the position its row
+ * came from: element (b, head, j) at scores + b*score_seq + head*score_head + j
+ * (slot_pos with its own strides), cols * page_size of them a head. */
+enum { TTSP_PAGED_MAX_SLOTS = 1 << 24 };
+typedef struct ttsp_paged_cache {
+  void* K;
+  void* V;
+  const int* table;
+  float* scores;
+  int* slot_pos;
+  long long k_page, k_head, k_row, v_page, v_head, v_row;
+  long long table_stride, score_seq, score_head, pos_seq, pos_head;
+  int seqs, cols, pages, page_size, n_kv, head_dim, dtype;
+} ttsp_paged_cache;
+
 #ifndef TTSP_HIP_TYPES_ONLY
 
 /* Y[N][M] = epi(X[N][K] . dequant(W)^T). N == 1 runs the HBM-bound GEMV (rows
@@ -550,6 +577,71 @@ int ttsp_fast_steps_grid(int dim, int n_head, int n_kv, int inter, int vocab, in
  * fast transformer's activation buffers inside the captured frame
  * (graphs.py:126-131). */
 int ttsp_fast_steps_work_bytes(int dim, int n_head, int n_kv, int inter);
+
+/* New rows of a paged cache from the wqkv output: row t at
+ * QKV + t*qkv_row_stride ((nh + 2 n_kv) heads of head_dim; a multiple of 8) is
+ * sequence SEQ[t]'s (NULL: sequence t's) row for slot SLOT[t] (int64). q and k
+ * heads are normed (x / sqrt(mean(x^2) + eps) * w, QW / KW [head_dim] of the
+ * cache's dtype, NULL: no norm) and rotated on interleaved pairs by row POS[t]
+ * (int64; NULL: row t) of the table F [n_freqs][head_dim / 2][2] (cos, sin) of
+ * ftype, in fp32 with one rounding at the end; q goes to Q [rows][nh][head_dim],
+ * k and v to the slot, whose score (if the cache has them) becomes 0 and whose
+ * slot_pos becomes POS[t]. A row whose slot lies outside [0, cols * page_size)
+ * or in a hole, or whose sequence lies outside [0, seqs), is not written; one
+ * whose position lies outside the table is not written either and its q is 0.
+ * No two rows may name one slot. Without norms the bits are those of
+ * ttsp_qk_rope_kv_rows. QKV, F, Q and the norm weights are 16-byte aligned; rows
+ * <= 2^24. Replaces: the head-norm / rotary / KV-write step of decode_block
+ * (app/engine/fusedlayer.py:56-92) for several sequences, which the reference
+ * decodes one at a time. */
+int ttsp_paged_qk_rope_kv(const ttsp_paged_cache* cache, const void* QKV, long long qkv_row_stride,
+                          const void* QW, const void* KW, float eps, const void* F, int ftype, int n_freqs,
+                          const long long* POS, const int* SEQ, const long long* SLOT, void* Q, int nh, int rows,
+                          void* stream);
+
+/* Rows that are finished already into a paged cache (a prompt's K and V from a
+ * contiguous one): element (t, kv head, d) at K + t*k_row_stride +
+ * head*k_head_stride + d (strides multiples of 8, bases 16-byte aligned), copied
+ * as ttsp_paged_qk_rope_kv's k and v. POS is needed where the cache has
+ * slot_pos. Replaces: nothing (see ttsp_paged_cache). */
+int ttsp_paged_store(const ttsp_paged_cache* cache, const void* K, long long k_row_stride, long long k_head_stride,
+                     const void* V, long long v_row_stride, long long v_head_stride, const long long* POS,
+                     const int* SEQ, const long long* SLOT, int rows, void* stream);
+
+/* KiB of ttsp_paged_attention's workspace (host-only; -1: over 2 TiB);
+ * tracked: the cache has scores. */
+int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size, int tracked);
+
+/* Attention of one new token per sequence over a paged cache: query (b, hd) at
+ * Q + b*q_seq_stride + hd*head_dim (a multiple of 8) attends, with kv head
+ * hd / (nh / n_kv), over slots 0 .. min(SLOT[b], cols * page_size - 1) of
+ * sequence b that lie in a page: Y[b][hd] = softmax(scale q . k) . v, zeros where
+ * there is none (SLOT[b] < 0). With scores, the sum over the kv head's query
+ * heads of the softmax weight of slot j is added to the score of slot j.
+ * work: ttsp_paged_attention_work_kib() KiB, 16-byte aligned, which calls that
+ * may overlap must not share; Q and Y are 16-byte aligned. Replaces: attn_partial
+ * + attn_combine, app/engine/fusedlayer.py:95-159, for several sequences. */
+int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
+                         const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
+
+/* KiB of ttsp_paged_evict's workspace (host-only; 0: no sequence can hold more
+ * than the budget; -1: over 2 TiB). */
+int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int budget);
+
+/* Cut every sequence of more than `budget` rows (SLOT[b] + 1, int64) down to
+ * it, in each kv head by itself: rows with slot_pos < sinks or slot_pos >
+ * POS[b] - recent (POS[b], int64: the newest position) come first, then the
+ * others by score (NaN lowest, as -inf), ties by the lowest slot, and the first
+ * `budget` are kept. Kept rows in slots from `budget` on move, in order, into
+ * the free slots below it, with their score and slot_pos; rows that stay, and
+ * what slots from `budget` on hold, are not touched. The sequence's next slot is
+ * then `budget` (the caller advances SLOT). sinks + recent <= budget. The
+ * pages of such a sequence belong to it alone and have no holes below SLOT[b];
+ * a row is not copied from or into a hole. work: ttsp_paged_evict_work_kib()
+ * KiB, 4-byte aligned, which calls that may overlap must not share. Replaces:
+ * nothing (the reference's cache is as long as its longest stream). */
+int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS, int budget,
+                     int sinks, int recent, int* work, void* stream);
 
 #endif /* TTSP_HIP_TYPES_ONLY */
 

@@ -45,6 +45,18 @@ class FastLayer(ctypes.Structure):
                 ("v_cache", _vp)]
 
 
+class PagedCache(ctypes.Structure):
+    """`ttsp_paged_cache`: a paged cache's pools, table and, optionally, scores and slot positions."""
+
+    _fields_ = [("K", _vp), ("V", _vp), ("table", _vp), ("scores", _vp), ("slot_pos", _vp),
+                *((name, _ll) for name in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row", "table_stride",
+                                           "score_seq", "score_head", "pos_seq", "pos_head")),
+                *((name, _i) for name in ("seqs", "cols", "pages", "page_size", "n_kv", "head_dim", "dtype"))]
+
+
+#: Most slots a sequence of a paged cache has (`TTSP_PAGED_MAX_SLOTS`).
+PAGED_MAX_SLOTS = 1 << 24
+
 #: `ttsp_fast_steps`' barrier words and the index of its failed-wait count.
 FAST_SYNC_WORDS, FAST_SYNC_FAILED = 192, 128
 
@@ -117,6 +129,13 @@ SIGNATURES: dict[str, list] = {
                         _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp],
     "ttsp_fast_steps_grid": [_i, _i, _i, _i, _i, _i, _i, _i],
     "ttsp_fast_steps_work_bytes": [_i, _i, _i, _i],
+    "ttsp_paged_qk_rope_kv": [ctypes.POINTER(PagedCache), _vp, _ll, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp, _vp, _i,
+                              _i, _vp],
+    "ttsp_paged_store": [ctypes.POINTER(PagedCache), _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _vp],
+    "ttsp_paged_attention_work_kib": [_i, _i, _i, _i, _i, _i, _i],
+    "ttsp_paged_attention": [ctypes.POINTER(PagedCache), _vp, _ll, _vp, _vp, _i, _f, _vp, _vp],
+    "ttsp_paged_evict_work_kib": [_i, _i, _i, _i, _i],
+    "ttsp_paged_evict": [ctypes.POINTER(PagedCache), _vp, _vp, _i, _i, _i, _vp, _vp],
 }
 
 

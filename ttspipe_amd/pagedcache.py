@@ -1,0 +1,433 @@
+"""Streams that decode together: a paged key-value cache, and the attention,
+writes and eviction that work on it.
+
+The reference decodes one sequence over one contiguous cache
+(app/engine/fusedlayer.py:162-306); a server of several streams keeps their
+keys and values in pages of one pool instead, so that a stream takes the pages
+it needs and gives them back. For D-wide heads (64 or 128) and 16-bit caches:
+
+* pools `k_pages`, `v_pages` (pages, n_local_heads, page size, D), the last
+  axis contiguous, any other strides that keep rows 16-byte aligned; the page
+  size a power of two from 16 to 4096;
+* `block_table` int32 (sequences, columns): row b names sequence b's pages, and
+  slot j of the sequence is row j % page size of its page j // page size. An
+  entry that is no page of the pool (-1) is a hole: its slots do not exist;
+* `slots` int64 (sequences,): the newest slot of each sequence, -1 for one that
+  holds nothing;
+* `scores` fp32 and `slot_pos` int32 (sequences, n_local_heads, columns * page
+  size), where a cache is evicted from: the attention weight each slot has
+  gathered and the position its row came from.
+
+`qk_rope_kv` and `store` write rows, `attention` reads them, `evict` cuts a
+sequence down to a budget. `PageTable` hands the pages out and keeps the device
+tensors above; `PagedKVCache` is one layer's pools with the four calls as
+methods; `fusedlayer.decode_batch` runs a transformer block on them.
+
+As elsewhere in the package a call the kernels cannot take returns None (and is
+counted in `stats()`), a wrong `out`, `work` or budget raises ValueError and a
+failed launch RuntimeError. Work is queued on the current stream of the
+tensors' device; nothing is synchronised, and with `out=` and `work=` given
+nothing is allocated, so that calls can be captured. Calls that may overlap
+(two streams, two graphs) need workspaces of their own.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from ttspipe_amd import _lib
+
+#: Head dims, and bounds of the page size (a power of two).
+HEAD_DIMS = (64, 128)
+MIN_PAGE, MAX_PAGE = 16, 4096
+
+_stats = {"rows": 0, "attention": 0, "evict": 0, "declined": 0}
+
+
+def stats() -> dict:
+    return dict(_stats)
+
+
+def _declined():
+    _stats["declined"] += 1
+
+
+def _pool(k_pages, v_pages, block_table, scores=None, slot_pos=None):
+    """The C-ABI's view of these tensors, or None where the kernels do not take them."""
+    dev = k_pages.device
+    if dev.type != "cuda" or v_pages.device != dev or block_table.device != dev:
+        return None
+    dt = _lib.dtype_code(k_pages.dtype)
+    if dt not in (_lib.DT_F16, _lib.DT_BF16) or v_pages.dtype != k_pages.dtype or block_table.dtype != torch.int32:
+        return None
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or block_table.dim() != 2:
+        return None
+    pages, nkv, page, hd = shape
+    seqs, cols = block_table.shape
+    if (hd not in HEAD_DIMS or not MIN_PAGE <= page <= MAX_PAGE or page & (page - 1) or not pages or not 1 <= nkv <= 4096
+            or not 1 <= seqs <= 65535 or not 1 <= cols <= _lib.PAGED_MAX_SLOTS // page):
+        return None
+    ks, vs, ts = k_pages.stride(), v_pages.stride(), block_table.stride()
+    for s in (ks, vs):
+        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or s[2] < hd or (nkv > 1 and s[1] < hd) or (
+                pages > 1 and s[0] < hd):
+            return None
+    if ts[1] != 1 and cols > 1 or (seqs > 1 and ts[0] < cols):
+        return None
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if kp % 16 or vp % 16:
+        return None
+    extra, strides = [], []
+    for t, dtype in ((scores, torch.float32), (slot_pos, torch.int32)):
+        if t is None:
+            extra.append(None)
+            strides += (0, 0)
+            continue
+        if t.dtype != dtype or t.device != dev or t.shape != (seqs, nkv, cols * page):
+            return None
+        st = t.stride()
+        if st[2] != 1 or (seqs > 1 and st[0] < cols * page) or (nkv > 1 and st[1] < cols * page):
+            return None
+        extra.append(t.data_ptr())
+        strides += (max(st[0], 1), st[1])
+    return _lib.PagedCache(kp, vp, block_table.data_ptr(), *extra, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                           max(ts[0], cols), *strides, seqs, cols, pages, page, nkv, hd, dt)
+
+
+def _vector(t, dtype, n, dev) -> bool:
+    """Whether `t` is a contiguous vector of n values of `dtype` on `dev`."""
+    return t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.device == dev and (n < 2 or t.stride(0) == 1)
+
+
+def _launch(what, dev, *args):
+    """`what` of the library on the current stream of `dev`."""
+    fn = getattr(_lib.lib(), what)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream())
+    if rc:
+        raise RuntimeError(f"{what} failed: hipError_t {rc}")
+
+
+def _rows_ok(rows, seqs_of, slots, positions, seqs, dev) -> bool:
+    if rows > 1 << 24 or not _vector(slots, torch.int64, rows, dev):
+        return False
+    if positions is not None and not _vector(positions, torch.int64, rows, dev):
+        return False
+    return rows <= seqs if seqs_of is None else _vector(seqs_of, torch.int32, rows, dev)
+
+
+def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, positions=None, *, q_weight=None,
+               k_weight=None, eps: float = 1e-6, seqs=None, scores=None, slot_pos=None, out=None):
+    """New rows from the wqkv output: qkv (rows, (n_head + 2 n_local_heads) D),
+    rows 16-byte aligned. Row t belongs to sequence `seqs[t]` (int32; None: to
+    sequence t), slot `slots[t]` (int64). Its q and k heads are normed with
+    `q_weight` / `k_weight` (None: no norm) and `eps` and rotated at
+    `positions[t]` (int64; None: row t) of `freqs_cis` (positions, D / 2, 2),
+    rounded once; k and v go to the slot, whose score becomes 0 and whose
+    `slot_pos` becomes the position. Returns q (rows, n_head, D), in `out` if
+    given, or None when declined.
+
+    A row whose slot has no page (or lies outside the table: -1 for a padding
+    row) is not written; a position outside `freqs_cis` makes its q zeros, too.
+    No two rows may name one slot. Without norms the result has the bits of the
+    contiguous cache's kernel, which with norms also rounds between the two."""
+    if not _lib.gpu_present():
+        return _declined()
+    c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
+    if c is None or qkv.dim() != 2:
+        return _declined()
+    dev, hd, dtype = k_pages.device, c.head_dim, k_pages.dtype
+    rows, width = qkv.shape
+    ftype = _lib.dtype_code(freqs_cis.dtype)
+    if (n_head < 1 or width != (n_head + 2 * c.n_kv) * hd or qkv.dtype != dtype or qkv.device != dev
+            or qkv.stride(1) != 1 or (rows > 1 and (qkv.stride(0) < width or qkv.stride(0) % 8)) or qkv.data_ptr() % 16
+            or ftype is None or freqs_cis.device != dev or freqs_cis.dim() != 3 or freqs_cis.shape[1:] != (hd // 2, 2)
+            or not freqs_cis.is_contiguous() or freqs_cis.data_ptr() % 16 or not freqs_cis.shape[0]
+            or freqs_cis.shape[0] >= 1 << 31 or not _rows_ok(rows, seqs, slots, positions, c.seqs, dev)):
+        return _declined()
+    if positions is None and (freqs_cis.shape[0] < rows or slot_pos is not None):
+        return _declined()
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != dtype or w.device != dev or w.shape != (hd,) or w.stride(0) != 1
+                              or w.data_ptr() % 16):
+            return _declined()
+    if out is None:
+        out = torch.empty(rows, n_head, hd, dtype=dtype, device=dev)
+    elif (out.shape != (rows, n_head, hd) or out.dtype != dtype or out.device != dev or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned (rows, n_head, head_dim) tensor of the cache's dtype")
+    if rows:
+        _launch("ttsp_paged_qk_rope_kv", dev, c, qkv.data_ptr(), max(qkv.stride(0), width) if rows > 1 else width,
+                _lib.ptr(q_weight), _lib.ptr(k_weight), eps, freqs_cis.data_ptr(), ftype, freqs_cis.shape[0],
+                _lib.ptr(positions), _lib.ptr(seqs), slots.data_ptr(), out.data_ptr(), n_head, rows)
+        _stats["rows"] += 1
+    return out
+
+
+def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=None, scores=None, slot_pos=None):
+    """Finished rows into the pages: k, v (rows, n_local_heads, D), the last axis
+    contiguous and rows 16-byte aligned (a contiguous cache's slice, transposed,
+    is taken in place). `seqs`, `slots`, `positions` (needed with `slot_pos`) and
+    the slots' scores as `qk_rope_kv`. True, or None when declined."""
+    if not _lib.gpu_present():
+        return _declined()
+    c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
+    if c is None or k.dim() != 3 or v.shape != k.shape:
+        return _declined()
+    dev, rows = k_pages.device, k.shape[0]
+    if k.shape[1:] != (c.n_kv, c.head_dim) or not _rows_ok(rows, seqs, slots, positions, c.seqs, dev):
+        return _declined()
+    if slot_pos is not None and positions is None:
+        return _declined()
+    for t in (k, v):
+        if (t.dtype != k_pages.dtype or t.device != dev or t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8
+                or t.data_ptr() % 16):
+            return _declined()
+    if rows:
+        _launch("ttsp_paged_store", dev, c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                v.stride(1), _lib.ptr(positions), _lib.ptr(seqs), slots.data_ptr(), rows)
+        _stats["rows"] += 1
+    return True
+
+
+def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, columns: int, page_size: int,
+                   tracked: bool = False) -> int:
+    """fp32 elements of `attention`'s workspace."""
+    kib = _lib.lib().ttsp_paged_attention_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
+                                                   int(tracked))
+    if kib < 0:
+        raise ValueError("the workspace would take more than 2 TiB")
+    return kib * 256
+
+
+def _workspace(work, need, dtype, dev):
+    """`work`, checked, or a workspace of `need` elements; its pointer and the tensor."""
+    if work is None:
+        work = torch.empty(need, dtype=dtype, device=dev)
+    elif (work.dtype != dtype or work.device != dev or not work.is_contiguous() or work.numel() < need
+          or work.data_ptr() % 16):
+        raise ValueError(f"work must be a contiguous, 16-byte aligned {dtype} tensor of at least {need} elements")
+    return work
+
+
+def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = None, scores=None, out=None,
+              work=None):
+    """One new token of each sequence over its cached rows: q (sequences, n_head,
+    D), a sequence's heads contiguous, over slots 0 .. slots[b] (cut to the
+    table's width), query head h with KV head h // (n_head / n_local_heads), the
+    scores scaled by `scale` (D^-0.5). Returns (sequences, n_head, D), in `out`
+    if given, or None when declined. A sequence without a row gives zeros.
+
+    With `scores`, each slot's weight, summed over the query heads of its KV
+    head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
+    `attention_work(...)` elements, else allocated per call."""
+    if not _lib.gpu_present():
+        return _declined()
+    c = _pool(k_pages, v_pages, block_table, scores)
+    if c is None or q.dim() != 3:
+        return _declined()
+    dev, hd = k_pages.device, c.head_dim
+    seqs, nh, d = q.shape
+    if (seqs != c.seqs or d != hd or nh < 1 or nh % c.n_kv or nh > 65535 or q.dtype != k_pages.dtype or q.device != dev
+            or q.stride(2) != 1 or (nh > 1 and q.stride(1) != hd)
+            or (seqs > 1 and (q.stride(0) < nh * hd or q.stride(0) % 8)) or q.data_ptr() % 16
+            or not _vector(slots, torch.int64, seqs, dev)):
+        return _declined()
+    if out is None:
+        out = torch.empty(seqs, nh, hd, dtype=q.dtype, device=dev)
+    elif (out.shape != (seqs, nh, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
+    work = _workspace(work, attention_work(seqs, nh, c.n_kv, hd, c.cols, c.page_size, scores is not None),
+                      torch.float32, dev)
+    _launch("ttsp_paged_attention", dev, c, q.data_ptr(), q.stride(0) if seqs > 1 else nh * hd, slots.data_ptr(),
+            out.data_ptr(), nh, hd**-0.5 if scale is None else scale, work.data_ptr())
+    _stats["attention"] += 1
+    return out
+
+
+def evict_work(seqs: int, n_local_heads: int, columns: int, page_size: int, budget: int) -> int:
+    """int32 elements of `evict`'s workspace."""
+    kib = _lib.lib().ttsp_paged_evict_work_kib(seqs, n_local_heads, columns, page_size, budget)
+    if kib < 0:
+        raise ValueError("the workspace would take more than 2 TiB")
+    return kib * 256
+
+
+def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, budget: int, *, sinks: int = 0,
+          recent: int = 0, work=None):
+    """Cut every sequence of more than `budget` rows down to it, in place and in
+    each KV head by itself: kept are rows of the first `sinks` positions and of
+    the last `recent` ones (up to `positions[b]`, int64, the newest), then those
+    of the largest scores (NaN counts as -inf), ties to the lowest slot. A kept
+    row below `budget` stays; the others move, in order, into the free slots
+    below it with their score and position. Slots from `budget` on are left as
+    they were, and so are `slots`: the caller's next slot is `budget`
+    (`PageTable.evicted`). True, or None when declined.
+
+    The pages of a sequence that is cut belong to it alone. `work`: an int32
+    workspace of `evict_work(...)` elements, else allocated per call."""
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget or budget > _lib.PAGED_MAX_SLOTS:
+        raise ValueError("evict needs a budget of at least one row, 0 <= sinks, 0 <= recent and sinks + recent <= budget")
+    if not _lib.gpu_present():
+        return _declined()
+    c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
+    dev = k_pages.device
+    if (c is None or scores is None or slot_pos is None or not _vector(slots, torch.int64, c.seqs, dev)
+            or not _vector(positions, torch.int64, c.seqs, dev)):
+        return _declined()
+    need = evict_work(c.seqs, c.n_kv, c.cols, c.page_size, budget)
+    if need:  # else no sequence can be longer than the budget
+        work = _workspace(work, need, torch.int32, dev)
+        _launch("ttsp_paged_evict", dev, c, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
+                work.data_ptr())
+    _stats["evict"] += 1
+    return True
+
+
+class PageTable:
+    """Pages of the pools handed to sequences, and the device tensors that the
+    calls read: `block_table`, `slots` and `positions` (the newest slot and
+    position of each sequence, -1: none). One table serves every layer's pools.
+
+    The host knows each sequence's row count without asking the device: `admit`
+    and `step` add rows, `evicted` cuts them, `release` drops them. Running out
+    of pages raises MemoryError and changes nothing."""
+
+    def __init__(self, seqs: int, max_len: int, pages: int, page_size: int = 64, device="cuda"):
+        if not MIN_PAGE <= page_size <= MAX_PAGE or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from {MIN_PAGE} to {MAX_PAGE}")
+        if seqs < 1 or pages < 1 or max_len < 1:
+            raise ValueError("seqs, max_len and pages must be positive")
+        self.page_size, self.pages, self.max_len = page_size, pages, max_len
+        columns = -(-max_len // page_size)
+        self.block_table = torch.full((seqs, columns), -1, dtype=torch.int32, device=device)
+        self.slots = torch.full((seqs,), -1, dtype=torch.int64, device=device)
+        self.positions = torch.full((seqs,), -1, dtype=torch.int64, device=device)
+        self._active = torch.zeros(seqs, dtype=torch.int64, device=device)
+        self._free = list(range(pages - 1, -1, -1))
+        self._held: list[list[int]] = [[] for _ in range(seqs)]
+        self._rows = [0] * seqs
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def rows(self, seq: int) -> int:
+        """Rows sequence `seq` holds."""
+        return self._rows[seq]
+
+    def _missing(self, seq: int, rows: int) -> int:
+        return max(0, -(-rows // self.page_size) - len(self._held[seq]))
+
+    def _grow(self, seq: int, rows: int) -> None:
+        held, n = self._held[seq], self._missing(seq, rows)
+        if n == 0:
+            return
+        new = [self._free.pop() for _ in range(n)]
+        self.block_table[seq, len(held): len(held) + n] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
+        held += new
+
+    def admit(self, rows: int):
+        """A free sequence with pages for `rows` rows (a prompt's, at positions
+        0 .. rows - 1): its index, or None when every sequence is taken."""
+        if not 1 <= rows <= self.max_len:
+            raise ValueError(f"a sequence holds 1 to {self.max_len} rows")
+        seq = next((i for i, n in enumerate(self._rows) if n == 0), None)
+        if seq is None:
+            return None
+        if self._missing(seq, rows) > len(self._free):
+            raise MemoryError(f"{self._missing(seq, rows)} pages needed, {len(self._free)} free")
+        self._grow(seq, rows)
+        self._rows[seq] = rows
+        self.slots[seq] = self.positions[seq] = rows - 1
+        self._active[seq] = 1
+        return seq
+
+    def step(self) -> None:
+        """One more row for every sequence: its page, slot and position."""
+        live = [i for i, n in enumerate(self._rows) if n]
+        if any(self._rows[i] == self.max_len for i in live):
+            raise ValueError(f"a sequence holds at most {self.max_len} rows")
+        need = sum(self._missing(i, self._rows[i] + 1) for i in live)
+        if need > len(self._free):
+            raise MemoryError(f"{need} pages needed, {len(self._free)} free")
+        for i in live:
+            self._grow(i, self._rows[i] + 1)
+            self._rows[i] += 1
+        self.slots += self._active
+        self.positions += self._active
+
+    def evicted(self, budget: int) -> None:
+        """After `evict` on every layer: no sequence holds more than `budget`
+        rows. Pages past those (and the next row's) go back to the pool."""
+        self.slots.clamp_(max=budget - 1)
+        keep = -(-(budget + 1) // self.page_size)
+        for seq, n in enumerate(self._rows):
+            if n > budget:
+                self._rows[seq] = budget
+                held = self._held[seq]
+                if len(held) > keep:
+                    self.block_table[seq, keep:] = -1
+                    self._free += held[keep:][::-1]
+                    del held[keep:]
+
+    def release(self, seq: int) -> None:
+        """Sequence `seq` ends: its pages go back to the pool."""
+        self._free += self._held[seq][::-1]
+        self._held[seq], self._rows[seq] = [], 0
+        self.block_table[seq] = -1
+        self.slots[seq] = self.positions[seq] = -1
+        self._active[seq] = 0
+
+
+class PagedKVCache(nn.Module):
+    """One layer's pools on a `PageTable`. `tracked`: with the scores and slot
+    positions that `evict` needs."""
+
+    def __init__(self, table: PageTable, n_heads: int, head_dim: int = 128, dtype=torch.bfloat16, tracked: bool = False):
+        super().__init__()
+        dev = table.block_table.device
+        self.table = table
+        shape = (table.pages, n_heads, table.page_size, head_dim)
+        self.register_buffer("k_pages", torch.zeros(shape, dtype=dtype, device=dev))
+        self.register_buffer("v_pages", torch.zeros(shape, dtype=dtype, device=dev))
+        slots = (table.block_table.shape[0], n_heads, table.block_table.shape[1] * table.page_size)
+        self.register_buffer("scores", torch.zeros(slots, dtype=torch.float32, device=dev) if tracked else None)
+        self.register_buffer("slot_pos", torch.zeros(slots, dtype=torch.int32, device=dev) if tracked else None)
+
+    def qk_rope_kv(self, qkv, n_head, freqs_cis, *, q_weight=None, k_weight=None, eps: float = 1e-6, out=None):
+        """`qk_rope_kv` of each sequence's newest row (qkv: one row a sequence)."""
+        t = self.table
+        return qk_rope_kv(qkv, n_head, self.k_pages, self.v_pages, t.block_table, t.slots, freqs_cis, t.positions,
+                          q_weight=q_weight, k_weight=k_weight, eps=eps, scores=self.scores, slot_pos=self.slot_pos,
+                          out=out)
+
+    def store(self, seq: int, k, v, start: int = 0):
+        """Rows start .. start + rows - 1 of sequence `seq` from k, v (rows, n_heads,
+        head_dim), their slots also their positions."""
+        t, rows = self.table, k.shape[0]
+        if start < 0 or start + rows > t.rows(seq):
+            raise ValueError(f"sequence {seq} holds {t.rows(seq)} rows")
+        slots = torch.arange(start, start + rows, dtype=torch.int64, device=t.slots.device)
+        seqs = torch.full((rows,), seq, dtype=torch.int32, device=t.slots.device)
+        return store(k, v, self.k_pages, self.v_pages, t.block_table, slots, positions=slots, seqs=seqs,
+                     scores=self.scores, slot_pos=self.slot_pos)
+
+    def attention(self, q, *, out=None, work=None):
+        """`attention` of each sequence's newest token; a tracked cache gathers its weights."""
+        t = self.table
+        return attention(q, self.k_pages, self.v_pages, t.block_table, t.slots, scores=self.scores, out=out, work=work)
+
+    def evict(self, budget: int, *, sinks: int = 0, recent: int = 0, work=None):
+        """`evict` on this layer (then, once for all layers, `PageTable.evicted`)."""
+        if self.scores is None:
+            raise ValueError("only a tracked cache is evicted from")
+        t = self.table
+        return evict(self.k_pages, self.v_pages, t.block_table, t.slots, self.scores, self.slot_pos, t.positions, budget,
+                     sinks=sinks, recent=recent, work=work)
