@@ -64,8 +64,9 @@ enum { TTSP_FAST_SYNC_WORDS = 192, TTSP_FAST_SYNC_FAILED = 128 };
  * in the reference, whose cache is one contiguous sequence). K and V are pools
  * of `pages` pages; element (page, kv head, row, d) of K is at
  * K + page*k_page + head*k_head + row*k_row + d, V likewise: strides in
- * elements, non-negative multiples of 8, bases 16-byte aligned, the pages' rows
- * not overlapping. Row b of `table` (int32, at table + b*table_stride, `cols`
+ * elements, non-negative multiples of 8 (k_row and v_row at most
+ * TTSP_PAGED_MAX_ROW_STRIDE), bases 16-byte aligned, the pages' rows not
+ * overlapping. Row b of `table` (int32, at table + b*table_stride, `cols`
  * entries) names the pages of sequence b, and slot j of the sequence is row
  * j % page_size of its page j / page_size; an entry outside [0, pages) is a
  * hole, through which nothing is read or written. page_size is a power of two
@@ -75,7 +76,7 @@ enum { TTSP_FAST_SYNC_WORDS = 192, TTSP_FAST_SYNC_FAILED = 128 };
  * and slot the attention weight the slot has gathered and the position its row
  * came from: element (b, head, j) at scores + b*score_seq + head*score_head + j
  * (slot_pos with its own strides), cols * page_size of them a head. */
-enum { TTSP_PAGED_MAX_SLOTS = 1 << 24 };
+enum { TTSP_PAGED_MAX_SLOTS = 1 << 24, TTSP_PAGED_MAX_ROW_STRIDE = 1 << 24 };
 typedef struct ttsp_paged_cache {
   void* K;
   void* V;

@@ -26,7 +26,7 @@ def _cache(**kw):
 
 
 BAD_CACHES = [dict(K=None), dict(V=None), dict(table=None), dict(K=P + 8), dict(V=P + 2), dict(table=P + 1), dict(k_page=-8),
-              dict(k_head=4), dict(v_row=129), dict(table_stride=3), dict(seqs=0), dict(seqs=65536), dict(cols=0),
+              dict(k_head=4), dict(v_row=129), dict(k_row=(1 << 24) + 8), dict(v_row=1 << 30), dict(table_stride=3), dict(seqs=0), dict(seqs=65536), dict(cols=0),
               dict(pages=0), dict(page_size=8), dict(page_size=24), dict(page_size=8192), dict(page_size=0), dict(n_kv=0),
               dict(n_kv=5000), dict(head_dim=96), dict(head_dim=256), dict(dtype=_lib.DT_F32), dict(dtype=7),
               dict(cols=(1 << 24) // 16 + 1, table_stride=1 << 30), dict(scores=P + 2), dict(score_seq=-1),

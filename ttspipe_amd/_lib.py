@@ -56,6 +56,8 @@ class PagedCache(ctypes.Structure):
 
 #: Most slots a sequence of a paged cache has (`TTSP_PAGED_MAX_SLOTS`).
 PAGED_MAX_SLOTS = 1 << 24
+#: Longest row stride of its pools, in elements (`TTSP_PAGED_MAX_ROW_STRIDE`).
+PAGED_MAX_ROW_STRIDE = 1 << 24
 
 #: `ttsp_fast_steps`' barrier words and the index of its failed-wait count.
 FAST_SYNC_WORDS, FAST_SYNC_FAILED = 192, 128

@@ -5,102 +5,495 @@
 // zeros. With scores, sum over the kv head's query heads of p_j is added to
 // the sequence's score of slot j.
 //
-// Workgroup = (kv head, sequence), one query head after the other: a thread a
-// key for the scores, a thread an output element for the sum over the values.
+// Memory bound: every cached row is read once for all the query heads of its
+// kv head (4 G flop a byte pair of K and V, G = nh / nkv), so what counts is
+// how many bytes are under way at once.
+//
+// The work. The sequences' rows are cut into chunks of about equal length,
+// enough of them to fill the GPU whatever the batch looks like (one long
+// sequence, many short ones): each workgroup reads all the slots, adds up the
+// rows, derives the chunk length and finds its own (sequence, chunk), so the
+// split follows the lengths on the device and a captured call keeps working as
+// they grow. Workgroup = (chunk, kv head or 16 of its query heads), four waves
+// that each take every fourth run of 32 keys and merge at the end; chunks of a
+// sequence join in a second launch. A sequence of one chunk is finished in the
+// first.
+//
+// A wave's 32 keys: S^T = K Q^T on the matrix cores (16 keys x 16 query heads a
+// tile; K straight from memory into the operand's layout, Q^T stays in
+// registers), so a lane holds 8 keys of one query head. The exponentials
+// subtract a reference that moves only when a score outgrows it by 2^8, so the
+// running maximum needs no exchange between lanes but a vote. P^T, rounded to
+// the cache's type for the matrix cores (half a step, 2^-9 or 2^-12 of each
+// term; the sums stay in fp32 and unrounded), feeds O^T += V^T P^T from the
+// registers it is in: the contraction takes the keys in the order the score
+// tiles hold them, and V^T comes from V's rows in LDS through the transposing
+// read. Each wave has its own 32 rows of LDS and never waits for another. K and
+// V rows of the next 32 keys are loaded while these are computed.
+//
+// MFMA 16x16x32: lane l supplies row (l % 16) of A and column (l % 16) of B at
+// k = 8 (l / 16) .. + 7; accumulator r of lane l is D[4 (l / 16) + r][l % 16].
 #include "paged_common.h"
 
 namespace ttsp {
+
+typedef __bf16 pg_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_f16x8 __attribute__((ext_vector_type(8)));
+typedef short pg_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pg_s16x4 pg_lds_s16x4;
+
+constexpr int PG_WAVES = 4, PG_KEYS = 32;      // waves a workgroup, keys a wave takes at once
+constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of this
+constexpr int PG_WGS = 1024;                   // workgroups the chunks are meant to make
+constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
+constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 
 struct AttnArgs {
   Paged c;
   const uint16_t* Q;  // [seqs][nh][D] by q_seq
   long long q_seq;
   const long long* SLOT;
-  uint16_t* Y;  // [seqs][nh][D]
-  float* work;  // scores in log2 units [seqs][nh][cap]
+  uint16_t* Y;   // [seqs][nh][D]
+  float* PM;     // [chunks][nh]: the chunk's reference (log2 units)
+  float* PL;     // [chunks][nh]: its sum of exp2(s - reference), -1: no key seen
+  float* PACC;   // [chunks][nh][D]: its sum of exp2(s - reference) v
+  float* S;      // scores in log2 units [seqs][nh][cap] (with scores to gather)
   float scale2;  // scale * log2(e)
-  int nh, seqs;
+  int nh, seqs, chunks, target;  // chunks: at most; target: chunks that fill the GPU
 };
 
-__device__ __forceinline__ float block_max(float v, float* s, int tid) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  __syncthreads();
-  if ((tid & 63) == 0) s[tid >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-}
-__device__ __forceinline__ float block_sum(float v, float* s, int tid) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((tid & 63) == 0) s[tid >> 6] = v;
-  __syncthreads();
-  return (s[0] + s[1]) + (s[2] + s[3]);
+template <int DT>
+__device__ __forceinline__ f32x4 pg_mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == DT_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf16x8, a), __builtin_bit_cast(pg_bf16x8, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_f16x8, a), __builtin_bit_cast(pg_f16x8, b), c, 0,
+                                                  0, 0);
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const AttnArgs a) {
-  __shared__ float q_s[D], red[4], y_s[256];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int n = a.c.rows(a.SLOT[b]), group = a.nh / a.c.nkv, mask = (1 << a.c.shift) - 1;
-  for (int g = 0; g < group; ++g) {
-    const int head = h * group + g;
-    float* w = a.work + ((size_t)b * a.nh + head) * a.c.cap();
-    uint16_t* y = a.Y + ((size_t)b * a.nh + head) * D;
-    __syncthreads();
-    if (tid < D) q_s[tid] = Elem<DT>::load(a.Q[b * a.q_seq + head * D + tid]);
-    __syncthreads();
-    float m = -3.0e38f, l = 0.0f, any = 0.0f;
-    for (int j = tid; j < n; j += 256) {
-      const int page = a.c.page(b, j);
-      float s = __uint_as_float(0xff800000u);
-      if (page >= 0) {
-        const uint16_t* k = a.c.K + page * a.c.k_page + h * a.c.k_head + (j & mask) * a.c.k_row;
-        s = 0.0f;
-        for (int d = 0; d < D; ++d) s = __builtin_fmaf(q_s[d], Elem<DT>::load(k[d]), s);
-        s *= a.scale2;
-        m = fmaxf(m, s);
-        any = 1.0f;
+// two fp32 values rounded to nearest even into a packed pair of DT
+template <int DT>
+__device__ __forceinline__ uint32_t pg_pack(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == DT_BF16) {
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, b16x2));
+  } else {
+    typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, h16x2));
+  }
+}
+
+// ds_read_b64_tr_b16: in each group of 16 lanes, lane j's element k is element
+// j % 4 of the 8 bytes that lane 4 k + j / 4 addresses.
+__device__ __forceinline__ uint2 pg_ld_tr(const uint8_t* p) {
+  const pg_lds_s16x4* q = (const pg_lds_s16x4*)(__attribute__((address_space(3))) const uint8_t*)p;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<pg_lds_s16x4*>(q)));
+}
+
+// Where chunk `gx` of the call lies.
+struct Chunk {
+  int b, n;       // its sequence (-1: there is no such chunk) and the sequence's rows
+  int c, count;   // its number in the sequence, and how many the sequence has
+  int first;      // the number in the call of the sequence's first chunk
+  int size;       // rows a chunk of this sequence
+};
+
+// A sequence's chunk count and their length, from the call's chunk length.
+__device__ __forceinline__ int chunk_count(int n, int len) { return (n + len - 1) / len; }
+__device__ __forceinline__ int chunk_size(int n, int count) {
+  return count < 2 ? n : ((n + count - 1) / count + PG_STEP - 1) / PG_STEP * PG_STEP;
+}
+
+// The call's chunk length: its rows over the chunks wanted, in steps.
+__device__ __forceinline__ int chunk_len(const AttnArgs& a, int lane) {
+  long long total = 0;
+  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+    const int b = b0 + lane;
+    long long n = b < a.seqs ? a.c.rows(a.SLOT[b]) : 0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
+    total += n;
+  }
+  const long long len = ((total + a.target - 1) / a.target + PG_STEP - 1) / PG_STEP * PG_STEP;
+  return (int)min(max(len, (long long)PG_STEP), 1LL << 30);
+}
+
+// Every wave finds it by itself; the result is uniform.
+__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int lane) {
+  const int len = chunk_len(a, lane);
+  int before = 0;
+  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < a.seqs ? a.c.rows(a.SLOT[b]) : 0;
+    const int count = chunk_count(n, len);
+    int x = count;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o, 64);
+      if (lane >= o) x += y;
+    }
+    const uint64_t past = __ballot(before + x > gx);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      Chunk k;
+      k.b = b0 + l;
+      k.n = __builtin_amdgcn_readlane(n, l);
+      k.count = __builtin_amdgcn_readlane(count, l);
+      k.first = before + __builtin_amdgcn_readlane(x, l) - k.count;
+      k.c = gx - k.first;
+      k.size = chunk_size(k.n, k.count);
+      return k;
+    }
+    before += __builtin_amdgcn_readlane(x, 63);
+  }
+  return Chunk{-1, 0, 0, 0, 0, 0};
+}
+
+template <int DT, int D, bool TRACK>
+__global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArgs a) {
+  constexpr int KC = D / 32, DC = D / 16;       // 32-wide steps of q . k, 16-wide tiles of V^T
+  constexpr int VPL = PG_KEYS * D * 2 / 1024;   // 16-byte pieces of the 32 V rows a lane
+  constexpr int VR = 1024 / (D * 2);            // V rows a load of the wave covers
+  constexpr int REGION = PG_KEYS * D * 2;       // a wave's LDS: V rows, at the end 16 fp32 rows of O
+  static_assert(REGION == PG_HEADS * D * 4, "the output tile takes the V rows' place");
+  __shared__ __align__(16) uint8_t lds[PG_WAVES * REGION];
+  __shared__ float m_s[PG_WAVES][PG_HEADS], l_s[PG_WAVES][PG_HEADS];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int group = a.nh / a.c.nkv, hgs = (group + PG_HEADS - 1) / PG_HEADS;
+  const int h = blockIdx.y / hgs, head0 = h * group + (blockIdx.y % hgs) * PG_HEADS;
+  const int heads = min(PG_HEADS, (h + 1) * group - head0);
+  const Chunk ck = find_chunk(a, blockIdx.x, lane);
+  if (ck.b < 0) return;
+  const int b = __builtin_amdgcn_readfirstlane(ck.b);
+  const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
+  const int mask = (1 << a.c.shift) - 1;
+  uint8_t* const vs = lds + wave * REGION;
+
+  // Q^T: column = query head lr, dims 32 i + 8 lg .. + 7
+  u32x4 qf[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i)
+    qf[i] = lr < heads ? *reinterpret_cast<const u32x4*>(a.Q + b * a.q_seq + (size_t)(head0 + lr) * D + 32 * i + 8 * lg)
+                       : u32x4{0u, 0u, 0u, 0u};
+
+  // pages of the two 16-key halves of the run at j (uniform; past the chunk: holes)
+  const int* const trow = a.c.table + b * a.c.table_stride;
+  auto page_at = [&](int j) {
+    const int p = j < k1 ? trow[j >> a.c.shift] : -1;
+    return (unsigned)p < (unsigned)a.c.pages ? p : -1;
+  };
+  const uint32_t ko = (uint32_t)(lr * (int)a.c.k_row + 8 * lg);
+  const uint32_t vo = (uint32_t)((lane / (64 / VR)) * (int)a.c.v_row + (lane % (64 / VR)) * 8);
+  u32x4 kf[2][KC], vf[VPL];
+  // A hole reads page 0's rows, which are masked; a page's 16-row runs are whole.
+  auto load = [&](int j, int p0, int p1) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int p = max(s ? p1 : p0, 0), row = (j + 16 * s) & mask;
+      const uint16_t* kb = a.c.K + p * a.c.k_page + h * a.c.k_head + row * a.c.k_row;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) kf[s][i] = *reinterpret_cast<const u32x4*>(kb + ko + 32 * i);
+      const uint16_t* vb = a.c.V + p * a.c.v_page + h * a.c.v_head + row * a.c.v_row;
+#pragma unroll
+      for (int i = 0; i < VPL / 2; ++i)
+        vf[s * (VPL / 2) + i] = *reinterpret_cast<const u32x4*>(vb + vo + (uint32_t)(i * VR * (int)a.c.v_row));
+    }
+  };
+  // V's 32-byte blocks lie swizzled by row, so that the transposing reads of
+  // eight rows touch all banks
+  auto vaddr = [&](int row, int blk) {
+    const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
+    return row * (D * 2) + ((blk ^ sw) << 5);
+  };
+
+  f32x4 o[DC];
+#pragma unroll
+  for (int d = 0; d < DC; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float mref = PG_NONE, lsum = 0.0f;
+  bool seen = false;
+  float* const srow = TRACK ? a.S + ((size_t)b * a.nh + head0 + lr) * a.c.cap() : nullptr;
+
+  int j = k0 + PG_KEYS * wave;
+  int p0 = page_at(j), p1 = page_at(j + 16);
+  if (j < k1) load(j, p0, p1);
+  int n0 = page_at(j + PG_STEP), n1 = page_at(j + PG_STEP + 16);
+  for (; j < k1; j += PG_STEP) {
+    const bool whole = j + PG_KEYS <= k1 && p0 >= 0 && p1 >= 0;
+    seen = seen || p0 >= 0 || p1 >= 0;
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < KC; ++i) s[t] = pg_mfma<DT>(kf[t][i], qf[i], s[t]);
+    }
+    // V rows into LDS; rows that are no keys as zeros (what they hold may be NaN)
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int row = i * VR + lane / (64 / VR), c16 = lane % (64 / VR);
+      u32x4 v = vf[i];
+      if (!whole && (j + row >= k1 || (row < 16 ? p0 : p1) < 0)) v = u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = v;
+    }
+    // the next run's rows
+    const int c0 = p0, c1 = p1;
+    p0 = n0, p1 = n1;
+    if (j + PG_STEP < k1) load(j + PG_STEP, p0, p1);
+    n0 = page_at(j + 2 * PG_STEP), n1 = page_at(j + 2 * PG_STEP + 16);
+
+    // scores in log2 units; keys 16 t + 4 lg + r of the run
+    bool over = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = s[t][r] * a.scale2;
+        if (!whole && (j + 16 * t + 4 * lg + r >= k1 || (t ? c1 : c0) < 0)) x = -__builtin_inff();
+        s[t][r] = x;
+        over = over || x > mref + 8.0f;
       }
-      w[j] = s;
+    if constexpr (TRACK) {
+      if (lr < heads)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (j + 16 * t < k1) *reinterpret_cast<f32x4*>(srow + j + 16 * t + 4 * lg) = s[t];
     }
-    m = block_max(m, red, tid);
-    any = block_max(any, red, tid);
-    for (int j = tid; j < n; j += 256) {
-      const float p = a.c.page(b, j) < 0 ? 0.0f : __builtin_amdgcn_exp2f(w[j] - m);
-      w[j] = p;
-      l += p;
+    if (__any(over)) {
+      float bm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+      const float mnew = bm > mref + 8.0f ? bm : mref;
+      const float alpha = __builtin_amdgcn_exp2f(mref - mnew);
+      mref = mnew;
+      lsum *= alpha;
+#pragma unroll
+      for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
     }
-    l = block_sum(l, red, tid);
-    if (any == 0.0f) {
-      if (tid < D) y[tid] = 0;
+    u32x4 pf;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(s[t][r] - mref);
+        lsum += p[r];
+      }
+      pf[2 * t] = pg_pack<DT>(p[0], p[1]);
+      pf[2 * t + 1] = pg_pack<DT>(p[2], p[3]);
+    }
+    // V^T: row = dim 16 d + lr at keys 4 lg .. + 3 and 16 + 4 lg .. + 3
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int d = 0; d < DC; ++d) {
+      const int row = 4 * lg + (lr >> 2);
+      const uint2 lo = pg_ld_tr(vs + vaddr(row, d) + 8 * (lr & 3));
+      const uint2 hi = pg_ld_tr(vs + vaddr(row + 16, d) + 8 * (lr & 3));
+      o[d] = pg_mfma<DT>(u32x4{lo.x, lo.y, hi.x, hi.y}, pf, o[d]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+
+  // The waves' parts: each leaves its reference, sum and O [head][D] in LDS.
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  if (lane < PG_HEADS) {
+    m_s[wave][lane] = mref;
+    l_s[wave][lane] = seen ? lsum : -1.0f;
+  }
+  float* const os = reinterpret_cast<float*>(vs);
+#pragma unroll
+  for (int d = 0; d < DC; ++d) *reinterpret_cast<f32x4*>(os + lr * D + 16 * d + 4 * lg) = o[d];
+  __syncthreads();
+  const float* const all = reinterpret_cast<const float*>(lds);
+  const bool alone = ck.count == 1;
+  for (int i = tid; i < heads * D; i += 64 * PG_WAVES) {
+    const int g = i / D, d = i % D;
+    float m = PG_NONE;
+#pragma unroll
+    for (int w = 0; w < PG_WAVES; ++w) m = fmaxf(m, m_s[w][g]);
+    float num = 0.0f, den = 0.0f;
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < PG_WAVES; ++w) {
+      const float l = l_s[w][g];
+      if (l < 0.0f) continue;
+      const float e = __builtin_amdgcn_exp2f(m_s[w][g] - m);
+      den += l * e;
+      num += all[(size_t)w * (REGION / 4) + g * D + d] * e;
+      any = true;
+    }
+    const int head = head0 + g;
+    if (alone) {
+      a.Y[((size_t)b * a.nh + head) * D + d] = Elem<DT>::store(any ? num / den : 0.0f);
       continue;
     }
-    for (int j = tid; j < n; j += 256) w[j] /= l;
-    __syncthreads();
-    constexpr int KS = 256 / D;
-    float acc = 0.0f;
-    for (int j = tid / D; j < n; j += KS) {
-      const int page = a.c.page(b, j);
-      if (page < 0) continue;
-      acc = __builtin_fmaf(w[j], Elem<DT>::load(a.c.V[page * a.c.v_page + h * a.c.v_head + (j & mask) * a.c.v_row + tid % D]), acc);
-    }
-    y_s[tid] = acc;
-    __syncthreads();
-    if (tid < D) {
-      for (int k = 1; k < KS; ++k) acc += y_s[tid + k * D];
-      y[tid] = Elem<DT>::store(acc);
+    const size_t at = (size_t)blockIdx.x * a.nh + head;
+    a.PACC[at * D + d] = num;
+    if (d == 0) {
+      a.PM[at] = m;
+      a.PL[at] = any ? den : -1.0f;
     }
   }
-  __syncthreads();
-  if (a.c.scores)
-    for (int j = tid; j < n; j += 256) {
-      if (a.c.page(b, j) < 0) continue;
-      float s = 0.0f;
-      for (int g = 0; g < group; ++g) s += a.work[((size_t)b * a.nh + h * group + g) * a.c.cap() + j];
-      a.c.scores[b * a.c.score_seq + h * a.c.score_head + j] += s;
+  if (!TRACK || !alone) {
+    return;
+  }
+  if (group > PG_HEADS) {  // several workgroups share the kv head: the second launch adds their weights up
+    const int g = tid;
+    if (g < heads) {
+      float m = PG_NONE, den = 0.0f;
+      bool any = false;
+      for (int w = 0; w < PG_WAVES; ++w) m = fmaxf(m, m_s[w][g]);
+      for (int w = 0; w < PG_WAVES; ++w)
+        if (!(l_s[w][g] < 0.0f)) den += l_s[w][g] * __builtin_amdgcn_exp2f(m_s[w][g] - m), any = true;
+      const size_t at = (size_t)blockIdx.x * a.nh + head0 + g;
+      a.PM[at] = m;
+      a.PL[at] = any ? den : -1.0f;
     }
+    return;
+  }
+  // the weights of a sequence of one chunk
+  for (int k = k0 + tid; k < k1; k += 64 * PG_WAVES) {
+    if (a.c.page(b, k) < 0) continue;
+    float w = 0.0f;
+    for (int g = 0; g < heads; ++g) {
+      float m = PG_NONE, den = 0.0f;
+      for (int v = 0; v < PG_WAVES; ++v) m = fmaxf(m, m_s[v][g]);
+      for (int v = 0; v < PG_WAVES; ++v)
+        if (!(l_s[v][g] < 0.0f)) den += l_s[v][g] * __builtin_amdgcn_exp2f(m_s[v][g] - m);
+      w += __builtin_amdgcn_exp2f(a.S[((size_t)b * a.nh + head0 + g) * a.c.cap() + k] - m) / den;
+    }
+    a.c.scores[b * a.c.score_seq + h * a.c.score_head + k] += w;
+  }
+}
+
+// The reference and sum of one query head over a sequence's chunks, by a wave;
+// uniform. den < 0: no key.
+__device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, int head, int lane, float* m, float* den) {
+  float mx = PG_NONE;
+  for (int c = lane; c < ck.count; c += 64) mx = fmaxf(mx, a.PM[(size_t)(ck.first + c) * a.nh + head]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  float l = 0.0f;
+  bool any = false;
+  for (int c = lane; c < ck.count; c += 64) {
+    const size_t at = (size_t)(ck.first + c) * a.nh + head;
+    const float x = a.PL[at];
+    if (x < 0.0f) continue;
+    l += x * __builtin_amdgcn_exp2f(a.PM[at] - mx);
+    any = true;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+  *m = mx;
+  *den = __any(any) ? l : -1.0f;
+}
+
+// Joins a sequence's chunks: workgroup (query head, sequence).
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
+  constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
+  __shared__ f32x4 part[256];
+  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int len = chunk_len(a, lane);
+  int first = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) {
+    int count = b0 + lane < b ? chunk_count(a.c.rows(a.SLOT[b0 + lane]), len) : 0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) count += __shfl_xor(count, o, 64);
+    first += count;
+  }
+  Chunk ck{b, a.c.rows(a.SLOT[b]), 0, 0, first, 0};
+  ck.count = chunk_count(ck.n, len);
+  uint16_t* const y = a.Y + ((size_t)b * a.nh + head) * D;
+  if (ck.count == 1) return;  // finished already
+  if (ck.count == 0) {
+    if (tid < D / 8) reinterpret_cast<u32x4*>(y)[tid] = u32x4{0u, 0u, 0u, 0u};
+    return;
+  }
+  float m, den;
+  join_sums(a, ck, head, lane, &m, &den);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int e = tid % (D / 4);
+  for (int c = tid / (D / 4); c < ck.count; c += ROWS) {
+    const size_t at = (size_t)(ck.first + c) * a.nh + head;
+    if (a.PL[at] < 0.0f) continue;
+    const f32x4 x = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
+    const float w = __builtin_amdgcn_exp2f(a.PM[at] - m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += x[i] * w;
+  }
+  part[tid] = acc;
+  __syncthreads();
+  if (tid >= D / 4) return;
+  for (int r = 1; r < ROWS; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += part[r * (D / 4) + tid][i];
+  uint2 out;
+  float q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = den < 0.0f ? 0.0f : acc[i] / den;
+  out.x = Elem<DT>::store(q[0]) | (uint32_t)Elem<DT>::store(q[1]) << 16;
+  out.y = Elem<DT>::store(q[2]) | (uint32_t)Elem<DT>::store(q[3]) << 16;
+  reinterpret_cast<uint2*>(y)[tid] = out;
+}
+
+// Adds the weights of a chunk's slots to their scores: workgroup (chunk, kv
+// head), for sequences that the first launch has not finished.
+__global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a) {
+  constexpr int HG = 64;  // query heads whose sums are held at once
+  __shared__ float m_s[HG], l_s[HG];
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = a.nh / a.c.nkv;
+  const Chunk ck = find_chunk(a, blockIdx.x, lane);
+  if (ck.b < 0 || (ck.count == 1 && group <= PG_HEADS)) return;
+  const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
+  for (int g0 = 0; g0 < group; g0 += HG) {
+    const int gs = min(HG, group - g0);
+    __syncthreads();
+    for (int g = wave; g < gs; g += 4) {
+      float m, den;
+      join_sums(a, ck, h * group + g0 + g, lane, &m, &den);
+      if (lane == 0) m_s[g] = m, l_s[g] = den;
+    }
+    __syncthreads();
+    for (int k = k0 + tid; k < k1; k += 256) {
+      if (a.c.page(ck.b, k) < 0) continue;
+      const float* s = a.S + ((size_t)ck.b * a.nh + h * group + g0) * a.c.cap() + k;
+      float w = 0.0f;
+      for (int g = 0; g < gs; ++g) w += __builtin_amdgcn_exp2f(s[(size_t)g * a.c.cap()] - m_s[g]) / l_s[g];
+      a.c.scores[ck.b * a.c.score_seq + h * a.c.score_head + k] += w;
+    }
+  }
+}
+
+// How a call is cut up; false where the workspace's size overflows.
+struct AttnPlan {
+  int target, chunks, hgs;
+  size_t parts, scores;  // floats
+};
+inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, bool tracked, AttnPlan* p) {
+  const int group = nh / nkv;
+  p->hgs = (group + PG_HEADS - 1) / PG_HEADS;
+  const long long wide = (long long)nkv * p->hgs;
+  p->target = (int)(wide < PG_WGS ? PG_WGS / wide : 1);
+  // a sequence adds at most one partly filled chunk to those the rows fill
+  const long long most = (long long)seqs * ((cap + PG_STEP - 1) / PG_STEP);
+  const long long chunks = p->target + (long long)seqs;
+  p->chunks = (int)(most < chunks ? most : chunks);
+  p->parts = (((size_t)p->chunks * nh * (2 + hd)) + 3) / 4 * 4;
+  p->scores = tracked ? (size_t)seqs * nh * cap : 0;
+  return (p->parts + p->scores) / 256 + 1 <= 0x7fffffff;
 }
 
 }  // namespace ttsp
@@ -109,37 +502,53 @@ using namespace ttsp;
 
 extern "C" int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size,
                                              int tracked) {
-  (void)nkv, (void)head_dim, (void)tracked;
-  if (seqs < 1 || nh < 1 || cols < 1 || page_size < 1) return 0;
-  const long long kib = ((long long)seqs * nh * cols * page_size * 4 + 1023) / 1024;
-  return kib > 0x7fffffffLL ? -1 : (int)kib;
+  if (seqs < 1 || nkv < 1 || nh < nkv || cols < 1 || page_size < 1 || head_dim < 1) return 0;
+  AttnPlan p;
+  if (!attn_plan(seqs, nh, nkv, head_dim, (long long)cols * page_size, tracked != 0, &p)) return -1;
+  return (int)((p.parts + p.scores + 255) / 256);
 }
 
 extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
                                     const long long* SLOT, void* Y, int nh, float scale, float* work,
                                     hipStream_t stream) {
   AttnArgs a{};
+  AttnPlan p;
   if (!paged_args(cache, &a.c) || !Q || !SLOT || !Y || !work || nh < 1 || nh > 65535 || nh % a.c.nkv ||
       (uintptr_t)Q % 16 || (uintptr_t)Y % 16 || (uintptr_t)work % 16 || q_seq_stride % 8 ||
       q_seq_stride < (long long)nh * cache->head_dim)
+    return (int)hipErrorInvalidValue;
+  const int hd = cache->head_dim;
+  const bool tracked = a.c.scores != nullptr;
+  if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p) || (long long)a.c.nkv * p.hgs > 65535)
     return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;
   a.q_seq = q_seq_stride;
   a.SLOT = SLOT;
   a.Y = (uint16_t*)Y;
-  a.work = work;
+  a.PACC = work;
+  a.PM = work + (size_t)p.chunks * nh * hd;
+  a.PL = a.PM + (size_t)p.chunks * nh;
+  a.S = tracked ? work + p.parts : nullptr;
   a.scale2 = scale * 1.4426950408889634f;
   a.nh = nh;
   a.seqs = a.c.seqs;
-#define TTSP_PATT(DTV, DV) \
-  hipLaunchKernelGGL((paged_attn_kernel<DTV, DV>), dim3(a.c.nkv, a.seqs), dim3(256), 0, stream, a)
+  a.chunks = p.chunks;
+  a.target = p.target;
+  const dim3 grid(p.chunks, a.c.nkv * p.hgs);
+#define TTSP_PATT(DTV, DV)                                                                                       \
+  do {                                                                                                           \
+    if (tracked) hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, true>), grid, dim3(64 * PG_WAVES), 0, stream, a); \
+    else hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, false>), grid, dim3(64 * PG_WAVES), 0, stream, a);        \
+    hipLaunchKernelGGL((paged_join_kernel<DTV, DV>), dim3(nh, a.seqs), dim3(256), 0, stream, a);                  \
+  } while (0)
   if (cache->dtype == DT_F16) {
-    if (cache->head_dim == 128) TTSP_PATT(DT_F16, 128);
+    if (hd == 128) TTSP_PATT(DT_F16, 128);
     else TTSP_PATT(DT_F16, 64);
   } else {
-    if (cache->head_dim == 128) TTSP_PATT(DT_BF16, 128);
+    if (hd == 128) TTSP_PATT(DT_BF16, 128);
     else TTSP_PATT(DT_BF16, 64);
   }
 #undef TTSP_PATT
+  if (tracked) hipLaunchKernelGGL(paged_gather_kernel, dim3(p.chunks, a.c.nkv), dim3(256), 0, stream, a);
   TTSP_RETURN_LAUNCH();
 }

@@ -48,6 +48,7 @@ inline bool paged_args(const ttsp_paged_cache* c, Paged* p) {
   const long long strides[] = {c->k_page, c->k_head, c->k_row, c->v_page, c->v_head, c->v_row};
   for (long long s : strides)
     if (s < 0 || s % 8) return false;
+  if (c->k_row > TTSP_PAGED_MAX_ROW_STRIDE || c->v_row > TTSP_PAGED_MAX_ROW_STRIDE) return false;
   if (c->n_kv < 1 || c->n_kv > 4096 || c->pages < 1 || c->seqs < 1 || c->seqs > 65535 || c->cols < 1 ||
       c->table_stride < c->cols || c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
     return false;

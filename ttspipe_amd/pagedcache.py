@@ -71,7 +71,7 @@ def _pool(k_pages, v_pages, block_table, scores=None, slot_pos=None):
         return None
     ks, vs, ts = k_pages.stride(), v_pages.stride(), block_table.stride()
     for s in (ks, vs):
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or s[2] < hd or (nkv > 1 and s[1] < hd) or (
+        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or not hd <= s[2] <= _lib.PAGED_MAX_ROW_STRIDE or (nkv > 1 and s[1] < hd) or (
                 pages > 1 and s[0] < hd):
             return None
     if ts[1] != 1 and cols > 1 or (seqs > 1 and ts[0] < cols):
