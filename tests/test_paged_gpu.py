@@ -400,7 +400,8 @@ def test_evict_matches_the_definition(kind, hd, page, dtype, budget, sinks, rece
     assert moved or budget == 1  # (budget 1: the kept row may be slot 0)
 
 
-@pytest.mark.parametrize("n,budget", [(1025, 1024), (1030, 1024), (1100, 1024), (5000, 4999), (8192, 4096), (70001, 20000),
+@pytest.mark.parametrize("n,budget", [(1025, 1024), (1030, 1024), (1100, 1024), (5000, 4999), (8192, 4096), (20000, 19990), (20000, 5000),
+                                      (65530, 70), (70001, 20000),
                                       (70001, 69000)])
 @pytest.mark.parametrize("kind", ["exp", "every"])
 def test_evict_of_long_sequences(n, budget, kind):

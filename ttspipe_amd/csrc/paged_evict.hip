@@ -8,10 +8,17 @@
 // slot below (K, V, score and position): sources and destinations do not
 // overlap, and only the rows that have to move are read and written.
 //
-// The threshold is the budget-th largest key, found digit by digit (four
-// passes over 8 bits of the key's order-preserving integer form, a histogram
-// in LDS each); a scan over the slots in order then names the movers and the
-// free slots. A second launch moves the K and V rows, a group of lanes each.
+// The threshold is the budget-th largest key, found digit by digit of the
+// key's order-preserving integer form (11, 11 and 10 bits): a histogram in LDS,
+// each bin in eight copies that neighbouring lanes spread over (scores share
+// their leading bits, and a wave's adds to one word queue up), and a scan from
+// the top bin. It ends early where a bin is kept whole. One workgroup ranks a
+// (sequence, kv head), its keys read once and held in registers (up to 64 a
+// thread; a longer cache's are read again in each pass), a wave's keys
+// neighbouring slots, so that ranks among equal keys, movers and free slots are
+// counted with ballots and one prefix over the waves each. A second launch
+// moves the K and V rows, a group of lanes each; where the cache has little room
+// past the budget (a step that evicts one row) the first moves them itself.
 #include "paged_common.h"
 
 namespace ttsp {
@@ -20,11 +27,13 @@ struct EvictArgs {
   Paged c;
   const long long* SLOT;
   const long long* POS;
-  int budget, sinks, recent, max_moves, hd;
+  int budget, sinks, recent, max_moves;
   int* work;  // per (sequence, kv head): the count, then max_moves sources and max_moves destinations
 };
 
-constexpr int EV_T = 1024;
+constexpr int EV_BINS = 2048, EV_COPIES = 8;
+// At most this many rows a (sequence, kv head) are moved by the ranking workgroup itself.
+constexpr int EV_INLINE = 256;
 
 // Larger keys are larger integers; -0 and +0 are one key.
 __device__ __forceinline__ uint32_t order_of(float f) {
@@ -32,91 +41,192 @@ __device__ __forceinline__ uint32_t order_of(float f) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, const float* sc, const int* sp, int j, long long pos) {
-  const float f = sc[j];
-  const int p = sp[j];
-  if (p < a.sinks || p > pos - a.recent) return order_of(__uint_as_float(0x7f800000u));
+// The key of a row of score f and position p: +inf if protected (p below
+// `sinks` or above `newest`, the last position that is not recent).
+__device__ __forceinline__ uint32_t evict_key(float f, int p, int sinks, long long newest) {
+  if (p < sinks || p > newest) return order_of(__uint_as_float(0x7f800000u));
   return order_of(f != f ? __uint_as_float(0xff800000u) : f);
 }
 
-// Exclusive prefix over the workgroup of v (0 .. a few), and the total.
-__device__ __forceinline__ int block_scan(int v, int* s, int tid, int* total) {
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if ((tid & 63) >= o) x += y;
-  }
-  __syncthreads();
-  if ((tid & 63) == 63) s[tid >> 6] = x;
-  __syncthreads();
-  int base = 0, all = 0;
-  for (int w = 0; w < EV_T / 64; ++w) {
-    if (w < (tid >> 6)) base += s[w];
-    all += s[w];
-  }
-  *total = all;
-  return base + x - v;
+// One row (K and V) from slot src to slot dst of sequence b, head h, by D / 8 lanes.
+template <int D>
+__device__ __forceinline__ void move_row(const Paged& c, int b, int h, int src, int dst, int lane) {
+  const int from = c.page(b, src), to = c.page(b, dst), mask = (1 << c.shift) - 1, e = lane * 8;
+  if (from < 0 || to < 0) return;
+  const u32x4 k = *reinterpret_cast<const u32x4*>(c.K + from * c.k_page + h * c.k_head + (src & mask) * c.k_row + e);
+  const u32x4 v = *reinterpret_cast<const u32x4*>(c.V + from * c.v_page + h * c.v_head + (src & mask) * c.v_row + e);
+  *reinterpret_cast<u32x4*>(c.K + to * c.k_page + h * c.k_head + (dst & mask) * c.k_row + e) = k;
+  *reinterpret_cast<u32x4*>(c.V + to * c.v_page + h * c.v_head + (dst & mask) * c.v_row + e) = v;
 }
 
-__global__ __launch_bounds__(EV_T) void paged_evict_select_kernel(const EvictArgs a) {
-  __shared__ int hist[256], scan_s[EV_T / 64], pick[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+// T threads; R: keys a thread holds (0: read again in every pass).
+template <int T, int R, int D, bool INLINE>
+__global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a) {
+  constexpr int W = T / 64, PER = EV_BINS / T;  // waves; bins a thread adds up
+  __shared__ __align__(16) int hist[EV_BINS * EV_COPIES];
+  __shared__ int wsum[2][W], pick[3];
+  __shared__ int moves_s[INLINE ? 2 * EV_INLINE : 1];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = a.c.rows(a.SLOT[b]);
-  int* work = a.work + ((size_t)b * a.c.nkv + h) * (1 + 2 * (size_t)a.max_moves);
+  int* const work = INLINE ? nullptr : a.work + ((size_t)b * a.c.nkv + h) * (1 + 2 * (size_t)a.max_moves);
   if (n <= a.budget) {
-    if (tid == 0) work[0] = 0;
+    if (!INLINE && tid == 0) work[0] = 0;
     return;
   }
-  float* sc = a.c.scores + b * a.c.score_seq + h * a.c.score_head;
-  int* sp = a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head;
-  const long long pos = a.POS[b];
-  uint32_t prefix = 0;
-  int want = a.budget;  // how many of the keys that share the prefix are still kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  float* const sc = a.c.scores + b * a.c.score_seq + h * a.c.score_head;
+  int* const sp = a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head;
+  const long long newest = a.POS[b] - a.recent;
+  // wave w takes slots w * span .. + span - 1, 64 at a time
+  const int steps = (n + T - 1) / T, first = wave * steps * 64 + lane;
+  uint32_t held[R ? R : 1];
+  if constexpr (R != 0) {
+    constexpr int AT_ONCE = R < 8 ? R : 8;  // loads of a lane under way together
+#pragma unroll
+    for (int i0 = 0; i0 < R; i0 += AT_ONCE) {
+      if (i0 >= steps) break;
+      float f[AT_ONCE];
+      int p[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int j = min(first + 64 * (i0 + i), n - 1);
+        f[i] = sc[j], p[i] = sp[j];
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) held[i0 + i] = evict_key(f[i], p[i], a.sinks, newest);
+    }
+  }
+  // f(slot, key) for this lane's rows in order; false in `live` for lanes past the last row
+  auto each = [&](auto&& f) {
+    if constexpr (R != 0) {
+      int at = first;
+      asm("" : "+v"(at));  // slots worked out anew each time: kept, 64 of them would not fit beside the keys
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (i < steps) f(at + 64 * i, held[i], at + 64 * i < n);
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        const int j = first + 64 * i, r = min(j, n - 1);
+        f(j, evict_key(sc[r], sp[r], a.sinks, newest), j < n);
+      }
+    }
+  };
+
+  uint32_t limit = 0;   // the digits found so far, the rest 0
+  int want = a.budget;  // how many of the keys with these digits are still kept
+  bool whole = false;   // all of them
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int above = pass == 1 ? 21 : 10;  // (pass > 0) the bits found lie from here on
+    const uint32_t bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid * 4; i < EV_BINS * EV_COPIES; i += T * 4) *reinterpret_cast<u32x4*>(hist + i) = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
-    for (int j = tid; j < n; j += EV_T) {
-      const uint32_t k = evict_key(a, sc, sp, j, pos);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+    each([&](int, uint32_t k, bool live) {
+      if (live && (pass == 0 || (k >> above) == (limit >> above)))
+        atomicAdd(&hist[((k >> shift) & (bins - 1)) * EV_COPIES + (lane & (EV_COPIES - 1))], 1);
+    });
+    __syncthreads();
+    // thread t's bins, from the top: EV_BINS - 1 - PER t and the PER - 1 below it
+    int sum[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u32x4* c = reinterpret_cast<const u32x4*>(hist + (EV_BINS - 1 - PER * tid - i) * EV_COPIES);
+      const u32x4 x = c[0], y = c[1];
+      sum[i] = (int)(((x[0] + x[1]) + (x[2] + x[3])) + ((y[0] + y[1]) + (y[2] + y[3])));
+      mine += sum[i];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 63) wsum[0][wave] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < W; ++w) before += w < wave ? wsum[0][w] : 0;
+    if (before < want && before + mine >= want) {  // exactly one thread
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (before < want && before + sum[i] >= want) {
+          pick[0] = EV_BINS - 1 - PER * tid - i;
+          pick[1] = want - before;
+          pick[2] = sum[i];
+        }
+        before += sum[i];
+      }
     }
     __syncthreads();
-    if (tid == 0) {
-      int d = 255, left = want;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      pick[0] = d;
-      pick[1] = left;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)pick[0] << shift;
+    limit |= (uint32_t)pick[0] << shift;
     want = pick[1];
+    whole = pick[2] == want;
+    if (whole) break;
   }
-  // keys above `prefix` are kept, and the first `want` equal to it
-  int* src = work + 1;
-  int* dst = src + a.max_moves;
-  int equal = 0, movers = 0, holes = 0;
-  for (int j0 = 0; j0 < n; j0 += EV_T) {
-    const int j = j0 + tid;
-    const uint32_t k = j < n ? evict_key(a, sc, sp, j, pos) : 0;
-    int total;
-    const int eq = block_scan(j < n && k == prefix, scan_s, tid, &total);
-    const bool kept = j < n && (k > prefix || (k == prefix && equal + eq < want));
-    equal += total;
-    const bool mover = kept && j >= a.budget, hole = j < a.budget && !kept;
-    const int m = block_scan(mover, scan_s, tid, &total);
-    if (mover && movers + m < a.max_moves) src[movers + m] = j;
-    movers += total;
-    const int o = block_scan(hole, scan_s, tid, &total);
-    if (hole && holes + o < a.max_moves) dst[holes + o] = j;
-    holes += total;
+  // kept: keys above `limit` and the first `want` equal to it (`whole`: limit's
+  // lower digits are 0 and every key from it on is kept; it is not 0 then, as
+  // not all keys are kept)
+  if (whole) --limit, want = 0;
+
+  // rank of this wave's first key among the equal ones
+  auto count_waves = [&](int x, int y, int* xb, int* yb, int* xt) {  // uniform values a wave
+    __syncthreads();
+    if (lane == 0) wsum[0][wave] = x, wsum[1][wave] = y;
+    __syncthreads();
+    *xb = *yb = *xt = 0;
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) *xb += wsum[0][w], *yb += wsum[1][w];
+      *xt += wsum[0][w];
+    }
+  };
+  int equal = 0, unused, total;
+  if (!whole) {
+    int mine = 0;
+    each([&](int, uint32_t k, bool live) { mine += __popcll(__ballot(live && k == limit)); });
+    count_waves(mine, 0, &equal, &unused, &total);
   }
+  // lanes before this one
+  auto before_me = [&](uint64_t m) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  };
+  int rank = equal;
+  auto keeps = [&](uint32_t k, bool live) {
+    const bool eq = live && k == limit && !whole;
+    const uint64_t m = __ballot(eq);
+    const bool kept = live && (k > limit || (eq && rank + before_me(m) < want));
+    rank += __popcll(m);
+    return kept;
+  };
+  int movers = 0, holes = 0;
+  each([&](int j, uint32_t k, bool live) {
+    const bool kept = keeps(k, live);
+    movers += __popcll(__ballot(kept && j >= a.budget));
+    holes += __popcll(__ballot(live && !kept && j < a.budget));
+  });
+  int mb, hb;
+  count_waves(movers, holes, &mb, &hb, &total);  // as many holes as movers
+  int* const src = INLINE ? moves_s : work + 1;
+  const int room = INLINE ? EV_INLINE : a.max_moves;
+  int* const dst = src + room;
+  rank = equal;
+  each([&](int j, uint32_t k, bool live) {
+    const bool kept = keeps(k, live), mover = kept && j >= a.budget, hole = live && !kept && j < a.budget;
+    const uint64_t mm = __ballot(mover), hm = __ballot(hole);
+    const int mi = mb + before_me(mm), hi = hb + before_me(hm);
+    if (mover && mi < room) src[mi] = j;
+    if (hole && hi < room) dst[hi] = j;
+    mb += __popcll(mm);
+    hb += __popcll(hm);
+  });
+  const int moves = min(total, room);
+  if (!INLINE && tid == 0) work[0] = moves;
   __syncthreads();
-  const int moves = min(min(movers, holes), a.max_moves);  // all three are one number
-  if (tid == 0) work[0] = moves;
-  for (int i = tid; i < moves; i += EV_T) {
+  for (int i = tid; i < moves; i += T) {
     sc[dst[i]] = sc[src[i]];
     sp[dst[i]] = sp[src[i]];
   }
+  if constexpr (INLINE)
+    for (int i = tid / (D / 8); i < moves; i += T / (D / 8)) move_row<D>(a.c, b, h, src[i], dst[i], tid % (D / 8));
 }
 
 template <int D>
@@ -124,15 +234,32 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const EvictArgs a
   constexpr int LH = D / 8, ROWS = 256 / LH;
   const int h = blockIdx.y, b = blockIdx.z;
   const int* work = a.work + ((size_t)b * a.c.nkv + h) * (1 + 2 * (size_t)a.max_moves);
-  const int i = blockIdx.x * ROWS + (int)threadIdx.x / LH, e = (threadIdx.x % LH) * 8;
+  const int i = blockIdx.x * ROWS + (int)threadIdx.x / LH;
   if (i >= work[0]) return;
-  const int src = work[1 + i], dst = work[1 + a.max_moves + i], mask = (1 << a.c.shift) - 1;
-  const int from = a.c.page(b, src), to = a.c.page(b, dst);
-  if (from < 0 || to < 0) return;
-  *reinterpret_cast<u32x4*>(a.c.K + to * a.c.k_page + h * a.c.k_head + (dst & mask) * a.c.k_row + e) =
-      *reinterpret_cast<const u32x4*>(a.c.K + from * a.c.k_page + h * a.c.k_head + (src & mask) * a.c.k_row + e);
-  *reinterpret_cast<u32x4*>(a.c.V + to * a.c.v_page + h * a.c.v_head + (dst & mask) * a.c.v_row + e) =
-      *reinterpret_cast<const u32x4*>(a.c.V + from * a.c.v_page + h * a.c.v_head + (src & mask) * a.c.v_row + e);
+  move_row<D>(a.c, b, h, work[1 + i], work[1 + a.max_moves + i], threadIdx.x % LH);
+}
+
+template <int D>
+void launch_evict(const EvictArgs& a, hipStream_t stream) {
+  const dim3 grid(a.c.nkv, a.c.seqs);
+  const int cap = a.c.cap();
+#define TTSP_EV(TV, RV, INL) \
+  hipLaunchKernelGGL((paged_evict_select_kernel<TV, RV, D, INL>), grid, dim3(TV), 0, stream, a)
+  if (a.max_moves <= EV_INLINE) {
+    if (cap <= 256 * 8) TTSP_EV(256, 8, true);
+    else if (cap <= 1024 * 8) TTSP_EV(1024, 8, true);
+    else if (cap <= 1024 * 64) TTSP_EV(1024, 64, true);
+    else TTSP_EV(1024, 0, true);
+    return;
+  }
+  if (cap <= 256 * 8) TTSP_EV(256, 8, false);
+  else if (cap <= 1024 * 8) TTSP_EV(1024, 8, false);
+  else if (cap <= 1024 * 64) TTSP_EV(1024, 64, false);
+  else TTSP_EV(1024, 0, false);
+#undef TTSP_EV
+  const int rows = 256 / (D / 8);
+  hipLaunchKernelGGL(paged_evict_move_kernel<D>, dim3((a.max_moves + rows - 1) / rows, a.c.nkv, a.c.seqs), dim3(256), 0,
+                     stream, a);
 }
 
 }  // namespace ttsp
@@ -163,12 +290,8 @@ extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* 
   a.sinks = sinks;
   a.recent = recent;
   a.max_moves = (int)(budget < cap - budget ? budget : cap - budget);
-  a.hd = cache->head_dim;
   a.work = work;
-  hipLaunchKernelGGL(paged_evict_select_kernel, dim3(a.c.nkv, a.c.seqs), dim3(EV_T), 0, stream, a);
-  const int rows = 256 / (cache->head_dim / 8);
-  const dim3 grid((a.max_moves + rows - 1) / rows, a.c.nkv, a.c.seqs);
-  if (cache->head_dim == 128) hipLaunchKernelGGL(paged_evict_move_kernel<128>, grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL(paged_evict_move_kernel<64>, grid, dim3(256), 0, stream, a);
+  if (cache->head_dim == 128) launch_evict<128>(a, stream);
+  else launch_evict<64>(a, stream);
   TTSP_RETURN_LAUNCH();
 }
