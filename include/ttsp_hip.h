@@ -609,8 +609,8 @@ int ttsp_paged_store(const ttsp_paged_cache* cache, const void* K, long long k_r
                      const void* V, long long v_row_stride, long long v_head_stride, const long long* POS,
                      const int* SEQ, const long long* SLOT, int rows, void* stream);
 
-/* KiB of ttsp_paged_attention's workspace (host-only; -1: over 2 TiB);
- * tracked: the cache has scores. */
+/* KiB of ttsp_paged_attention's workspace (host-only; 0: none is needed, -1:
+ * over 2 TiB); tracked: the cache has scores. */
 int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size, int tracked);
 
 /* Attention of one new token per sequence over a paged cache: query (b, hd) at
@@ -619,14 +619,14 @@ int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int c
  * sequence b that lie in a page: Y[b][hd] = softmax(scale q . k) . v, zeros where
  * there is none (SLOT[b] < 0). With scores, the sum over the kv head's query
  * heads of the softmax weight of slot j is added to the score of slot j.
- * work: ttsp_paged_attention_work_kib() KiB, 16-byte aligned, which calls that
- * may overlap must not share; Q and Y are 16-byte aligned. Replaces: attn_partial
+ * work: ttsp_paged_attention_work_kib() KiB (0: may be NULL), 16-byte aligned,
+ * which calls that may overlap must not share; Q and Y are 16-byte aligned. Replaces: attn_partial
  * + attn_combine, app/engine/fusedlayer.py:95-159, for several sequences. */
 int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
                          const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
 
-/* KiB of ttsp_paged_evict's workspace (host-only; 0: no sequence can hold more
- * than the budget; -1: over 2 TiB). */
+/* KiB of ttsp_paged_evict's workspace (host-only; 0: none is needed, where no
+ * sequence can have more than 256 rows to move; -1: over 2 TiB). */
 int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int budget);
 
 /* Cut every sequence of more than `budget` rows (SLOT[b] + 1, int64) down to
@@ -639,7 +639,7 @@ int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int bu
  * then `budget` (the caller advances SLOT). sinks + recent <= budget. The
  * pages of such a sequence belong to it alone and have no holes below SLOT[b];
  * a row is not copied from or into a hole. work: ttsp_paged_evict_work_kib()
- * KiB, 4-byte aligned, which calls that may overlap must not share. Replaces:
+ * KiB (0: may be NULL), 4-byte aligned, which calls that may overlap must not share. Replaces:
  * nothing (the reference's cache is as long as its longest stream). */
 int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS, int budget,
                      int sinks, int recent, int* work, void* stream);

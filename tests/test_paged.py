@@ -25,6 +25,10 @@ def _cache(**kw):
     return _lib.PagedCache(**{**base, **kw})
 
 
+def _at(c):
+    return None if c is None else ctypes.byref(c)
+
+
 BAD_CACHES = [dict(K=None), dict(V=None), dict(table=None), dict(K=P + 8), dict(V=P + 2), dict(table=P + 1), dict(k_page=-8),
               dict(k_head=4), dict(v_row=129), dict(k_row=(1 << 24) + 8), dict(v_row=1 << 30), dict(table_stride=3), dict(seqs=0), dict(seqs=65536), dict(cols=0),
               dict(pages=0), dict(page_size=8), dict(page_size=24), dict(page_size=8192), dict(page_size=0), dict(n_kv=0),
@@ -36,26 +40,26 @@ BAD_CACHES = [dict(K=None), dict(V=None), dict(table=None), dict(K=P + 8), dict(
 def _rope(lib, c, **kw):
     a = dict(QKV=P, rs=1536, QW=P, KW=P, eps=1e-6, F=P, ftype=1, n=10, POS=P, SEQ=P, SLOT=P, Q=P, nh=4, rows=3, **{})
     a.update(kw)
-    return lib.ttsp_paged_qk_rope_kv(c, *(a[k] for k in ("QKV", "rs", "QW", "KW", "eps", "F", "ftype", "n", "POS", "SEQ",
+    return lib.ttsp_paged_qk_rope_kv(_at(c), *(a[k] for k in ("QKV", "rs", "QW", "KW", "eps", "F", "ftype", "n", "POS", "SEQ",
                                                          "SLOT", "Q", "nh", "rows")), None)
 
 
 def _store(lib, c, **kw):
     a = dict(K=P, krs=512, khs=128, V=P, vrs=512, vhs=128, POS=P, SEQ=P, SLOT=P, rows=3)
     a.update(kw)
-    return lib.ttsp_paged_store(c, *a.values(), None)
+    return lib.ttsp_paged_store(_at(c), *a.values(), None)
 
 
 def _attention(lib, c, **kw):
     a = dict(Q=P, qs=1024, SLOT=P, Y=P, nh=8, scale=0.1, work=P)
     a.update(kw)
-    return lib.ttsp_paged_attention(c, *a.values(), None)
+    return lib.ttsp_paged_attention(_at(c), *a.values(), None)
 
 
 def _evict(lib, c, **kw):
     a = dict(SLOT=P, POS=P, budget=20, sinks=2, recent=3, work=P)
     a.update(kw)
-    return lib.ttsp_paged_evict(c, *a.values(), None)
+    return lib.ttsp_paged_evict(_at(c), *a.values(), None)
 
 
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda b: next(iter(b)) + str(next(iter(b.values()))))
@@ -80,11 +84,17 @@ def test_bad_arguments_are_refused_before_any_launch():
                dict(POS=None), dict(SEQ=None), dict(SLOT=None), dict(rows=-2), dict(rows=1 << 25)):
         assert _store(lib, c, **kw) == 1, kw
     for kw in (dict(Q=None), dict(Q=P + 2), dict(qs=1023), dict(qs=1016), dict(SLOT=None), dict(Y=None), dict(Y=P + 8), dict(nh=0),
-               dict(nh=6), dict(nh=65540), dict(work=None), dict(work=P + 4)):
+               dict(nh=6), dict(nh=65540)):
         assert _attention(lib, c, **kw) == 1, kw
+    for big in (_cache(cols=100, table_stride=100, scores=None), c):  # partial sums, or scores to gather
+        for kw in (dict(work=None), dict(work=P + 4)):
+            assert _attention(lib, big, **kw) == 1, kw
     for kw in (dict(SLOT=None), dict(POS=None), dict(budget=0), dict(budget=-3), dict(sinks=-1), dict(recent=-1),
-               dict(sinks=10, recent=11), dict(sinks=2**31 - 1, recent=2**31 - 1), dict(work=None), dict(work=P + 2)):
+               dict(sinks=10, recent=11), dict(sinks=2**31 - 1, recent=2**31 - 1)):
         assert _evict(lib, c, **kw) == 1, kw
+    wide = _cache(cols=100, table_stride=100)
+    for kw in (dict(work=None, budget=800), dict(work=P + 2, budget=800)):
+        assert _evict(lib, wide, **kw) == 1, kw
     assert _evict(lib, _cache(scores=None)) == 1 and _evict(lib, _cache(slot_pos=None)) == 1
     # nothing to do: no launch either
     assert _rope(lib, c, rows=0) == 0 and _store(lib, c, rows=0) == 0
@@ -98,8 +108,8 @@ def test_workspace_queries():
     assert lib.ttsp_paged_attention_work_kib(65535, 4096, 1, 128, 1 << 20, 16, 1) == -1
     with pytest.raises(ValueError):
         pc.attention_work(65535, 4096, 1, 128, 1 << 20, 16, True)
-    assert pc.evict_work(3, 2, 4, 16, 64) == 0 and pc.evict_work(3, 2, 4, 16, 63) >= 3 * 2 * 3
-    assert pc.evict_work(1, 1, 100, 16, 100) >= 201
+    assert pc.evict_work(3, 2, 4, 16, 64) == 0 and pc.evict_work(3, 2, 4, 16, 20) == 0
+    assert pc.evict_work(3, 2, 100, 16, 1300) >= 3 * 2 * (1 + 2 * 300) and pc.evict_work(1, 1, 100, 16, 257) >= 515
     assert lib.ttsp_paged_evict_work_kib(65535, 4096, 1 << 20, 16, 1 << 23) == -1
 
 
@@ -146,6 +156,9 @@ def test_the_argument_block_matches_the_header(tmp_path):
     exe = tmp_path / "layout"
     subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert pc._BLOCK.size == ctypes.sizeof(_lib.PagedCache)  # the calls pack the block by itself
+    block = _lib.PagedCache.from_buffer_copy(pc._BLOCK.pack(*range(1, len(names) + 1)))
+    assert [getattr(block, n) for n in names] == list(range(1, len(names) + 1))
     assert got == [getattr(_lib.PagedCache, n).offset for n in names] + [ctypes.sizeof(_lib.PagedCache), _lib.PAGED_MAX_SLOTS]
 
 

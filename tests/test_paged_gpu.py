@@ -409,6 +409,27 @@ def test_evict_of_long_sequences(n, budget, kind):
     _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=4, recent=64)
 
 
+@pytest.mark.parametrize("cap", [1056, 8192, 20000, 70000])
+@pytest.mark.parametrize("kind", ["exp", "few", "same", "every"])
+def test_evict_of_a_few_rows(cap, kind):
+    """1 to 6 rows over the budget, in every ranking variant."""
+    budget = cap - 20
+    lens = [budget + i for i in range(7)]
+    c, s, sp = _tracked(lens, 2, 64, 16, BF, seed=cap, kind=kind, cols=-(-cap // 16))
+    _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=8)
+
+
+def test_evict_of_the_newest_rows_themselves():
+    """The lowest keys past the budget: nothing moves, or only what stays of them."""
+    c, s, sp = _tracked([104, 103, 102, 101], 2, 128, 16, FP, seed=34, cols=8)
+    s[:, :, 100:] = -1.0
+    assert _evict(c, s, sp, sp.amax((1, 2)).long() + 1000, 100) == 0
+    s[:, :, 101:103] = 10.0
+    s[:, :, 103] = -2.0
+    s[:, :, 7], s[:, :, 55] = -3.0, -4.0
+    assert _evict(c, s, sp, sp.amax((1, 2)).long() + 1000, 100) > 0
+
+
 def test_evict_leaves_short_sequences_and_wide_budgets_alone():
     c, s, sp = _tracked([50, 0, 64], 2, 64, 16, FP, seed=30)
     pos = sp.amax((1, 2)).long()
@@ -538,8 +559,13 @@ def test_calls_that_raise():
         if need:
             with pytest.raises(ValueError):
                 pc.attention(c.q, *c.pools(), c.slots, work=work)
-    with pytest.raises(ValueError):
-        pc.evict(*c.pools(), c.slots, c.scores, sp, c.slots, 20, work=torch.empty(0, dtype=torch.int32, device="cuda"))
+    w = Case([900, 40], 2, 2, 64, 16, BF, seed=41)
+    wp = torch.zeros(w.scores.shape, dtype=torch.int32, device="cuda")
+    need = pc.evict_work(2, 2, w.table.shape[1], 16, 400)
+    for work in (torch.empty(0, dtype=torch.int32, device="cuda"), torch.empty(need, device="cuda"),
+                 torch.empty(need, dtype=torch.int32), torch.empty(need - 1, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            pc.evict(*w.pools(), w.slots, w.scores, wp, w.slots, 400, work=work)
     with pytest.raises(ValueError):
         pc.qk_rope_kv(torch.zeros(2, 12 * 128, dtype=BF, device="cuda"), 8, *c.pools(), c.slots, _freqs(64, 128), c.slots,
                       out=torch.empty(2, 8, 64, dtype=BF, device="cuda"))

@@ -131,13 +131,14 @@ SIGNATURES: dict[str, list] = {
                         _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp],
     "ttsp_fast_steps_grid": [_i, _i, _i, _i, _i, _i, _i, _i],
     "ttsp_fast_steps_work_bytes": [_i, _i, _i, _i],
-    "ttsp_paged_qk_rope_kv": [ctypes.POINTER(PagedCache), _vp, _ll, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp, _vp, _i,
+    # (a paged cache: the address of a PagedCache, or its bytes)
+    "ttsp_paged_qk_rope_kv": [_vp, _vp, _ll, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp, _vp, _i,
                               _i, _vp],
-    "ttsp_paged_store": [ctypes.POINTER(PagedCache), _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _vp],
+    "ttsp_paged_store": [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _vp],
     "ttsp_paged_attention_work_kib": [_i, _i, _i, _i, _i, _i, _i],
-    "ttsp_paged_attention": [ctypes.POINTER(PagedCache), _vp, _ll, _vp, _vp, _i, _f, _vp, _vp],
+    "ttsp_paged_attention": [_vp, _vp, _ll, _vp, _vp, _i, _f, _vp, _vp],
     "ttsp_paged_evict_work_kib": [_i, _i, _i, _i, _i],
-    "ttsp_paged_evict": [ctypes.POINTER(PagedCache), _vp, _vp, _i, _i, _i, _vp, _vp],
+    "ttsp_paged_evict": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
 }
 
 

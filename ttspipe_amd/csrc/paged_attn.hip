@@ -45,6 +45,7 @@ typedef __attribute__((address_space(3))) pg_s16x4 pg_lds_s16x4;
 constexpr int PG_WAVES = 4, PG_KEYS = 32;      // waves a workgroup, keys a wave takes at once
 constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of this
 constexpr int PG_WGS = 1024;                   // workgroups the chunks are meant to make
+constexpr int PG_SHORT = 512;                  // caches of up to this many slots: a sequence is one chunk
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 
@@ -59,7 +60,7 @@ struct AttnArgs {
   float* PACC;   // [chunks][nh][D]: its sum of exp2(s - reference) v
   float* S;      // scores in log2 units [seqs][nh][cap] (with scores to gather)
   float scale2;  // scale * log2(e)
-  int nh, seqs, chunks, target;  // chunks: at most; target: chunks that fill the GPU
+  int nh, seqs, target;  // target: chunks that fill the GPU (0: chunk b is the whole sequence b)
 };
 
 template <int DT>
@@ -122,6 +123,10 @@ __device__ __forceinline__ int chunk_len(const AttnArgs& a, int lane) {
 
 // Every wave finds it by itself; the result is uniform.
 __device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int lane) {
+  if (a.target == 0) {
+    const int n = a.c.rows(a.SLOT[gx]);
+    return Chunk{gx, n, 0, 1, gx, n};
+  }
   const int len = chunk_len(a, lane);
   int before = 0;
   for (int b0 = 0; b0 < a.seqs; b0 += 64) {
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   const int h = blockIdx.y / hgs, head0 = h * group + (blockIdx.y % hgs) * PG_HEADS;
   const int heads = min(PG_HEADS, (h + 1) * group - head0);
   const Chunk ck = find_chunk(a, blockIdx.x, lane);
-  if (ck.b < 0) return;
+  if (ck.b < 0) return;  // (a sequence without a row is no chunk, or with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   const int mask = (1 << a.c.shift) - 1;
@@ -487,13 +492,17 @@ inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, bool tra
   p->hgs = (group + PG_HEADS - 1) / PG_HEADS;
   const long long wide = (long long)nkv * p->hgs;
   p->target = (int)(wide < PG_WGS ? PG_WGS / wide : 1);
+  p->parts = p->scores = 0;
+  const bool one = cap <= PG_SHORT;
+  if (one) p->target = 0;
   // a sequence adds at most one partly filled chunk to those the rows fill
   const long long most = (long long)seqs * ((cap + PG_STEP - 1) / PG_STEP);
   const long long chunks = p->target + (long long)seqs;
-  p->chunks = (int)(most < chunks ? most : chunks);
-  p->parts = (((size_t)p->chunks * nh * (2 + hd)) + 3) / 4 * 4;
+  p->chunks = one ? seqs : (int)(most < chunks ? most : chunks);
+  // several workgroups of a kv head leave their sums for the gathering launch even so
+  if (!one || (tracked && p->hgs > 1)) p->parts = (((size_t)p->chunks * nh * (2 + hd)) + 3) / 4 * 4;
   p->scores = tracked ? (size_t)seqs * nh * cap : 0;
-  return (p->parts + p->scores) / 256 + 1 <= 0x7fffffff;
+  return (p->parts + p->scores + 255) / 256 <= 0x7fffffff;
 }
 
 }  // namespace ttsp
@@ -513,14 +522,15 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
                                     hipStream_t stream) {
   AttnArgs a{};
   AttnPlan p;
-  if (!paged_args(cache, &a.c) || !Q || !SLOT || !Y || !work || nh < 1 || nh > 65535 || nh % a.c.nkv ||
-      (uintptr_t)Q % 16 || (uintptr_t)Y % 16 || (uintptr_t)work % 16 || q_seq_stride % 8 ||
+  if (!paged_args(cache, &a.c) || !Q || !SLOT || !Y || nh < 1 || nh > 65535 || nh % a.c.nkv ||
+      (uintptr_t)Q % 16 || (uintptr_t)Y % 16 || q_seq_stride % 8 ||
       q_seq_stride < (long long)nh * cache->head_dim)
     return (int)hipErrorInvalidValue;
   const int hd = cache->head_dim;
   const bool tracked = a.c.scores != nullptr;
   if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p) || (long long)a.c.nkv * p.hgs > 65535)
     return (int)hipErrorInvalidValue;
+  if (p.parts + p.scores && (!work || (uintptr_t)work % 16)) return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;
   a.q_seq = q_seq_stride;
   a.SLOT = SLOT;
@@ -532,14 +542,13 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
   a.scale2 = scale * 1.4426950408889634f;
   a.nh = nh;
   a.seqs = a.c.seqs;
-  a.chunks = p.chunks;
   a.target = p.target;
   const dim3 grid(p.chunks, a.c.nkv * p.hgs);
 #define TTSP_PATT(DTV, DV)                                                                                       \
   do {                                                                                                           \
     if (tracked) hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, true>), grid, dim3(64 * PG_WAVES), 0, stream, a); \
     else hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, false>), grid, dim3(64 * PG_WAVES), 0, stream, a);        \
-    hipLaunchKernelGGL((paged_join_kernel<DTV, DV>), dim3(nh, a.seqs), dim3(256), 0, stream, a);                  \
+    if (p.target) hipLaunchKernelGGL((paged_join_kernel<DTV, DV>), dim3(nh, a.seqs), dim3(256), 0, stream, a);    \
   } while (0)
   if (cache->dtype == DT_F16) {
     if (hd == 128) TTSP_PATT(DT_F16, 128);
@@ -549,6 +558,6 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
     else TTSP_PATT(DT_BF16, 64);
   }
 #undef TTSP_PATT
-  if (tracked) hipLaunchKernelGGL(paged_gather_kernel, dim3(p.chunks, a.c.nkv), dim3(256), 0, stream, a);
+  if (tracked && (p.target || p.hgs > 1)) hipLaunchKernelGGL(paged_gather_kernel, dim3(p.chunks, a.c.nkv), dim3(256), 0, stream, a);
   TTSP_RETURN_LAUNCH();
 }

@@ -18,7 +18,10 @@
 // neighbouring slots, so that ranks among equal keys, movers and free slots are
 // counted with ballots and one prefix over the waves each. A second launch
 // moves the K and V rows, a group of lanes each; where the cache has little room
-// past the budget (a step that evicts one row) the first moves them itself.
+// past the budget the first moves them itself. A sequence only a few rows over
+// its budget, as after a decode step, has its lowest keys taken out one by one
+// instead, while the rows past the budget, which may have to move, are on
+// their way already.
 #include "paged_common.h"
 
 namespace ttsp {
@@ -34,6 +37,8 @@ struct EvictArgs {
 constexpr int EV_BINS = 2048, EV_COPIES = 8;
 // At most this many rows a (sequence, kv head) are moved by the ranking workgroup itself.
 constexpr int EV_INLINE = 256;
+// Rows over the budget up to which the lowest are taken out one by one.
+constexpr int EV_FEW = 4;
 
 // Larger keys are larger integers; -0 and +0 are one key.
 __device__ __forceinline__ uint32_t order_of(float f) {
@@ -48,15 +53,24 @@ __device__ __forceinline__ uint32_t evict_key(float f, int p, int sinks, long lo
   return order_of(f != f ? __uint_as_float(0xff800000u) : f);
 }
 
-// One row (K and V) from slot src to slot dst of sequence b, head h, by D / 8 lanes.
-template <int D>
+// A row's K and V, eight elements a lane (D / 8 lanes a row).
+struct Row {
+  u32x4 k, v;
+};
+// Slot j's row of sequence b, head h, in `page` (not a hole).
+__device__ __forceinline__ Row load_row(const Paged& c, int page, int h, int j, int lane) {
+  const int row = j & ((1 << c.shift) - 1), e = lane * 8;
+  return Row{*reinterpret_cast<const u32x4*>(c.K + page * c.k_page + h * c.k_head + row * c.k_row + e),
+             *reinterpret_cast<const u32x4*>(c.V + page * c.v_page + h * c.v_head + row * c.v_row + e)};
+}
+__device__ __forceinline__ void store_row(const Paged& c, int page, int h, int j, int lane, const Row& r) {
+  const int row = j & ((1 << c.shift) - 1), e = lane * 8;
+  *reinterpret_cast<u32x4*>(c.K + page * c.k_page + h * c.k_head + row * c.k_row + e) = r.k;
+  *reinterpret_cast<u32x4*>(c.V + page * c.v_page + h * c.v_head + row * c.v_row + e) = r.v;
+}
 __device__ __forceinline__ void move_row(const Paged& c, int b, int h, int src, int dst, int lane) {
-  const int from = c.page(b, src), to = c.page(b, dst), mask = (1 << c.shift) - 1, e = lane * 8;
-  if (from < 0 || to < 0) return;
-  const u32x4 k = *reinterpret_cast<const u32x4*>(c.K + from * c.k_page + h * c.k_head + (src & mask) * c.k_row + e);
-  const u32x4 v = *reinterpret_cast<const u32x4*>(c.V + from * c.v_page + h * c.v_head + (src & mask) * c.v_row + e);
-  *reinterpret_cast<u32x4*>(c.K + to * c.k_page + h * c.k_head + (dst & mask) * c.k_row + e) = k;
-  *reinterpret_cast<u32x4*>(c.V + to * c.v_page + h * c.v_head + (dst & mask) * c.v_row + e) = v;
+  const int from = c.page(b, src), to = c.page(b, dst);
+  if (from >= 0 && to >= 0) store_row(c, to, h, dst, lane, load_row(c, from, h, src, lane));
 }
 
 // T threads; R: keys a thread holds (0: read again in every pass).
@@ -77,6 +91,16 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
   float* const sc = a.c.scores + b * a.c.score_seq + h * a.c.score_head;
   int* const sp = a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head;
   const long long newest = a.POS[b] - a.recent;
+  const bool few = INLINE && R != 0 && n - a.budget <= EV_FEW;
+  constexpr int LH = D / 8;
+  // few: group g of LH lanes holds the row of slot budget + g
+  const int over = a.budget + tid / LH;
+  Row row{};
+  int row_page = -1;
+  if (few && over < n) {
+    row_page = a.c.page(b, over);
+    if (row_page >= 0) row = load_row(a.c, row_page, h, over, tid % LH);
+  }
   // wave w takes slots w * span .. + span - 1, 64 at a time
   const int steps = (n + T - 1) / T, first = wave * steps * 64 + lane;
   uint32_t held[R ? R : 1];
@@ -94,6 +118,62 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
       }
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) held[i0 + i] = evict_key(f[i], p[i], a.sinks, newest);
+    }
+  }
+  if constexpr (INLINE && R != 0) {
+    if (few) {
+      __shared__ unsigned long long low_s[EV_FEW][W];
+      int out[EV_FEW];  // the slots taken out
+#pragma unroll
+      for (int r = 0; r < EV_FEW; ++r) {
+        out[r] = 0x7fffffff;
+        if (r >= n - a.budget) continue;
+        // the lowest key, of equal ones the highest slot's; ~0: none of this lane's
+        unsigned long long low = ~0ull;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int j = first + 64 * i;
+          bool live = i < steps && j < n;
+#pragma unroll
+          for (int q = 0; q < r; ++q) live = live && j != out[q];
+          if (live) low = min(low, (unsigned long long)held[i] << 32 | (uint32_t)~j);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) low = min(low, (unsigned long long)__shfl_xor((long long)low, o, 64));
+        if (lane == 0) low_s[r][wave] = low;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) low = min(low, low_s[r][w]);
+        out[r] = (int)~(uint32_t)low;
+      }
+      // this group's slot moves if it stays: to the hole of its rank among the movers
+      if (over >= n) return;
+      int rank = 0, dst = -1;
+      bool stays = true;
+#pragma unroll
+      for (int r = 0; r < EV_FEW; ++r) stays = stays && out[r] != over;
+#pragma unroll
+      for (int q = 0; q < EV_FEW; ++q) {
+        bool kept = a.budget + q < over;
+#pragma unroll
+        for (int r = 0; r < EV_FEW; ++r) kept = kept && out[r] != a.budget + q;
+        rank += kept;
+      }
+#pragma unroll
+      for (int r = 0; r < EV_FEW; ++r) {
+        int below = 0;
+#pragma unroll
+        for (int q = 0; q < EV_FEW; ++q) below += out[q] < out[r];
+        if (below == rank && out[r] < a.budget) dst = out[r];
+      }
+      if (!stays || dst < 0) return;
+      const int to = a.c.page(b, dst);
+      if (row_page >= 0 && to >= 0) store_row(a.c, to, h, dst, tid % LH, row);
+      if (tid % LH == 0) {
+        sc[dst] = sc[over];
+        sp[dst] = sp[over];
+      }
+      return;
     }
   }
   // f(slot, key) for this lane's rows in order; false in `live` for lanes past the last row
@@ -226,7 +306,7 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
     sp[dst[i]] = sp[src[i]];
   }
   if constexpr (INLINE)
-    for (int i = tid / (D / 8); i < moves; i += T / (D / 8)) move_row<D>(a.c, b, h, src[i], dst[i], tid % (D / 8));
+    for (int i = tid / (D / 8); i < moves; i += T / (D / 8)) move_row(a.c, b, h, src[i], dst[i], tid % (D / 8));
 }
 
 template <int D>
@@ -236,7 +316,7 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const EvictArgs a
   const int* work = a.work + ((size_t)b * a.c.nkv + h) * (1 + 2 * (size_t)a.max_moves);
   const int i = blockIdx.x * ROWS + (int)threadIdx.x / LH;
   if (i >= work[0]) return;
-  move_row<D>(a.c, b, h, work[1 + i], work[1 + a.max_moves + i], threadIdx.x % LH);
+  move_row(a.c, b, h, work[1 + i], work[1 + a.max_moves + i], threadIdx.x % LH);
 }
 
 template <int D>
@@ -271,6 +351,7 @@ extern "C" int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_s
   const long long cap = (long long)cols * page_size;
   if (cap <= budget) return 0;
   const long long moves = budget < cap - budget ? budget : cap - budget;
+  if (moves <= EV_INLINE) return 0;
   const long long kib = ((long long)seqs * nkv * (1 + 2 * moves) * 4 + 1023) / 1024;
   return kib > 0x7fffffffLL ? -1 : (int)kib;
 }
@@ -283,13 +364,13 @@ extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* 
     return (int)hipErrorInvalidValue;
   const long long cap = a.c.cap();
   if (cap <= budget) return 0;  // no table row holds more than the budget
-  if (!work || (uintptr_t)work % 4) return (int)hipErrorInvalidValue;
   a.SLOT = SLOT;
   a.POS = POS;
   a.budget = budget;
   a.sinks = sinks;
   a.recent = recent;
   a.max_moves = (int)(budget < cap - budget ? budget : cap - budget);
+  if (a.max_moves > EV_INLINE && (!work || (uintptr_t)work % 4)) return (int)hipErrorInvalidValue;
   a.work = work;
   if (cache->head_dim == 128) launch_evict<128>(a, stream);
   else launch_evict<64>(a, stream);

@@ -33,6 +33,9 @@ nothing is allocated, so that calls can be captured. Calls that may overlap
 
 from __future__ import annotations
 
+import functools
+import struct
+
 import torch
 from torch import nn
 
@@ -53,64 +56,82 @@ def _declined():
     _stats["declined"] += 1
 
 
+#: `ttsp_paged_cache`'s fields in order (`_lib.PagedCache` names them).
+_BLOCK = struct.Struct("@5P11q7i4x")
+
+
+def _strides_ok(s, nkv, pages, hd) -> bool:
+    return (s[3] == 1 and not (s[0] % 8 or s[1] % 8 or s[2] % 8) and hd <= s[2] <= _lib.PAGED_MAX_ROW_STRIDE
+            and (nkv == 1 or s[1] >= hd) and (pages == 1 or s[0] >= hd))
+
+
 def _pool(k_pages, v_pages, block_table, scores=None, slot_pos=None):
-    """The C-ABI's view of these tensors, or None where the kernels do not take them."""
-    dev = k_pages.device
-    if dev.type != "cuda" or v_pages.device != dev or block_table.device != dev:
+    """(the C-ABI's argument block, n_kv, page size, head dim, sequences, columns,
+    the cache's dtype, its device's index) of these tensors, or None where the
+    kernels do not take them. On every call's host path: plain integers, each
+    tensor asked for a thing once."""
+    dev, dtype, shape, table = k_pages.get_device(), k_pages.dtype, k_pages.shape, block_table.shape
+    if dtype is torch.bfloat16:
+        dt = _lib.DT_BF16
+    elif dtype is torch.float16:
+        dt = _lib.DT_F16
+    else:
         return None
-    dt = _lib.dtype_code(k_pages.dtype)
-    if dt not in (_lib.DT_F16, _lib.DT_BF16) or v_pages.dtype != k_pages.dtype or block_table.dtype != torch.int32:
-        return None
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or block_table.dim() != 2:
+    if (dev < 0 or v_pages.get_device() != dev or block_table.get_device() != dev or v_pages.dtype is not dtype
+            or block_table.dtype is not torch.int32 or len(shape) != 4 or len(table) != 2 or v_pages.shape != shape):
         return None
     pages, nkv, page, hd = shape
-    seqs, cols = block_table.shape
+    seqs, cols = table
     if (hd not in HEAD_DIMS or not MIN_PAGE <= page <= MAX_PAGE or page & (page - 1) or not pages or not 1 <= nkv <= 4096
             or not 1 <= seqs <= 65535 or not 1 <= cols <= _lib.PAGED_MAX_SLOTS // page):
         return None
-    ks, vs, ts = k_pages.stride(), v_pages.stride(), block_table.stride()
-    for s in (ks, vs):
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or not hd <= s[2] <= _lib.PAGED_MAX_ROW_STRIDE or (nkv > 1 and s[1] < hd) or (
-                pages > 1 and s[0] < hd):
-            return None
-    if ts[1] != 1 and cols > 1 or (seqs > 1 and ts[0] < cols):
+    ks, vs, (t0, t1) = k_pages.stride(), v_pages.stride(), block_table.stride()
+    if not _strides_ok(ks, nkv, pages, hd) or (vs != ks and not _strides_ok(vs, nkv, pages, hd)):
         return None
     kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
-    if kp % 16 or vp % 16:
+    if kp % 16 or vp % 16 or (t1 != 1 and cols > 1) or (seqs > 1 and t0 < cols):
         return None
-    extra, strides = [], []
-    for t, dtype in ((scores, torch.float32), (slot_pos, torch.int32)):
-        if t is None:
-            extra.append(None)
-            strides += (0, 0)
-            continue
-        if t.dtype != dtype or t.device != dev or t.shape != (seqs, nkv, cols * page):
+    scp = spp = sc0 = sc1 = sp0 = sp1 = 0
+    cap = cols * page
+    if scores is not None:
+        if scores.dtype is not torch.float32 or scores.get_device() != dev or scores.shape != (seqs, nkv, cap):
             return None
-        st = t.stride()
-        if st[2] != 1 or (seqs > 1 and st[0] < cols * page) or (nkv > 1 and st[1] < cols * page):
+        sc0, sc1, last = scores.stride()
+        if last != 1 or (seqs > 1 and sc0 < cap) or (nkv > 1 and sc1 < cap):
             return None
-        extra.append(t.data_ptr())
-        strides += (max(st[0], 1), st[1])
-    return _lib.PagedCache(kp, vp, block_table.data_ptr(), *extra, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                           max(ts[0], cols), *strides, seqs, cols, pages, page, nkv, hd, dt)
+        scp = scores.data_ptr()
+    if slot_pos is not None:
+        if slot_pos.dtype is not torch.int32 or slot_pos.get_device() != dev or slot_pos.shape != (seqs, nkv, cap):
+            return None
+        sp0, sp1, last = slot_pos.stride()
+        if last != 1 or (seqs > 1 and sp0 < cap) or (nkv > 1 and sp1 < cap):
+            return None
+        spp = slot_pos.data_ptr()
+    block = _BLOCK.pack(kp, vp, block_table.data_ptr(), scp, spp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                        t0 if t0 > cols else cols, sc0 or 1, sc1, sp0 or 1, sp1, seqs, cols, pages, page, nkv, hd, dt)
+    return block, nkv, page, hd, seqs, cols, dtype, dev
 
 
 def _vector(t, dtype, n, dev) -> bool:
     """Whether `t` is a contiguous vector of n values of `dtype` on `dev`."""
-    return t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.device == dev and (n < 2 or t.stride(0) == 1)
+    return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.get_device() == dev
 
 
 def _launch(what, dev, *args):
-    """`what` of the library on the current stream of `dev`."""
+    """`what` of the library on the current stream of device `dev`."""
     fn = getattr(_lib.lib(), what)
-    if dev.index == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(*args, _lib.stream())
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _lib.stream())
     if rc:
         raise RuntimeError(f"{what} failed: hipError_t {rc}")
+
+
+def _out_ok(out, shape, dtype, dev) -> bool:
+    return (out.shape == shape and out.dtype is dtype and out.get_device() == dev and out.is_contiguous()
+            and not out.data_ptr() % 16)
 
 
 def _rows_ok(rows, seqs_of, slots, positions, seqs, dev) -> bool:
@@ -141,30 +162,35 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
     c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
     if c is None or qkv.dim() != 2:
         return _declined()
-    dev, hd, dtype = k_pages.device, c.head_dim, k_pages.dtype
+    block, nkv, _, hd, n_seqs, _, dtype, dev = c
     rows, width = qkv.shape
-    ftype = _lib.dtype_code(freqs_cis.dtype)
-    if (n_head < 1 or width != (n_head + 2 * c.n_kv) * hd or qkv.dtype != dtype or qkv.device != dev
-            or qkv.stride(1) != 1 or (rows > 1 and (qkv.stride(0) < width or qkv.stride(0) % 8)) or qkv.data_ptr() % 16
-            or ftype is None or freqs_cis.device != dev or freqs_cis.dim() != 3 or freqs_cis.shape[1:] != (hd // 2, 2)
-            or not freqs_cis.is_contiguous() or freqs_cis.data_ptr() % 16 or not freqs_cis.shape[0]
-            or freqs_cis.shape[0] >= 1 << 31 or not _rows_ok(rows, seqs, slots, positions, c.seqs, dev)):
+    step, last = qkv.stride()
+    n_freqs, ftype = freqs_cis.shape[0] if freqs_cis.dim() == 3 else 0, _lib.dtype_code(freqs_cis.dtype)
+    qp, fp = qkv.data_ptr(), freqs_cis.data_ptr()
+    if (n_head < 1 or width != (n_head + 2 * nkv) * hd or qkv.dtype is not dtype or qkv.get_device() != dev or last != 1
+            or (rows > 1 and (step < width or step % 8)) or qp % 16 or ftype is None or freqs_cis.get_device() != dev
+            or not 0 < n_freqs < 1 << 31 or freqs_cis.shape != (n_freqs, hd // 2, 2) or not freqs_cis.is_contiguous()
+            or fp % 16 or not _rows_ok(rows, seqs, slots, positions, n_seqs, dev)):
         return _declined()
-    if positions is None and (freqs_cis.shape[0] < rows or slot_pos is not None):
+    if positions is None and (n_freqs < rows or slot_pos is not None):
         return _declined()
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != dtype or w.device != dev or w.shape != (hd,) or w.stride(0) != 1
-                              or w.data_ptr() % 16):
+    qw = kw = 0
+    if q_weight is not None:
+        qw = q_weight.data_ptr()
+        if not _out_ok(q_weight, (hd,), dtype, dev):
+            return _declined()
+    if k_weight is not None:
+        kw = k_weight.data_ptr()
+        if not _out_ok(k_weight, (hd,), dtype, dev):
             return _declined()
     if out is None:
-        out = torch.empty(rows, n_head, hd, dtype=dtype, device=dev)
-    elif (out.shape != (rows, n_head, hd) or out.dtype != dtype or out.device != dev or not out.is_contiguous()
-          or out.data_ptr() % 16):
+        out = torch.empty((rows, n_head, hd), dtype=dtype, device=qkv.device)
+    elif not _out_ok(out, (rows, n_head, hd), dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (rows, n_head, head_dim) tensor of the cache's dtype")
     if rows:
-        _launch("ttsp_paged_qk_rope_kv", dev, c, qkv.data_ptr(), max(qkv.stride(0), width) if rows > 1 else width,
-                _lib.ptr(q_weight), _lib.ptr(k_weight), eps, freqs_cis.data_ptr(), ftype, freqs_cis.shape[0],
-                _lib.ptr(positions), _lib.ptr(seqs), slots.data_ptr(), out.data_ptr(), n_head, rows)
+        _launch("ttsp_paged_qk_rope_kv", dev, block, qp, step if rows > 1 else width, qw, kw, eps, fp, ftype, n_freqs,
+                0 if positions is None else positions.data_ptr(), 0 if seqs is None else seqs.data_ptr(),
+                slots.data_ptr(), out.data_ptr(), n_head, rows)
         _stats["rows"] += 1
     return out
 
@@ -177,24 +203,27 @@ def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=No
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
-    if c is None or k.dim() != 3 or v.shape != k.shape:
+    shape = k.shape
+    if c is None or len(shape) != 3 or v.shape != shape:
         return _declined()
-    dev, rows = k_pages.device, k.shape[0]
-    if k.shape[1:] != (c.n_kv, c.head_dim) or not _rows_ok(rows, seqs, slots, positions, c.seqs, dev):
+    block, nkv, _, hd, n_seqs, _, dtype, dev = c
+    rows = shape[0]
+    if (shape[1] != nkv or shape[2] != hd or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != dev
+            or v.get_device() != dev or not _rows_ok(rows, seqs, slots, positions, n_seqs, dev)
+            or (slot_pos is not None and positions is None)):
         return _declined()
-    if slot_pos is not None and positions is None:
+    (kr, kh, kl), (vr, vh, vl) = k.stride(), v.stride()
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if kl != 1 or vl != 1 or kr % 8 or kh % 8 or vr % 8 or vh % 8 or kp % 16 or vp % 16:
         return _declined()
-    for t in (k, v):
-        if (t.dtype != k_pages.dtype or t.device != dev or t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8
-                or t.data_ptr() % 16):
-            return _declined()
     if rows:
-        _launch("ttsp_paged_store", dev, c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                v.stride(1), _lib.ptr(positions), _lib.ptr(seqs), slots.data_ptr(), rows)
+        _launch("ttsp_paged_store", dev, block, kp, kr, kh, vp, vr, vh, 0 if positions is None else positions.data_ptr(),
+                0 if seqs is None else seqs.data_ptr(), slots.data_ptr(), rows)
         _stats["rows"] += 1
     return True
 
 
+@functools.lru_cache(maxsize=256)
 def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, columns: int, page_size: int,
                    tracked: bool = False) -> int:
     """fp32 elements of `attention`'s workspace."""
@@ -205,12 +234,12 @@ def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, co
     return kib * 256
 
 
-def _workspace(work, need, dtype, dev):
-    """`work`, checked, or a workspace of `need` elements; its pointer and the tensor."""
+def _workspace(work, need, dtype, like):
+    """`work`, checked, or a new workspace of `need` elements on the device of `like` (None: none is needed)."""
     if work is None:
-        work = torch.empty(need, dtype=dtype, device=dev)
-    elif (work.dtype != dtype or work.device != dev or not work.is_contiguous() or work.numel() < need
-          or work.data_ptr() % 16):
+        return torch.empty(need, dtype=dtype, device=like.device) if need else None
+    if (work.dtype is not dtype or work.device != like.device or not work.is_contiguous() or work.numel() < need
+            or work.data_ptr() % 16):
         raise ValueError(f"work must be a contiguous, 16-byte aligned {dtype} tensor of at least {need} elements")
     return work
 
@@ -229,28 +258,29 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores)
-    if c is None or q.dim() != 3:
+    shape = q.shape
+    if c is None or len(shape) != 3:
         return _declined()
-    dev, hd = k_pages.device, c.head_dim
-    seqs, nh, d = q.shape
-    if (seqs != c.seqs or d != hd or nh < 1 or nh % c.n_kv or nh > 65535 or q.dtype != k_pages.dtype or q.device != dev
-            or q.stride(2) != 1 or (nh > 1 and q.stride(1) != hd)
-            or (seqs > 1 and (q.stride(0) < nh * hd or q.stride(0) % 8)) or q.data_ptr() % 16
+    block, nkv, page, hd, n_seqs, cols, dtype, dev = c
+    seqs, nh, d = shape
+    step, head_step, last = q.stride()
+    qp = q.data_ptr()
+    if (seqs != n_seqs or d != hd or nh < 1 or nh % nkv or nh > 65535 or q.dtype is not dtype or q.get_device() != dev
+            or last != 1 or (nh > 1 and head_step != hd) or (seqs > 1 and (step < nh * hd or step % 8)) or qp % 16
             or not _vector(slots, torch.int64, seqs, dev)):
         return _declined()
     if out is None:
-        out = torch.empty(seqs, nh, hd, dtype=q.dtype, device=dev)
-    elif (out.shape != (seqs, nh, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous()
-          or out.data_ptr() % 16):
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif not _out_ok(out, shape, dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
-    work = _workspace(work, attention_work(seqs, nh, c.n_kv, hd, c.cols, c.page_size, scores is not None),
-                      torch.float32, dev)
-    _launch("ttsp_paged_attention", dev, c, q.data_ptr(), q.stride(0) if seqs > 1 else nh * hd, slots.data_ptr(),
-            out.data_ptr(), nh, hd**-0.5 if scale is None else scale, work.data_ptr())
+    work = _workspace(work, attention_work(seqs, nh, nkv, hd, cols, page, scores is not None), torch.float32, q)
+    _launch("ttsp_paged_attention", dev, block, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
+            hd**-0.5 if scale is None else scale, 0 if work is None else work.data_ptr())
     _stats["attention"] += 1
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def evict_work(seqs: int, n_local_heads: int, columns: int, page_size: int, budget: int) -> int:
     """int32 elements of `evict`'s workspace."""
     kib = _lib.lib().ttsp_paged_evict_work_kib(seqs, n_local_heads, columns, page_size, budget)
@@ -276,16 +306,16 @@ def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, bud
         raise ValueError("evict needs a budget of at least one row, 0 <= sinks, 0 <= recent and sinks + recent <= budget")
     if not _lib.gpu_present():
         return _declined()
-    c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
-    dev = k_pages.device
-    if (c is None or scores is None or slot_pos is None or not _vector(slots, torch.int64, c.seqs, dev)
-            or not _vector(positions, torch.int64, c.seqs, dev)):
+    c = None if scores is None or slot_pos is None else _pool(k_pages, v_pages, block_table, scores, slot_pos)
+    if c is None:
         return _declined()
-    need = evict_work(c.seqs, c.n_kv, c.cols, c.page_size, budget)
-    if need:  # else no sequence can be longer than the budget
-        work = _workspace(work, need, torch.int32, dev)
-        _launch("ttsp_paged_evict", dev, c, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
-                work.data_ptr())
+    block, nkv, page, _, seqs, cols, _, dev = c
+    if not _vector(slots, torch.int64, seqs, dev) or not _vector(positions, torch.int64, seqs, dev):
+        return _declined()
+    if cols * page > budget:  # else no sequence can be longer
+        work = _workspace(work, evict_work(seqs, nkv, cols, page, budget), torch.int32, k_pages)
+        _launch("ttsp_paged_evict", dev, block, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
+                0 if work is None else work.data_ptr())
     _stats["evict"] += 1
     return True
 
