@@ -610,7 +610,7 @@ int ttsp_paged_store(const ttsp_paged_cache* cache, const void* K, long long k_r
                      const int* SEQ, const long long* SLOT, int rows, void* stream);
 
 /* KiB of ttsp_paged_attention's workspace (host-only; 0: none is needed, -1:
- * over 2 TiB); tracked: the cache has scores. */
+ * over 2 TiB, or seqs * cols * page_size over 2^37); tracked: the cache has scores. */
 int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size, int tracked);
 
 /* Attention of one new token per sequence over a paged cache: query (b, hd) at

@@ -101,24 +101,37 @@ struct Chunk {
   int size;       // rows a chunk of this sequence
 };
 
-// A sequence's chunk count and their length, from the call's chunk length.
-__device__ __forceinline__ int chunk_count(int n, int len) { return (n + len - 1) / len; }
+// Rows in units of PG_STEP, the steps that chunks are cut in.
+__device__ __forceinline__ uint32_t units(int n) { return (uint32_t)(n + PG_STEP - 1) / PG_STEP; }
+
+// A sequence's chunk count from the call's chunk length (units).
+__device__ __forceinline__ int chunk_count(int n, uint32_t len) { return (int)((units(n) + len - 1) / len); }
+// The rows a chunk then has: the sequence's, evenly.
 __device__ __forceinline__ int chunk_size(int n, int count) {
-  return count < 2 ? n : ((n + count - 1) / count + PG_STEP - 1) / PG_STEP * PG_STEP;
+  return count < 2 ? n : (int)((units(n) + count - 1) / count * PG_STEP);
 }
 
-// The call's chunk length: its rows over the chunks wanted, in steps.
-__device__ __forceinline__ int chunk_len(const AttnArgs& a, int lane) {
-  long long total = 0;
-  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    const int b = b0 + lane;
-    long long n = b < a.seqs ? a.c.rows(a.SLOT[b]) : 0;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) n += __shfl_xor(n, o, 64);
-    total += n;
-  }
-  const long long len = ((total + a.target - 1) / a.target + PG_STEP - 1) / PG_STEP * PG_STEP;
-  return (int)min(max(len, (long long)PG_STEP), 1LL << 30);
+// v plus the lower lanes' v, by shifts within the rows of 16 lanes and two row
+// broadcasts (lanes without a source add 0).
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+// Rows of sequence b, 0 past the last.
+__device__ __forceinline__ int rows_of(const AttnArgs& a, int b) { return b < a.seqs ? a.c.rows(a.SLOT[b]) : 0; }
+
+// The call's chunk length (units): its rows over the chunks wanted. `n0`: the
+// rows of sequence `lane`. (attn_plan keeps all units within 31 bits.)
+__device__ __forceinline__ uint32_t chunk_len(const AttnArgs& a, int lane, int n0) {
+  uint32_t total = __builtin_amdgcn_readlane(lane_prefix(units(n0)), 63);
+  for (int b0 = 64; b0 < a.seqs; b0 += 64) total += __builtin_amdgcn_readlane(lane_prefix(units(rows_of(a, b0 + lane))), 63);
+  return max((total + a.target - 1) / (uint32_t)a.target, 1u);
 }
 
 // Every wave finds it by itself; the result is uniform.
@@ -127,18 +140,12 @@ __device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int lane)
     const int n = a.c.rows(a.SLOT[gx]);
     return Chunk{gx, n, 0, 1, gx, n};
   }
-  const int len = chunk_len(a, lane);
+  int n = rows_of(a, lane);
+  const uint32_t len = chunk_len(a, lane, n);
   int before = 0;
   for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < a.seqs ? a.c.rows(a.SLOT[b]) : 0;
-    const int count = chunk_count(n, len);
-    int x = count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o, 64);
-      if (lane >= o) x += y;
-    }
+    if (b0) n = rows_of(a, b0 + lane);
+    const int count = chunk_count(n, len), x = (int)lane_prefix(count);
     const uint64_t past = __ballot(before + x > gx);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -191,21 +198,23 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
     const int p = j < k1 ? trow[j >> a.c.shift] : -1;
     return (unsigned)p < (unsigned)a.c.pages ? p : -1;
   };
-  const uint32_t ko = (uint32_t)(lr * (int)a.c.k_row + 8 * lg);
-  const uint32_t vo = (uint32_t)((lane / (64 / VR)) * (int)a.c.v_row + (lane % (64 / VR)) * 8);
+  // a lane's place in a 16-key half: 32-bit byte offsets from a uniform base
+  const uint32_t ko = (uint32_t)(lr * (int)a.c.k_row + 8 * lg) * 2;
+  const uint32_t vo = (uint32_t)((lane / (64 / VR)) * (int)a.c.v_row + (lane % (64 / VR)) * 8) * 2;
   u32x4 kf[2][KC], vf[VPL];
   // A hole reads page 0's rows, which are masked; a page's 16-row runs are whole.
   auto load = [&](int j, int p0, int p1) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int p = max(s ? p1 : p0, 0), row = (j + 16 * s) & mask;
-      const uint16_t* kb = a.c.K + p * a.c.k_page + h * a.c.k_head + row * a.c.k_row;
+      const uint8_t* kb = (const uint8_t*)(a.c.K + p * a.c.k_page + h * a.c.k_head + row * a.c.k_row);
 #pragma unroll
-      for (int i = 0; i < KC; ++i) kf[s][i] = *reinterpret_cast<const u32x4*>(kb + ko + 32 * i);
-      const uint16_t* vb = a.c.V + p * a.c.v_page + h * a.c.v_head + row * a.c.v_row;
+      for (int i = 0; i < KC; ++i) kf[s][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb + 64 * i + ko));
+      const uint8_t* vb = (const uint8_t*)(a.c.V + p * a.c.v_page + h * a.c.v_head + row * a.c.v_row);
 #pragma unroll
       for (int i = 0; i < VPL / 2; ++i)
-        vf[s * (VPL / 2) + i] = *reinterpret_cast<const u32x4*>(vb + vo + (uint32_t)(i * VR * (int)a.c.v_row));
+        vf[s * (VPL / 2) + i] =
+            __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vb + (size_t)i * VR * a.c.v_row * 2 + vo));
     }
   };
   // V's 32-byte blocks lie swizzled by row, so that the transposing reads of
@@ -240,9 +249,15 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int row = i * VR + lane / (64 / VR), c16 = lane % (64 / VR);
-      u32x4 v = vf[i];
-      if (!whole && (j + row >= k1 || (row < 16 ? p0 : p1) < 0)) v = u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = v;
+      *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = vf[i];
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const int row = i * VR + lane / (64 / VR), c16 = lane % (64 / VR);
+        if (j + row >= k1 || (row < 16 ? p0 : p1) < 0)
+          *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};
+      }
     }
     // the next run's rows
     const int c0 = p0, c1 = p1;
@@ -330,13 +345,12 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
     float num = 0.0f, den = 0.0f;
     bool any = false;
 #pragma unroll
-    for (int w = 0; w < PG_WAVES; ++w) {
-      const float l = l_s[w][g];
-      if (l < 0.0f) continue;
-      const float e = __builtin_amdgcn_exp2f(m_s[w][g] - m);
-      den += l * e;
+    for (int w = 0; w < PG_WAVES; ++w) {  // (a wave without a key has a sum of -1 and zeros in O)
+      const float l = l_s[w][g], e = __builtin_amdgcn_exp2f(m_s[w][g] - m);
+      const bool none = l < 0.0f;
+      den += (none ? 0.0f : l) * e;
       num += all[(size_t)w * (REGION / 4) + g * D + d] * e;
-      any = true;
+      any = any || !none;
     }
     const int head = head0 + g;
     if (alone) {
@@ -410,16 +424,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
   __shared__ f32x4 part[256];
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int len = chunk_len(a, lane);
-  int first = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) {
-    int count = b0 + lane < b ? chunk_count(a.c.rows(a.SLOT[b0 + lane]), len) : 0;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) count += __shfl_xor(count, o, 64);
-    first += count;
+  int n = rows_of(a, lane);
+  const uint32_t len = chunk_len(a, lane, n);
+  Chunk ck{b, 0, 0, 0, 0, 0};
+  for (int b0 = 0; b0 <= b; b0 += 64) {  // the chunks of the sequences before this one, and its own
+    if (b0) n = rows_of(a, b0 + lane);
+    const int count = chunk_count(n, len), x = (int)lane_prefix(count);
+    const int l = min(b - b0, 63);
+    ck.count = __builtin_amdgcn_readlane(count, l);
+    ck.first += __builtin_amdgcn_readlane(x, l) - (b - b0 < 64 ? ck.count : 0);
   }
-  Chunk ck{b, a.c.rows(a.SLOT[b]), 0, 0, first, 0};
-  ck.count = chunk_count(ck.n, len);
   uint16_t* const y = a.Y + ((size_t)b * a.nh + head) * D;
   if (ck.count == 1) return;  // finished already
   if (ck.count == 0) {
@@ -493,6 +507,7 @@ inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, bool tra
   const long long wide = (long long)nkv * p->hgs;
   p->target = (int)(wide < PG_WGS ? PG_WGS / wide : 1);
   p->parts = p->scores = 0;
+  if ((long long)seqs * ((cap + PG_STEP - 1) / PG_STEP) > 0x3fffffff) return false;  // (more rows than any memory holds)
   const bool one = cap <= PG_SHORT;
   if (one) p->target = 0;
   // a sequence adds at most one partly filled chunk to those the rows fill

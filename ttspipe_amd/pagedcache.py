@@ -230,7 +230,7 @@ def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, co
     kib = _lib.lib().ttsp_paged_attention_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
                                                    int(tracked))
     if kib < 0:
-        raise ValueError("the workspace would take more than 2 TiB")
+        raise ValueError("the table is too wide, or the workspace would take more than 2 TiB")
     return kib * 256
 
 
