@@ -422,7 +422,10 @@ __device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, in
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
+  constexpr int AHEAD = 8;             // reads of a lane under way together
+  constexpr int WMAX = 1024;           // chunks whose weights are held at once
   __shared__ f32x4 part[256];
+  __shared__ float w_s[WMAX];
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   int n = rows_of(a, lane);
   const uint32_t len = chunk_len(a, lane, n);
@@ -440,17 +443,37 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     if (tid < D / 8) reinterpret_cast<u32x4*>(y)[tid] = u32x4{0u, 0u, 0u, 0u};
     return;
   }
+  const int e = tid % (D / 4), r0 = tid / (D / 4);
+  f32x4 x[AHEAD];
+  auto load = [&](int c0) {  // past the last chunk: the last one's, of weight 0
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const size_t at = (size_t)(ck.first + min(c0 + r0 + i * ROWS, ck.count - 1)) * a.nh + head;
+      x[i] = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
+    }
+  };
+  load(0);  // under way while the sums are joined
   float m, den;
   join_sums(a, ck, head, lane, &m, &den);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int e = tid % (D / 4);
-  for (int c = tid / (D / 4); c < ck.count; c += ROWS) {
-    const size_t at = (size_t)(ck.first + c) * a.nh + head;
-    if (a.PL[at] < 0.0f) continue;
-    const f32x4 x = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
-    const float w = __builtin_amdgcn_exp2f(a.PM[at] - m);
+  for (int c0 = 0; c0 < ck.count; c0 += ROWS * AHEAD) {
+    if (c0) load(c0);
+    if (c0 % WMAX == 0) {
+      __syncthreads();
+      for (int c = tid; c < WMAX; c += 256) {  // (a chunk without a key has zeros, and its reference does not count)
+        const bool there = c0 + c < ck.count;
+        w_s[c] = there ? __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c0 + c) * a.nh + head] - m) : 0.0f;
+      }
+      __syncthreads();
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += x[i] * w;
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = c0 + r0 + i * ROWS;
+      const float w = w_s[c % WMAX];
+      if (c < ck.count)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += x[i][k] * w;
+    }
   }
   part[tid] = acc;
   __syncthreads();
