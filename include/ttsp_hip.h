@@ -626,7 +626,7 @@ int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long
                          const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
 
 /* KiB of ttsp_paged_evict's workspace (host-only; 0: none is needed, where no
- * sequence can have more than 256 rows to move; -1: over 2 TiB). */
+ * sequence can have more than 256 rows to move, in caches of up to 8192 slots; -1: over 2 TiB). */
 int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int budget);
 
 /* Cut every sequence of more than `budget` rows (SLOT[b] + 1, int64) down to
@@ -639,7 +639,7 @@ int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int bu
  * then `budget` (the caller advances SLOT). sinks + recent <= budget. The
  * pages of such a sequence belong to it alone and have no holes below SLOT[b];
  * a row is not copied from or into a hole. work: ttsp_paged_evict_work_kib()
- * KiB (0: may be NULL), 4-byte aligned, which calls that may overlap must not share. Replaces:
+ * KiB (0: may be NULL), 16-byte aligned, which calls that may overlap must not share. Replaces:
  * nothing (the reference's cache is as long as its longest stream). */
 int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS, int budget,
                      int sinks, int recent, int* work, void* stream);

@@ -44,8 +44,14 @@ typedef __attribute__((address_space(3))) pg_s16x4 pg_lds_s16x4;
 
 constexpr int PG_WAVES = 4, PG_KEYS = 32;      // waves a workgroup, keys a wave takes at once
 constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of this
-constexpr int PG_WGS = 1024;                   // workgroups the chunks are meant to make
-constexpr int PG_SHORT = 512;                  // caches of up to this many slots: a sequence is one chunk
+// Workgroups the chunks are meant to make, two rounds of the two that fit a CU.
+// Per call, 512 / 1024 / 1536 / 2048 of them: 32 sequences of 200 to 2304 rows 48.9 /
+// 43.0 / 44.0 / 45.0 us; 64 of 2048 to 5119 200 / 171 / 168 / 166; one of 130995 88 /
+// 89 / 98 / 94 (32 query and 8 kv heads of 128, bf16).
+constexpr int PG_WGS = 1024;
+// Caches of up to this many slots: a sequence is one chunk, and there is no
+// joining launch (300 rows, alone: 7.6 us; in three chunks and joined: 10.0).
+constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   const int h = blockIdx.y / hgs, head0 = h * group + (blockIdx.y % hgs) * PG_HEADS;
   const int heads = min(PG_HEADS, (h + 1) * group - head0);
   const Chunk ck = find_chunk(a, blockIdx.x, lane);
-  if (ck.b < 0) return;  // (a sequence without a row is no chunk, or with target == 0 an empty one)
+  if (ck.b < 0) return;  // (a sequence without a row has no chunk; with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   const int mask = (1 << a.c.shift) - 1;
@@ -418,14 +424,73 @@ __device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, in
   *den = __any(any) ? l : -1.0f;
 }
 
-// Joins a sequence's chunks: workgroup (query head, sequence).
-template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
+// One query head's output from its sequence's chunks (two or more), given the
+// joined reference and sum; all 256 threads. The chunks' sums of the first round
+// are on their way before the reference is known.
+template <int DT, int D, typename Sums>
+__device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, int head, int tid, Sums&& sums) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
   constexpr int AHEAD = 8;             // reads of a lane under way together
   constexpr int WMAX = 1024;           // chunks whose weights are held at once
+  static_assert(WMAX % (ROWS * AHEAD) == 0, "weights change between rounds");
   __shared__ f32x4 part[256];
   __shared__ float w_s[WMAX];
+  const int e = tid % (D / 4), r0 = tid / (D / 4);
+  f32x4 x[AHEAD];
+  auto load = [&](int c0) {  // past the last chunk: the last one's, not used
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const size_t at = (size_t)(ck.first + min(c0 + r0 + i * ROWS, ck.count - 1)) * a.nh + head;
+      x[i] = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
+    }
+  };
+  load(0);
+  float m, den;
+  sums(&m, &den);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c0 = 0; c0 < ck.count; c0 += ROWS * AHEAD) {
+    if (c0) load(c0);
+    if (c0 % WMAX == 0) {
+      __syncthreads();
+      for (int c = tid; c < WMAX && c0 + c < ck.count; c += 256)  // (a chunk without a key: weight times zeros)
+        w_s[c] = __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c0 + c) * a.nh + head] - m);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int c = c0 + r0 + i * ROWS;
+      if (c < ck.count) {
+        const float w = w_s[c % WMAX];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += x[i][k] * w;
+      }
+    }
+  }
+  part[tid] = acc;
+  __syncthreads();
+  if (tid < D / 4) {
+    for (int r = 1; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += part[r * (D / 4) + tid][i];
+    uint2 out;
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = den < 0.0f ? 0.0f : acc[i] / den;
+    out.x = Elem<DT>::store(q[0]) | (uint32_t)Elem<DT>::store(q[1]) << 16;
+    out.y = Elem<DT>::store(q[2]) | (uint32_t)Elem<DT>::store(q[3]) << 16;
+    reinterpret_cast<uint2*>(a.Y + ((size_t)ck.b * a.nh + head) * D)[tid] = out;
+  }
+}
+
+// The outputs of a sequence without a row, which is no chunk's. (In the first
+// launch, stores that never run took 10 % off its speed.)
+__device__ __forceinline__ void zero_rows(uint16_t* y, int elems, int tid) {
+  for (int i = tid; i < elems / 8; i += 256) reinterpret_cast<u32x4*>(y)[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
+// Joins a sequence's chunks: workgroup (query head, sequence).
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   int n = rows_of(a, lane);
   const uint32_t len = chunk_len(a, lane, n);
@@ -437,68 +502,27 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     ck.count = __builtin_amdgcn_readlane(count, l);
     ck.first += __builtin_amdgcn_readlane(x, l) - (b - b0 < 64 ? ck.count : 0);
   }
-  uint16_t* const y = a.Y + ((size_t)b * a.nh + head) * D;
-  if (ck.count == 1) return;  // finished already
+  if (ck.count == 1) return;  // finished by the first launch
   if (ck.count == 0) {
-    if (tid < D / 8) reinterpret_cast<u32x4*>(y)[tid] = u32x4{0u, 0u, 0u, 0u};
+    zero_rows(a.Y + ((size_t)b * a.nh + head) * D, D, tid);
     return;
   }
-  const int e = tid % (D / 4), r0 = tid / (D / 4);
-  f32x4 x[AHEAD];
-  auto load = [&](int c0) {  // past the last chunk: the last one's, of weight 0
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const size_t at = (size_t)(ck.first + min(c0 + r0 + i * ROWS, ck.count - 1)) * a.nh + head;
-      x[i] = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
-    }
-  };
-  load(0);  // under way while the sums are joined
-  float m, den;
-  join_sums(a, ck, head, lane, &m, &den);
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c0 = 0; c0 < ck.count; c0 += ROWS * AHEAD) {
-    if (c0) load(c0);
-    if (c0 % WMAX == 0) {
-      __syncthreads();
-      for (int c = tid; c < WMAX; c += 256) {  // (a chunk without a key has zeros, and its reference does not count)
-        const bool there = c0 + c < ck.count;
-        w_s[c] = there ? __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c0 + c) * a.nh + head] - m) : 0.0f;
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int c = c0 + r0 + i * ROWS;
-      const float w = w_s[c % WMAX];
-      if (c < ck.count)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += x[i][k] * w;
-    }
-  }
-  part[tid] = acc;
-  __syncthreads();
-  if (tid >= D / 4) return;
-  for (int r = 1; r < ROWS; ++r)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += part[r * (D / 4) + tid][i];
-  uint2 out;
-  float q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = den < 0.0f ? 0.0f : acc[i] / den;
-  out.x = Elem<DT>::store(q[0]) | (uint32_t)Elem<DT>::store(q[1]) << 16;
-  out.y = Elem<DT>::store(q[2]) | (uint32_t)Elem<DT>::store(q[3]) << 16;
-  reinterpret_cast<uint2*>(y)[tid] = out;
+  join_head<DT, D>(a, ck, head, tid, [&](float* m, float* den) { join_sums(a, ck, head, lane, m, den); });
 }
 
-// Adds the weights of a chunk's slots to their scores: workgroup (chunk, kv
-// head), for sequences that the first launch has not finished.
+// With scores to gather: workgroup (chunk, kv head) adds the weights of its
+// chunk's slots to their scores, and joins the kv head's query heads c, c + count,
+// ... (c its number among the sequence's count chunks).
+template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a) {
   constexpr int HG = 64;  // query heads whose sums are held at once
   __shared__ float m_s[HG], l_s[HG];
   const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int group = a.nh / a.c.nkv;
+  if ((int)blockIdx.x < a.seqs && a.SLOT[blockIdx.x] < 0)
+    zero_rows(a.Y + ((size_t)blockIdx.x * a.nh + h * group) * D, group * D, tid);
   const Chunk ck = find_chunk(a, blockIdx.x, lane);
-  if (ck.b < 0 || (ck.count == 1 && group <= PG_HEADS)) return;
+  if (ck.b < 0 || (ck.count == 1 && group <= PG_HEADS)) return;  // (finished by the first launch)
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   for (int g0 = 0; g0 < group; g0 += HG) {
     const int gs = min(HG, group - g0);
@@ -516,6 +540,10 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a) {
       for (int g = 0; g < gs; ++g) w += __builtin_amdgcn_exp2f(s[(size_t)g * a.c.cap()] - m_s[g]) / l_s[g];
       a.c.scores[ck.b * a.c.score_seq + h * a.c.score_head + k] += w;
     }
+    if (ck.count > 1)
+      for (int g = ck.c; g < group; g += ck.count)
+        if (g >= g0 && g < g0 + gs)
+          join_head<DT, D>(a, ck, h * group + g, tid, [&](float* m, float* den) { *m = m_s[g - g0], *den = l_s[g - g0]; });
   }
 }
 
@@ -586,7 +614,10 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
   do {                                                                                                           \
     if (tracked) hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, true>), grid, dim3(64 * PG_WAVES), 0, stream, a); \
     else hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, false>), grid, dim3(64 * PG_WAVES), 0, stream, a);        \
-    if (p.target) hipLaunchKernelGGL((paged_join_kernel<DTV, DV>), dim3(nh, a.seqs), dim3(256), 0, stream, a);    \
+    if (tracked && (p.target || p.hgs > 1))                                                                       \
+      hipLaunchKernelGGL((paged_gather_kernel<DTV, DV>), dim3(p.chunks, a.c.nkv), dim3(256), 0, stream, a);       \
+    else if (p.target)                                                                                            \
+      hipLaunchKernelGGL((paged_join_kernel<DTV, DV>), dim3(nh, a.seqs), dim3(256), 0, stream, a);                \
   } while (0)
   if (cache->dtype == DT_F16) {
     if (hd == 128) TTSP_PATT(DT_F16, 128);
@@ -596,6 +627,5 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
     else TTSP_PATT(DT_BF16, 64);
   }
 #undef TTSP_PATT
-  if (tracked && (p.target || p.hgs > 1)) hipLaunchKernelGGL(paged_gather_kernel, dim3(p.chunks, a.c.nkv), dim3(256), 0, stream, a);
   TTSP_RETURN_LAUNCH();
 }
