@@ -48,7 +48,7 @@ HEAD_DIM = 128
 #: Cache positions per attention workgroup (the kernel's ACHUNK).
 CHUNK = 64
 
-_stats = {"fused": 0, "fallback": 0, "prefill": 0}
+_stats = {"fused": 0, "fallback": 0, "prefill": 0, "batch": 0}
 _installed = False
 
 
@@ -215,6 +215,80 @@ def make_workspace(block, x, nchunk: int, *, with_out: bool = False) -> dict:
     if with_out:
         ws["out"] = torch.empty((1, x.shape[-1]), dtype=x.dtype, device=x.device)
     return ws
+
+
+def decode_batch(block, x, freqs_cis, cache):
+    """`TransformerBlock.forward` for the newest token of several sequences that
+    share a paged cache: x (sequences, 1, dim), row b the token at position
+    `cache.table.positions[b]` whose K/V go to slot `cache.table.slots[b]`;
+    `freqs_cis` (positions, head_dim / 2, 2) is the whole rotary table and
+    `cache` this layer's `pagedcache.PagedKVCache`. Returns the blocks' outputs,
+    shaped as x; a row of the table that holds no sequence gives what its x
+    gives with an attention of zeros. None when declined.
+
+    RMSNorm, wqkv, `pagedcache.qk_rope_kv`, `pagedcache.attention` (a tracked
+    cache gathers its weights), wo with the residual and the FFN norm, w1 and w3
+    with the gate, w2 with the residual: the products of the few-row kernels,
+    each weight read once for all sequences, where the reference decodes one
+    sequence at a time (fusedlayer.py:162-269). Its results are `decode_block`'s
+    up to the order of sums and one rounding less of q and k.
+    """
+    import torch
+
+    from ttspipe_amd import fusedops, nf4gemv
+
+    a, ff = block.attention, block.feed_forward
+    table = cache.table
+    if not _lib.gpu_present() or x.dim() != 3 or x.shape[1] != 1 or x.shape[0] != table.slots.shape[0]:
+        return None
+    if x.dtype not in (torch.float16, torch.bfloat16) or x.device.type != "cuda" or not x.is_contiguous():
+        return None
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return decode_batch(block, x, freqs_cis, cache)
+    pools = cache.k_pages
+    if pools.dtype != x.dtype or pools.shape[1] != a.n_local_heads or pools.shape[3] != a.head_dim:
+        return None
+    for linear in (a.wqkv, a.wo, ff.w1, ff.w2, ff.w3):
+        if getattr(linear, "bias", None) is not None or not nf4gemv.prepare(linear):
+            return None
+    an, fn = block.attention_norm, block.ffn_norm
+    rows, nh = x.shape[0], a.n_head
+    qkv = None
+    if rows <= nf4gemv.FUSED_MAX_ROWS:
+        qkv = nf4gemv.matmul_fused(a.wqkv, x, norm_weight=an.weight, eps=an.eps)
+    if qkv is None:
+        xn = fusedops.rms_norm(x, an.weight, an.eps)
+        qkv = None if xn is None else nf4gemv.matmul(a.wqkv, xn)
+    if qkv is None:
+        return None
+    qn, kn = (a.q_norm, a.k_norm) if a.attention_qk_norm else (None, None)
+    q = cache.qk_rope_kv(qkv.view(rows, -1), nh, freqs_cis, q_weight=None if qn is None else qn.weight,
+                         k_weight=None if kn is None else kn.weight, eps=1e-6 if qn is None else float(qn.eps))
+    if q is None:
+        return None
+    y = cache.attention(q)
+    if y is None:
+        raise RuntimeError("decode_batch: the attention declined after the rows were written")
+    y = y.view(rows, 1, nh * a.head_dim)
+    hh = nf4gemv.matmul_norm(a.wo, y, fn.weight, fn.eps, epi=nf4gemv.EPI_RESIDUAL, operand=x)
+    h, hn = hh if hh is not None else (nf4gemv.matmul(a.wo, y, epi=nf4gemv.EPI_RESIDUAL, operand=x), None)
+    u = None
+    if h is not None:
+        h = h.view(x.shape)
+        if hn is None and rows <= nf4gemv.FUSED_MAX_ROWS:
+            u = nf4gemv.matmul_fused(ff.w1, h, norm_weight=fn.weight, eps=fn.eps, module3=ff.w3)
+        if u is None:
+            hn = fusedops.rms_norm(h, fn.weight, fn.eps) if hn is None else hn.view(x.shape)
+            u = None if hn is None else nf4gemv.matmul_swiglu(ff.w1, ff.w3, hn)
+            if u is None and hn is not None:
+                g = nf4gemv.matmul(ff.w1, hn)
+                u = None if g is None else nf4gemv.matmul(ff.w3, hn, epi=nf4gemv.EPI_SILU_GATE, operand=g)
+    out = None if u is None else nf4gemv.matmul(ff.w2, u, epi=nf4gemv.EPI_RESIDUAL, operand=h)
+    if out is None:
+        raise RuntimeError("decode_batch: a prepared layer declined mid-block")
+    _stats["batch"] += 1
+    return out.view(x.shape)
 
 
 def _block_classes():
