@@ -95,6 +95,8 @@ def test_bad_arguments_are_refused_before_any_launch():
     wide = _cache(cols=100, table_stride=100)
     for kw in (dict(work=None, budget=800), dict(work=P + 2, budget=800)):
         assert _evict(lib, wide, **kw) == 1, kw
+    for kw in (dict(score_seq=0), dict(pos_seq=0), dict(score_head=0), dict(pos_head=0)):  # one row for several
+        assert _evict(lib, _cache(**kw)) == 1, kw
     assert _evict(lib, _cache(scores=None)) == 1 and _evict(lib, _cache(slot_pos=None)) == 1
     # nothing to do: no launch either
     assert _rope(lib, c, rows=0) == 0 and _store(lib, c, rows=0) == 0
@@ -240,6 +242,25 @@ def test_page_table_refuses_what_does_not_fit():
     with pytest.raises(ValueError):  # 64 rows are the table's width
         t.step()
     _consistent(t)
+
+
+def test_page_table_keeps_positions_below_their_end():
+    with pytest.raises(ValueError):
+        pc.PageTable(1, 64, 4, 16, device="cpu", max_position=0)
+    t = pc.PageTable(2, 64, 8, 16, device="cpu", max_position=20)
+    with pytest.raises(ValueError):
+        t.admit(21)
+    assert t.admit(18) == 0 and t.positions_used == 18
+    t.step()
+    t.evicted(10)
+    t.step()
+    assert t.rows(0) == 11 and t.positions.tolist() == [19, -1] and t.positions_used == 20
+    with pytest.raises(ValueError):
+        t.step()
+    assert t.positions.tolist() == [19, -1] and t.rows(0) == 11
+    _consistent(t)
+    t.release(0)
+    assert t.positions_used == 0 and t.admit(20) == 0
 
 
 def test_paged_cache_shapes():

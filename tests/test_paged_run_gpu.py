@@ -267,3 +267,20 @@ def test_decode_batch_declines():
                  (x, freqs, pc.PagedKVCache(table, 4)), (x, freqs, pc.PagedKVCache(table, 2, 64)),
                  (x, freqs, pc.PagedKVCache(table, 2, dtype=FP))):
         assert fusedlayer.decode_batch(block, *args) is None
+
+
+def test_decode_batch_refuses_positions_past_the_rotary_table():
+    from tests.test_fused_gpu import _block
+    from ttspipe_amd import fusedlayer
+
+    block, _ = _block(BF, True)
+    table = pc.PageTable(2, 64, 8, 16)
+    cache = pc.PagedKVCache(table, 2)
+    table.admit(30)
+    table.step()
+    x = torch.zeros(2, 1, 512, dtype=BF, device="cuda")
+    k0 = cache.k_pages.clone()
+    with pytest.raises(ValueError):
+        fusedlayer.decode_batch(block, x, _freqs(30, 128), cache)
+    assert torch.equal(k0, cache.k_pages)
+    assert fusedlayer.decode_batch(block, x, _freqs(31, 128), cache) is not None

@@ -28,7 +28,8 @@ counted in `stats()`), a wrong `out`, `work` or budget raises ValueError and a
 failed launch RuntimeError. Work is queued on the current stream of the
 tensors' device; nothing is synchronised, and with `out=` and `work=` given
 nothing is allocated, so that calls can be captured. Calls that may overlap
-(two streams, two graphs) need workspaces of their own.
+(two streams, two graphs) need workspaces of their own. These are calls of a
+decode: they have no gradients.
 """
 
 from __future__ import annotations
@@ -155,8 +156,9 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
 
     A row whose slot has no page (or lies outside the table: -1 for a padding
     row) is not written; a position outside `freqs_cis` makes its q zeros, too.
-    No two rows may name one slot. Without norms the result has the bits of the
-    contiguous cache's kernel, which with norms also rounds between the two."""
+    No two rows may name one slot, and `out` must not overlap qkv. Without norms
+    the result has the bits of the contiguous cache's kernel, which with norms
+    also rounds between the two."""
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
@@ -184,7 +186,7 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
         if not _out_ok(k_weight, (hd,), dtype, dev):
             return _declined()
     if out is None:
-        out = torch.empty((rows, n_head, hd), dtype=dtype, device=qkv.device)
+        out = qkv.new_empty((rows, n_head, hd))
     elif not _out_ok(out, (rows, n_head, hd), dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (rows, n_head, head_dim) tensor of the cache's dtype")
     if rows:
@@ -199,7 +201,8 @@ def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=No
     """Finished rows into the pages: k, v (rows, n_local_heads, D), the last axis
     contiguous and rows 16-byte aligned (a contiguous cache's slice, transposed,
     is taken in place). `seqs`, `slots`, `positions` (needed with `slot_pos`) and
-    the slots' scores as `qk_rope_kv`. True, or None when declined."""
+    the slots' scores as `qk_rope_kv`; positions are noted as 32-bit integers.
+    True, or None when declined."""
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores, slot_pos)
@@ -237,7 +240,7 @@ def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, co
 def _workspace(work, need, dtype, like):
     """`work`, checked, or a new workspace of `need` elements on the device of `like` (None: none is needed)."""
     if work is None:
-        return torch.empty(need, dtype=dtype, device=like.device) if need else None
+        return like.new_empty(need, dtype=dtype) if need else None
     if (work.dtype is not dtype or work.device != like.device or not work.is_contiguous() or work.numel() < need
             or work.data_ptr() % 16):
         raise ValueError(f"work must be a contiguous, 16-byte aligned {dtype} tensor of at least {need} elements")
@@ -270,7 +273,7 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
             or not _vector(slots, torch.int64, seqs, dev)):
         return _declined()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = q.new_empty(shape)
     elif not _out_ok(out, shape, dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
     work = _workspace(work, attention_work(seqs, nh, nkv, hd, cols, page, scores is not None), torch.float32, q)
@@ -325,16 +328,20 @@ class PageTable:
     calls read: `block_table`, `slots` and `positions` (the newest slot and
     position of each sequence, -1: none). One table serves every layer's pools.
 
-    The host knows each sequence's row count without asking the device: `admit`
-    and `step` add rows, `evicted` cuts them, `release` drops them. Running out
-    of pages raises MemoryError and changes nothing."""
+    The host knows each sequence's row count and position without asking the
+    device: `admit` and `step` add rows, `evicted` cuts them, `release` drops
+    them. Running out of pages raises MemoryError and changes nothing; so does,
+    with ValueError, a row past `max_len` rows or past `max_position` positions
+    (the rotary table's rows: a sequence that is evicted from runs on while its
+    rows stay few; None: not checked here)."""
 
-    def __init__(self, seqs: int, max_len: int, pages: int, page_size: int = 64, device="cuda"):
+    def __init__(self, seqs: int, max_len: int, pages: int, page_size: int = 64, device="cuda",
+                 max_position: int | None = None):
         if not MIN_PAGE <= page_size <= MAX_PAGE or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from {MIN_PAGE} to {MAX_PAGE}")
-        if seqs < 1 or pages < 1 or max_len < 1:
-            raise ValueError("seqs, max_len and pages must be positive")
-        self.page_size, self.pages, self.max_len = page_size, pages, max_len
+        if seqs < 1 or pages < 1 or max_len < 1 or (max_position is not None and max_position < 1):
+            raise ValueError("seqs, max_len, pages and max_position must be positive")
+        self.page_size, self.pages, self.max_len, self.max_position = page_size, pages, max_len, max_position
         columns = -(-max_len // page_size)
         self.block_table = torch.full((seqs, columns), -1, dtype=torch.int32, device=device)
         self.slots = torch.full((seqs,), -1, dtype=torch.int64, device=device)
@@ -342,11 +349,16 @@ class PageTable:
         self._active = torch.zeros(seqs, dtype=torch.int64, device=device)
         self._free = list(range(pages - 1, -1, -1))
         self._held: list[list[int]] = [[] for _ in range(seqs)]
-        self._rows = [0] * seqs
+        self._rows, self._next = [0] * seqs, [0] * seqs  # rows held, the next position
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    @property
+    def positions_used(self) -> int:
+        """Positions the furthest sequence has used (its newest one and those before it)."""
+        return max(self._next)
 
     def rows(self, seq: int) -> int:
         """Rows sequence `seq` holds."""
@@ -366,15 +378,15 @@ class PageTable:
     def admit(self, rows: int):
         """A free sequence with pages for `rows` rows (a prompt's, at positions
         0 .. rows - 1): its index, or None when every sequence is taken."""
-        if not 1 <= rows <= self.max_len:
-            raise ValueError(f"a sequence holds 1 to {self.max_len} rows")
+        if not 1 <= rows <= self.max_len or rows > (self.max_position or rows):
+            raise ValueError(f"a sequence holds 1 to {self.max_len} rows, at positions below {self.max_position}")
         seq = next((i for i, n in enumerate(self._rows) if n == 0), None)
         if seq is None:
             return None
         if self._missing(seq, rows) > len(self._free):
             raise MemoryError(f"{self._missing(seq, rows)} pages needed, {len(self._free)} free")
         self._grow(seq, rows)
-        self._rows[seq] = rows
+        self._rows[seq] = self._next[seq] = rows
         self.slots[seq] = self.positions[seq] = rows - 1
         self._active[seq] = 1
         return seq
@@ -384,12 +396,15 @@ class PageTable:
         live = [i for i, n in enumerate(self._rows) if n]
         if any(self._rows[i] == self.max_len for i in live):
             raise ValueError(f"a sequence holds at most {self.max_len} rows")
+        if self.max_position is not None and any(self._next[i] >= self.max_position for i in live):
+            raise ValueError(f"positions end at {self.max_position}")
         need = sum(self._missing(i, self._rows[i] + 1) for i in live)
         if need > len(self._free):
             raise MemoryError(f"{need} pages needed, {len(self._free)} free")
         for i in live:
             self._grow(i, self._rows[i] + 1)
             self._rows[i] += 1
+            self._next[i] += 1
         self.slots += self._active
         self.positions += self._active
 
@@ -410,7 +425,7 @@ class PageTable:
     def release(self, seq: int) -> None:
         """Sequence `seq` ends: its pages go back to the pool."""
         self._free += self._held[seq][::-1]
-        self._held[seq], self._rows[seq] = [], 0
+        self._held[seq], self._rows[seq], self._next[seq] = [], 0, 0
         self.block_table[seq] = -1
         self.slots[seq] = self.positions[seq] = -1
         self._active[seq] = 0
