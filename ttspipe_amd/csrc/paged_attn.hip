@@ -17,7 +17,9 @@
 // they grow. Workgroup = (chunk, kv head or 16 of its query heads), four waves
 // that each take every fourth run of 32 keys and merge at the end; chunks of a
 // sequence join in a second launch. A sequence of one chunk is finished in the
-// first.
+// first. A chunk's kv heads are neighbouring workgroups: their rows are
+// neighbours in the pages (171 against 167 us for 64 sequences of 2048 to 5119
+// rows where its chunks were, 43.5 against 41.2 for 32 of 200 to 2304).
 //
 // A wave's 32 keys: S^T = K Q^T on the matrix cores (16 keys x 16 query heads a
 // tile; K straight from memory into the operand's layout, Q^T stays in
@@ -46,9 +48,9 @@ typedef __attribute__((address_space(3))) pg_s16x4 pg_lds_s16x4;
 constexpr int PG_WAVES = 4, PG_KEYS = 32;      // waves a workgroup, keys a wave takes at once
 constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of this
 // Workgroups the chunks are meant to make, two rounds of the two that fit a CU.
-// Per call, 512 / 1024 / 1536 / 2048 of them: 32 sequences of 200 to 2304 rows 48.9 /
-// 43.0 / 44.0 / 45.0 us; 64 of 2048 to 5119 200 / 171 / 168 / 166; one of 130995 88 /
-// 89 / 98 / 94 (32 query and 8 kv heads of 128, bf16).
+// Per call, 1024 / 1536 / 2048 of them: 32 sequences of 200 to 2304 rows 41.1 / 42.2 /
+// 42.5 us; 64 of 2048 to 5119 167 / 166 / 165; one of 130995 90 / 96 / 96 (32 query
+// and 8 kv heads of 128, bf16; 512 of them, one round: 49 / 200 / 88).
 constexpr int PG_WGS = 1024;
 // Caches of up to this many slots: a sequence is one chunk, and there is no
 // joining launch (300 rows, alone: 7.6 us; in three chunks and joined: 10.0).
@@ -196,9 +198,10 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int group = a.nh / a.c.nkv, hgs = (group + PG_HEADS - 1) / PG_HEADS;
-  const int h = blockIdx.y / hgs, head0 = h * group + (blockIdx.y % hgs) * PG_HEADS;
+  const int wide = a.c.nkv * hgs, part = blockIdx.x % wide, gx = blockIdx.x / wide;
+  const int h = part / hgs, head0 = h * group + (part % hgs) * PG_HEADS;
   const int heads = min(PG_HEADS, (h + 1) * group - head0);
-  const Chunk ck = find_chunk(a, blockIdx.x, lane);
+  const Chunk ck = find_chunk(a, gx, lane);
   if (ck.b < 0) return;  // (a sequence without a row has no chunk; with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
       a.Y[((size_t)b * a.nh + head) * D + d] = Elem<DT>::store(any ? quotient(num, den) : 0.0f);
       continue;
     }
-    const size_t at = (size_t)blockIdx.x * a.nh + head;
+    const size_t at = (size_t)gx * a.nh + head;
     a.PACC[at * D + d] = num;
     if (d == 0) {
       a.PM[at] = m;
@@ -400,7 +403,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
       for (int w = 0; w < PG_WAVES; ++w) m = fmaxf(m, m_s[w][g]);
       for (int w = 0; w < PG_WAVES; ++w)
         if (!(l_s[w][g] < 0.0f)) den += l_s[w][g] * __builtin_amdgcn_exp2f(m_s[w][g] - m), any = true;
-      const size_t at = (size_t)blockIdx.x * a.nh + head0 + g;
+      const size_t at = (size_t)gx * a.nh + head0 + g;
       a.PM[at] = m;
       a.PL[at] = any ? den : -1.0f;
     }
@@ -623,7 +626,7 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
   const int hd = cache->head_dim;
   const bool tracked = a.c.scores != nullptr;
   if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p) || (long long)a.c.nkv * p.hgs > 65535 ||
-      (long long)p.chunks * a.c.nkv + (long long)a.c.seqs * nh > 0x7fffffffLL)
+      (long long)p.chunks * a.c.nkv * p.hgs + (long long)a.c.seqs * nh > 0x7fffffffLL)
     return (int)hipErrorInvalidValue;
   if (p.parts + p.scores && (!work || (uintptr_t)work % 16)) return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;
@@ -638,7 +641,7 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
   a.nh = nh;
   a.seqs = a.c.seqs;
   a.target = p.target;
-  const dim3 grid(p.chunks, a.c.nkv * p.hgs);
+  const dim3 grid((unsigned)p.chunks * a.c.nkv * p.hgs);
   const int gathers = p.chunks * a.c.nkv;
 #define TTSP_PATT(DTV, DV)                                                                                       \
   do {                                                                                                           \
