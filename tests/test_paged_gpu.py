@@ -50,6 +50,55 @@ def test_attention_of_one_sequence(n, dtype, page, hd):
     attention_check(c, y, c.scores, before)
 
 
+@pytest.mark.parametrize("nh,nkv,hd,dtype", [(8, 2, 128, BF), (40, 2, 64, FP), (3, 3, 64, BF)])
+@pytest.mark.parametrize("cap", [16, 512, 528])
+@pytest.mark.parametrize("tracked", [False, True])
+def test_attention_at_the_width_of_short_caches(nh, nkv, hd, dtype, cap, tracked):
+    """Tables one slot group below, at and above the width up to which a
+    sequence is never cut."""
+    lens = [cap, 0, 1, max(1, cap - 15), cap // 2 + 1]
+    c = Case(lens, nh, nkv, hd, 16, dtype, seed=cap + nh, tracked=tracked)
+    y, before = _attend(c)
+    assert not y[1].any()
+    attention_check(c, y, c.scores, before)
+
+
+@pytest.mark.parametrize("seqs,hi", [(65, 40), (130, 700), (200, 16), (200, 600)])
+@pytest.mark.parametrize("tracked", [False, True])
+def test_attention_of_many_sequences(seqs, hi, tracked):
+    """More sequences than a wave has lanes, with empty ones among them, at the
+    ends, and 64 in a row."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, hi + 1, (seqs,), generator=g).tolist()
+    lens[0] = lens[-1] = lens[64] = 0
+    lens[-2] = hi
+    if seqs > 190:
+        lens[64:128] = [0] * 64
+    c = Case(lens, 4, 2, 64, 16, BF, seed=seqs, tracked=tracked)
+    y, before = _attend(c)
+    attention_check(c, y, c.scores, before)
+
+
+def test_attention_on_two_streams_at_once():
+    cs = [Case([2000, 700, 3], 32, 8, 128, 16, BF, seed=50 + i) for i in range(2)]
+    want = []
+    for c in cs:
+        s = c.scores.clone()
+        want.append((pc.attention(c.q, *c.pools(), c.slots, scores=s), s))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[] for _ in cs]
+    for _ in range(4):
+        for c, stream, out in zip(cs, streams, got):
+            with torch.cuda.stream(stream):
+                s = c.scores.clone()
+                out.append((pc.attention(c.q, *c.pools(), c.slots, scores=s), s))
+    torch.cuda.synchronize()
+    for (y, s), outs in zip(want, got):
+        for y2, s2 in outs:
+            assert np.array_equal(bits(y), bits(y2)) and torch.equal(s, s2)
+
+
 @pytest.mark.parametrize("tracked", [False, True])
 def test_attention_of_one_long_sequence_among_short_ones(tracked):
     c = Case([3, 9000, 1, 0, 40], 8, 2, 128, 32, BF, seed=5, tracked=tracked)
@@ -417,6 +466,13 @@ def test_evict_of_a_few_rows(cap, kind):
     lens = [budget + i for i in range(7)]
     c, s, sp = _tracked(lens, 2, 64, 16, BF, seed=cap, kind=kind, cols=-(-cap // 16))
     _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=8)
+
+
+def test_evict_of_many_sequences():
+    g = torch.Generator().manual_seed(60)
+    lens = torch.randint(0, 300, (90,), generator=g).tolist()
+    c, s, sp = _tracked(lens, 3, 64, 16, FP, seed=60, cols=20)
+    assert _evict(c, s, sp, sp.amax((1, 2)).long(), 100, sinks=2, recent=9) > 0
 
 
 def test_evict_of_the_newest_rows_themselves():
