@@ -271,5 +271,9 @@ def test_paged_cache_shapes():
     assert plain.scores is None and plain.k_pages.shape == (12, 2, 16, 128)
     with pytest.raises(ValueError):
         plain.evict(20)
-    with pytest.raises(ValueError):
-        c.store(0, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64))
+    for seq in (0, -1, 3):
+        with pytest.raises(ValueError):
+            c.store(seq, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64))
+    for seq in (-1, 3):
+        with pytest.raises(ValueError):
+            t.release(seq)

@@ -169,7 +169,7 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
     step, last = qkv.stride()
     n_freqs, ftype = freqs_cis.shape[0] if freqs_cis.dim() == 3 else 0, _lib.dtype_code(freqs_cis.dtype)
     qp, fp = qkv.data_ptr(), freqs_cis.data_ptr()
-    if (n_head < 1 or width != (n_head + 2 * nkv) * hd or qkv.dtype is not dtype or qkv.get_device() != dev or last != 1
+    if (not 1 <= n_head <= 4096 or width != (n_head + 2 * nkv) * hd or qkv.dtype is not dtype or qkv.get_device() != dev or last != 1
             or (rows > 1 and (step < width or step % 8)) or qp % 16 or ftype is None or freqs_cis.get_device() != dev
             or not 0 < n_freqs < 1 << 31 or freqs_cis.shape != (n_freqs, hd // 2, 2) or not freqs_cis.is_contiguous()
             or fp % 16 or not _rows_ok(rows, seqs, slots, positions, n_seqs, dev)):
@@ -424,6 +424,8 @@ class PageTable:
 
     def release(self, seq: int) -> None:
         """Sequence `seq` ends: its pages go back to the pool."""
+        if not 0 <= seq < len(self._rows):
+            raise ValueError(f"there is no sequence {seq}")
         self._free += self._held[seq][::-1]
         self._held[seq], self._rows[seq], self._next[seq] = [], 0, 0
         self.block_table[seq] = -1
@@ -457,8 +459,8 @@ class PagedKVCache(nn.Module):
         """Rows start .. start + rows - 1 of sequence `seq` from k, v (rows, n_heads,
         head_dim), their slots also their positions."""
         t, rows = self.table, k.shape[0]
-        if start < 0 or start + rows > t.rows(seq):
-            raise ValueError(f"sequence {seq} holds {t.rows(seq)} rows")
+        if not 0 <= seq < t.slots.shape[0] or start < 0 or start + rows > t.rows(seq):
+            raise ValueError(f"sequence {seq} has no rows {start} to {start + rows - 1}")
         slots = torch.arange(start, start + rows, dtype=torch.int64, device=t.slots.device)
         seqs = torch.full((rows,), seq, dtype=torch.int32, device=t.slots.device)
         return store(k, v, self.k_pages, self.v_pages, t.block_table, slots, positions=slots, seqs=seqs,
