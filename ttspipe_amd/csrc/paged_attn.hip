@@ -152,41 +152,110 @@ __device__ __forceinline__ uint32_t lane_prefix(uint32_t v) {
 // Rows of sequence b, 0 past the last.
 __device__ __forceinline__ int rows_of(const AttnArgs& a, int b) { return b < a.seqs ? a.c.rows(a.SLOT[b]) : 0; }
 
-// The call's chunk length (units): its rows over the chunks wanted. `n0`: the
-// rows of sequence `lane`. (attn_plan keeps all units within 31 bits.)
-__device__ __forceinline__ uint32_t chunk_len(const AttnArgs& a, int lane, int n0) {
-  uint32_t total = __builtin_amdgcn_readlane(lane_prefix(units(n0)), 63);
-  for (int b0 = 64; b0 < a.seqs; b0 += 64) total += __builtin_amdgcn_readlane(lane_prefix(units(rows_of(a, b0 + lane))), 63);
+// The call's chunk length (units): its rows over the chunks wanted. (attn_plan
+// keeps all units within 31 bits.)
+__device__ __forceinline__ uint32_t chunk_len(const AttnArgs& a, uint32_t total) {
   return max((total + a.target - 1) / (uint32_t)a.target, 1u);
 }
 
-// Every wave finds it by itself; the result is uniform.
-__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int lane) {
+// Up to 64 sequences a wave counts by itself, one a lane; more are counted by the
+// workgroup, a run of neighbours a thread (all 256 threads, with barriers). Sequences
+// of up to 1000 rows, where each wave counts all by itself and where the workgroup
+// does: 65 of them 41 and 42 us, 256 of them 115 and 108, 1024 of them 548 and 425.
+constexpr int PG_T = 64 * PG_WAVES;
+static_assert(PG_T == 256, "the launches that look for chunks have 256 threads");
+
+// The sum of v over the workgroup, and over the threads before this one.
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* sums, int tid, uint32_t* total) {
+  const uint32_t upto = lane_prefix(v);
+  __syncthreads();
+  if ((tid & 63) == 63) sums[tid >> 6] = upto;
+  __syncthreads();
+  uint32_t before = upto - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < PG_T / 64; ++w) {
+    if (w < (tid >> 6)) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before;
+}
+
+// Chunk `gx` of the call; the result is uniform.
+__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int tid) {
+  __shared__ uint32_t sums[PG_T / 64];
+  __shared__ int found[4];
+  const int lane = tid & 63;
   if (a.target == 0) {
     const int n = a.c.rows(a.SLOT[gx]);
     return Chunk{gx, n, 0, 1, gx, n};
   }
-  int n = rows_of(a, lane);
-  const uint32_t len = chunk_len(a, lane, n);
-  int before = 0;
-  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-    if (b0) n = rows_of(a, b0 + lane);
-    const int count = chunk_count(n, len), x = (int)lane_prefix(count);
-    const uint64_t past = __ballot(before + x > gx);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      Chunk k;
-      k.b = b0 + l;
-      k.n = __builtin_amdgcn_readlane(n, l);
-      k.count = __builtin_amdgcn_readlane(count, l);
-      k.first = before + __builtin_amdgcn_readlane(x, l) - k.count;
-      k.c = gx - k.first;
-      k.size = chunk_size(k.n, k.count);
-      return k;
-    }
-    before += __builtin_amdgcn_readlane(x, 63);
+  Chunk k{-1, 0, 0, 0, 0, 0};
+  if (a.seqs <= 64) {
+    const int n = rows_of(a, lane);
+    const uint32_t len = chunk_len(a, __builtin_amdgcn_readlane(lane_prefix(units(n)), 63));
+    const int count = chunk_count(n, len), upto = (int)lane_prefix(count);
+    const uint64_t past = __ballot(upto > gx);
+    if (!past) return k;
+    const int l = __builtin_ctzll(past);
+    k.b = l;
+    k.n = __builtin_amdgcn_readlane(n, l);
+    k.count = __builtin_amdgcn_readlane(count, l);
+    k.first = __builtin_amdgcn_readlane(upto, l) - k.count;
+  } else {
+    const int per = (a.seqs + PG_T - 1) / PG_T, b0 = tid * per;
+    uint32_t mine = 0, total;
+    for (int i = 0; i < per; ++i) mine += units(rows_of(a, b0 + i));
+    block_prefix(mine, sums, tid, &total);
+    const uint32_t len = chunk_len(a, total);
+    mine = 0;
+    for (int i = 0; i < per; ++i) mine += chunk_count(rows_of(a, b0 + i), len);
+    int first = (int)block_prefix(mine, sums, tid, &total);
+    if ((uint32_t)gx >= total) return k;
+    if (gx >= first && gx < first + (int)mine)  // one thread
+      for (int i = 0; i < per; ++i) {
+        const int n = rows_of(a, b0 + i), count = chunk_count(n, len);
+        if (gx < first + count) {
+          found[0] = b0 + i, found[1] = n, found[2] = count, found[3] = first;
+          break;
+        }
+        first += count;
+      }
+    __syncthreads();
+    k.b = __builtin_amdgcn_readfirstlane(found[0]);
+    k.n = __builtin_amdgcn_readfirstlane(found[1]);
+    k.count = __builtin_amdgcn_readfirstlane(found[2]);
+    k.first = __builtin_amdgcn_readfirstlane(found[3]);
   }
-  return Chunk{-1, 0, 0, 0, 0, 0};
+  k.c = gx - k.first;
+  k.size = chunk_size(k.n, k.count);
+  return k;
+}
+
+// The chunks of sequence b (its rows and the numbers `c`, `size` left out).
+__device__ __forceinline__ Chunk sequence_chunks(const AttnArgs& a, int b, int tid) {
+  __shared__ uint32_t sums[PG_T / 64];
+  Chunk k{b, 0, 0, 1, b, 0};
+  if (a.target == 0) return k;
+  if (a.seqs <= 64) {
+    const int n = rows_of(a, tid & 63);
+    const uint32_t len = chunk_len(a, __builtin_amdgcn_readlane(lane_prefix(units(n)), 63));
+    const int count = chunk_count(n, len), upto = (int)lane_prefix(count);
+    k.count = __builtin_amdgcn_readlane(count, b);
+    k.first = __builtin_amdgcn_readlane(upto, b) - k.count;
+    return k;
+  }
+  const int per = (a.seqs + PG_T - 1) / PG_T, b0 = tid * per;
+  uint32_t mine = 0, total;
+  for (int i = 0; i < per; ++i) mine += units(rows_of(a, b0 + i));
+  block_prefix(mine, sums, tid, &total);
+  const uint32_t len = chunk_len(a, total);
+  mine = 0;
+  for (int i = 0; i < per && b0 + i < b; ++i) mine += chunk_count(rows_of(a, b0 + i), len);
+  block_prefix(mine, sums, tid, &total);
+  k.first = (int)total;
+  k.count = chunk_count(rows_of(a, b), len);
+  return k;
 }
 
 template <int DT, int D, bool TRACK>
@@ -205,7 +274,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   const int wide = a.c.nkv * hgs, part = blockIdx.x % wide, gx = blockIdx.x / wide;
   const int h = part / hgs, head0 = h * group + (part % hgs) * PG_HEADS;
   const int heads = min(PG_HEADS, (h + 1) * group - head0);
-  const Chunk ck = find_chunk(a, gx, lane);
+  const Chunk ck = find_chunk(a, gx, tid);
   if (ck.b < 0) return;  // (a sequence without a row has no chunk; with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
@@ -517,20 +586,7 @@ __device__ __forceinline__ void zero_rows(uint16_t* y, int elems, int tid) {
 // Query head `head` of sequence b, where the first launch has not finished it.
 template <int DT, int D>
 __device__ __forceinline__ void join_sequence(const AttnArgs& a, int b, int head, int tid) {
-  const int lane = tid & 63;
-  Chunk ck{b, 0, 0, 1, b, 0};
-  if (a.target) {
-    int n = rows_of(a, lane);
-    const uint32_t len = chunk_len(a, lane, n);
-    ck.first = 0;
-    for (int b0 = 0; b0 <= b; b0 += 64) {  // the chunks of the sequences before this one, and its own
-      if (b0) n = rows_of(a, b0 + lane);
-      const int count = chunk_count(n, len), x = (int)lane_prefix(count);
-      const int l = min(b - b0, 63);
-      ck.count = __builtin_amdgcn_readlane(count, l);
-      ck.first += __builtin_amdgcn_readlane(x, l) - (b - b0 < 64 ? ck.count : 0);
-    }
-  }
+  const Chunk ck = sequence_chunks(a, b, tid);
   if (ck.count > 1)
     join_head<DT, D>(a, ck, head, tid);
   else if (ck.count == 0)  // no row, so no chunk. (In the first launch, stores that never ran took 10 % off its speed.)
@@ -558,7 +614,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
     return;
   }
   const int h = blockIdx.x % a.c.nkv, group = a.nh / a.c.nkv;
-  const Chunk ck = find_chunk(a, blockIdx.x / a.c.nkv, lane);
+  const Chunk ck = find_chunk(a, blockIdx.x / a.c.nkv, tid);
   if (ck.b < 0 || (ck.count == 1 && group <= PG_HEADS)) return;  // (finished by the first launch)
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   for (int g0 = 0; g0 < group; g0 += HG) {

@@ -253,7 +253,9 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     D), a sequence's heads contiguous, over slots 0 .. slots[b] (cut to the
     table's width), query head h with KV head h // (n_head / n_local_heads), the
     scores scaled by `scale` (D^-0.5). Returns (sequences, n_head, D), in `out`
-    if given, or None when declined. A sequence without a row gives zeros.
+    if given, or None when declined. A sequence without a row gives zeros; a
+    row's infinities and NaN give what the formula gives, but for an infinite
+    value in an fp16 cache, which may give NaN.
 
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
