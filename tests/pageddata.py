@@ -52,9 +52,9 @@ def attention64(q, k, v, table, slots, scale=None):
     within 1 +- 2d; exp2 and the sums of n terms, 32 and more at a time, add
     2^-20 + 2^-23 (n / 8 + 64): together the weights' relative error e. For y the
     matrix cores take each term exp(s - m) in two parts of the cache's type,
-    together within 2^-16 of it, and 2^-25 of 1 where an fp16 part is subnormal;
-    the largest term of each partial sum is at least 1, so the denominator is
-    too."""
+    together within 2^-16 of it, and 2^-25 where an fp16 part is subnormal; the
+    largest term of each partial sum in fp16 is at least 2^13, so that is at most
+    2^-38 of the denominator."""
     fp16 = k.dtype == torch.float16
     q, k, v, table = q.double().cpu(), k.cpu(), v.cpu(), table.cpu()
     B, nh, D = q.shape
@@ -77,7 +77,7 @@ def attention64(q, k, v, table, slots, scale=None):
             mag = (qq.abs() @ K.abs().t()).max(1, keepdim=True).values * scale
             e = 2 * (D + 4) * 2.0**-24 * mag + 2.0**-20 + 2.0**-23 * (n / 8 + 64)
             y[b, h * group:(h + 1) * group] = w @ V
-            yb[b, h * group:(h + 1) * group] = (w @ V.abs()) * (e + 2.0**-16) + fp16 * 2.0**-25 * V.abs().sum(0)
+            yb[b, h * group:(h + 1) * group] = (w @ V.abs()) * (e + 2.0**-16) + fp16 * 2.0**-38 * V.abs().sum(0)
             p[b, h, j] = w.sum(0)
             pb[b, h, j] = (w * e).sum(0)
     return y, p, yb, pb

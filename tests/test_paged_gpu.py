@@ -184,6 +184,32 @@ def test_attention_with_a_minus_infinite_key_among_finite_ones():
     assert_within(y, ref, rounding(ref, FP) * (1 + 2**-7) + yb)
 
 
+@pytest.mark.parametrize("gap", [9, 14, 17, 21])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_keeps_a_long_tail_of_small_weights(dtype, first, gap):
+    """16380 rows e^-gap of the four largest weights each (one in the share of
+    each wave of a sequence that is not cut), whose values alone count: weights of
+    2^-13 to 2^-30. Relative to y: 2 (D + 4) 2^-24 gap for the scores, 2^-23 (n / 8
+    + 64) for the sums, 2^-16 for the weights' parts (and, in fp16, 2^-38 of the
+    largest weight)."""
+    n, hd, heads, seqs = 16384, 64, 64, 16
+    k, v = torch.zeros(n // 64, heads, 64, hd), torch.ones(n // 64, heads, 64, hd)
+    for j in (0, 32, 64, 96):
+        j += 0 if first else n - 128
+        k[j // 64, :, j % 64, 0] = gap
+        v[j // 64, :, j % 64] = 0.0
+    q = torch.zeros(seqs, heads, hd)
+    q[:, :, 0] = 1.0
+    k, v, q = (x.to(dtype).cuda() for x in (k, v, q))
+    table = torch.arange(n // 64, dtype=torch.int32, device="cuda").expand(seqs, -1).contiguous()
+    y = pc.attention(q, k, v, table, torch.full((seqs,), n - 1, device="cuda"), scale=1.0)
+    tail = (n - 4) * math.exp(-gap) / 4
+    ref = torch.full((seqs, heads, hd), tail / (1 + tail), dtype=torch.float64)
+    e = 2 * (hd + 4) * 2.0**-24 * gap + 2.0**-20 + 2.0**-23 * (n / 8 + 64) + 2.0**-16 + 2.0**-38 * math.exp(gap)
+    assert_within(y, ref, rounding(ref, dtype) * (1 + 2**-7) + ref * e, "tail")
+
+
 def test_attention_scale_out_and_work():
     c = Case([90, 33], 8, 2, 64, 16, BF, seed=11)
     need = pc.attention_work(2, 8, 2, 64, c.table.shape[1], 16, tracked=True)

@@ -28,7 +28,7 @@
 // A wave's 32 keys: S^T = K Q^T on the matrix cores (16 keys x 16 query heads a
 // tile; K straight from memory into the operand's layout, Q^T stays in
 // registers), so a lane holds 8 keys of one query head. The exponentials
-// subtract a reference that moves only when a score outgrows it by 2^8, so the
+// subtract a reference that moves only when a score outgrows it (pg_above), so the
 // running maximum needs no exchange between lanes but a vote. P^T goes to the
 // matrix cores in two parts of the cache's type (together within 2^-16 of each
 // weight; one part, half a step off, took y's error against 64 bits from 0.0016 to
@@ -61,6 +61,12 @@ constexpr int PG_WGS = 1024;
 constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
+// A moved reference lies `pg_below` under the largest score and moves again when a
+// score is `pg_above` over it. bf16 weights have room on both sides. fp16 ones end
+// at 2^-24: a largest weight of 2^13 to 2^15 lets those 2^-38 of it count, where one
+// of 1 to 2^8 would round a long tail of weights around 2^-24 to 0 or to double.
+template <int DT> constexpr float pg_below = DT == DT_F16 ? 13.0f : 0.0f;
+template <int DT> constexpr float pg_above = DT == DT_F16 ? 15.0f : 8.0f;
 
 struct AttnArgs {
   Paged c;
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
         float x = s[t][r] * a.scale2;
         if (!whole && (j + 16 * t + 4 * lg + r >= k1 || (t ? c1 : c0) < 0)) x = -__builtin_inff();
         s[t][r] = x;
-        over = over || x > mref + 8.0f;
+        over = over || x > mref + pg_above<DT>;
       }
     if constexpr (TRACK) {
       if (lr < heads)
@@ -383,7 +389,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
       bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mnew = bm > mref + 8.0f ? bm : mref;
+      const float mnew = bm > mref + pg_above<DT> ? bm - pg_below<DT> : mref;
       const float alpha = __builtin_amdgcn_exp2f(mref - mnew);
       mref = mnew;
       lsum *= alpha;
@@ -575,12 +581,6 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, in
     out.y = Elem<DT>::store(q[2]) | (uint32_t)Elem<DT>::store(q[3]) << 16;
     reinterpret_cast<uint2*>(a.Y + ((size_t)ck.b * a.nh + head) * D)[tid] = out;
   }
-}
-
-// The outputs of a sequence without a row, which is no chunk's. (In the first
-// launch, stores that never run took 10 % off its speed.)
-__device__ __forceinline__ void zero_rows(uint16_t* y, int elems, int tid) {
-  for (int i = tid; i < elems / 8; i += 256) reinterpret_cast<u32x4*>(y)[i] = u32x4{0u, 0u, 0u, 0u};
 }
 
 // Query head `head` of sequence b, where the first launch has not finished it.

@@ -255,7 +255,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     scores scaled by `scale` (D^-0.5). Returns (sequences, n_head, D), in `out`
     if given, or None when declined. A sequence without a row gives zeros; a
     row's infinities and NaN give what the formula gives, but for an infinite
-    value in an fp16 cache, which may give NaN.
+    value in an fp16 cache, which may give NaN, and scores beyond 2e38, which
+    count as infinite.
 
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
