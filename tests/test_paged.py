@@ -103,6 +103,20 @@ def test_bad_arguments_are_refused_before_any_launch():
     assert _evict(lib, c, budget=64, work=None) == 0 and _evict(lib, c, budget=1 << 24, work=None) == 0
 
 
+def test_calls_of_more_workgroups_than_a_launch_counts_are_refused_before_it():
+    lib, c = _lib.load(), _cache()
+    rows, rs = 1 << 24, 4096 * 128 + 8 * 128
+    assert _rope(lib, c, rows=rows, nh=64, rs=rs) == 1 and _rope(lib, c, rows=rows, nh=4096, rs=rs) == 1
+    assert _store(lib, _cache(n_kv=16), rows=rows) == 1
+    assert _attention(lib, _cache(seqs=65535, scores=None, pages=1 << 20), nh=512, qs=512 * 128) == 1
+
+
+def test_attention_refuses_scores_that_several_share():
+    lib = _lib.load()
+    for kw in (dict(score_seq=0), dict(score_head=0)):
+        assert _attention(lib, _cache(**kw)) == 1, kw
+
+
 def test_workspace_queries():
     lib = _lib.load()
     assert pc.attention_work(1, 1, 1, 64, 1, 16) >= 0
@@ -241,6 +255,16 @@ def test_page_table_refuses_what_does_not_fit():
         t.step()
     with pytest.raises(ValueError):  # 64 rows are the table's width
         t.step()
+    _consistent(t)
+
+
+def test_page_table_keeps_at_least_a_row_of_each_sequence():
+    t = pc.PageTable(2, 64, 8, 16, device="cpu")
+    t.admit(20)
+    for budget in (0, -1):
+        with pytest.raises(ValueError):
+            t.evicted(budget)
+    assert t.rows(0) == 20 and t.slots.tolist() == [19, -1]
     _consistent(t)
 
 

@@ -15,6 +15,9 @@
 
 namespace ttsp {
 
+// Workgroups of 256 threads a launch may have (its threads are counted in 32 bits).
+constexpr long long PG_MAX_GRID = 0xffffff;
+
 // ttsp_paged_cache with the page size as a shift (the kernels' argument).
 struct Paged {
   uint16_t* K;

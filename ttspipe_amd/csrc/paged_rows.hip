@@ -136,7 +136,7 @@ template <bool ROPE>
 int launch_rows(const RowsArgs& a, int hd, int dtype, hipStream_t stream) {
   const int heads = a.nh + 2 * a.c.nkv;
   const long long groups = ((long long)a.rows * heads * (hd / 8) + 255) / 256;
-  if (groups > 0x7fffffffLL) return (int)hipErrorInvalidValue;
+  if (groups > PG_MAX_GRID) return (int)hipErrorInvalidValue;
 #define TTSP_ROWS(DTV, DV) \
   hipLaunchKernelGGL((paged_rows_kernel<DTV, DV, ROPE>), dim3((unsigned)groups), dim3(256), 0, stream, a)
   if (dtype == DT_F16) {

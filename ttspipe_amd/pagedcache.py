@@ -135,8 +135,9 @@ def _out_ok(out, shape, dtype, dev) -> bool:
             and not out.data_ptr() % 16)
 
 
-def _rows_ok(rows, seqs_of, slots, positions, seqs, dev) -> bool:
-    if rows > 1 << 24 or not _vector(slots, torch.int64, rows, dev):
+def _rows_ok(rows, width, seqs_of, slots, positions, seqs, dev) -> bool:
+    # (a thread takes eight of a row's `width` elements, and a launch is counted in 32 bits)
+    if rows > 1 << 24 or rows * width > 0xffffff << 11 or not _vector(slots, torch.int64, rows, dev):
         return False
     if positions is not None and not _vector(positions, torch.int64, rows, dev):
         return False
@@ -172,7 +173,7 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
     if (not 1 <= n_head <= 4096 or width != (n_head + 2 * nkv) * hd or qkv.dtype is not dtype or qkv.get_device() != dev or last != 1
             or (rows > 1 and (step < width or step % 8)) or qp % 16 or ftype is None or freqs_cis.get_device() != dev
             or not 0 < n_freqs < 1 << 31 or freqs_cis.shape != (n_freqs, hd // 2, 2) or not freqs_cis.is_contiguous()
-            or fp % 16 or not _rows_ok(rows, seqs, slots, positions, n_seqs, dev)):
+            or fp % 16 or not _rows_ok(rows, width, seqs, slots, positions, n_seqs, dev)):
         return _declined()
     if positions is None and (n_freqs < rows or slot_pos is not None):
         return _declined()
@@ -212,7 +213,7 @@ def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=No
     block, nkv, _, hd, n_seqs, _, dtype, dev = c
     rows = shape[0]
     if (shape[1] != nkv or shape[2] != hd or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != dev
-            or v.get_device() != dev or not _rows_ok(rows, seqs, slots, positions, n_seqs, dev)
+            or v.get_device() != dev or not _rows_ok(rows, 2 * nkv * hd, seqs, slots, positions, n_seqs, dev)
             or (slot_pos is not None and positions is None)):
         return _declined()
     (kr, kh, kl), (vr, vh, vl) = k.stride(), v.stride()
@@ -253,8 +254,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     D), a sequence's heads contiguous, over slots 0 .. slots[b] (cut to the
     table's width), query head h with KV head h // (n_head / n_local_heads), the
     scores scaled by `scale` (D^-0.5). Returns (sequences, n_head, D), in `out`
-    if given, or None when declined. A sequence without a row gives zeros; a
-    row's infinities and NaN give what the formula gives, but for an infinite
+    if given (which must not overlap q), or None when declined. A sequence
+    without a row gives zeros; a row's infinities and NaN give what the formula gives, but for an infinite
     value in an fp16 cache, which may give NaN, and scores beyond 2e38, which
     count as infinite.
 
@@ -414,6 +415,8 @@ class PageTable:
     def evicted(self, budget: int) -> None:
         """After `evict` on every layer: no sequence holds more than `budget`
         rows. Pages past those (and the next row's) go back to the pool."""
+        if budget < 1:
+            raise ValueError("a sequence keeps at least one row")
         self.slots.clamp_(max=budget - 1)
         keep = -(-(budget + 1) // self.page_size)
         for seq, n in enumerate(self._rows):
