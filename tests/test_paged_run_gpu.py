@@ -252,6 +252,22 @@ def test_decode_batch_of_one_is_close_to_the_decode_block():
     assert (got - ref).norm() / ref.norm() < 5e-3
 
 
+def test_decode_batch_takes_head_norms_without_an_epsilon_as_the_decode_block_does():
+    from tests.test_fused_gpu import _block
+    from ttspipe_amd import fusedlayer
+
+    block, _ = _block(BF, True)
+    x = torch.randn(2, 1, 512, device="cuda").to(BF)
+    got = []
+    for eps in (None, 1e-6):
+        table = pc.PageTable(2, 64, 8, 16)
+        cache = pc.PagedKVCache(table, 2)
+        table.admit(3), table.step()
+        block.attention.q_norm.eps = block.attention.k_norm.eps = eps
+        got += [fusedlayer.decode_batch(block, x, _freqs(64, 128), cache), cache.k_pages]
+    assert np.array_equal(bits(got[0]), bits(got[2])) and np.array_equal(bits(got[1]), bits(got[3]))
+
+
 def test_decode_batch_declines():
     from tests.test_fused_gpu import _block
     from ttspipe_amd import fusedlayer

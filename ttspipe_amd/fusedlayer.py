@@ -265,8 +265,9 @@ def decode_batch(block, x, freqs_cis, cache):
     if qkv is None:
         return None
     qn, kn = (a.q_norm, a.k_norm) if a.attention_qk_norm else (None, None)
+    eps = float(qn.eps if qn is not None and qn.eps is not None else 1e-6)
     q = cache.qk_rope_kv(qkv.view(rows, -1), nh, freqs_cis, q_weight=None if qn is None else qn.weight,
-                         k_weight=None if kn is None else kn.weight, eps=1e-6 if qn is None else float(qn.eps))
+                         k_weight=None if kn is None else kn.weight, eps=eps)
     if q is None:
         return None
     y = cache.attention(q)
