@@ -1,0 +1,45 @@
+"""The paged cache's operators in forms and at sizes that lie between those of
+`test_paged_gpu.py` (GPU): each against its definition in 64 bits, with the
+bounds of `tests/pageddata.py` unless a test derives its own."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.pageddata import assert_within, rounding
+from ttspipe_amd import pagedcache as pc
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def cancelling(seqs, cols, hd=64, page=16):
+    """bf16 caches of three rows whose scores are 0, 0 and -s and whose values are
+    what bf16 holds of w = exp(-s), what it holds of the rest, both negative, and
+    1: y = (w - hi - mid) / (2 + w), 2^-18 w and less, so that the bits of w
+    beyond two parts of eight are all that is left."""
+    s = torch.linspace(0.03, 2.0, seqs).to(BF)
+    w = torch.exp(-s.double())
+    hi = w.to(BF)
+    mid = (w - hi.double()).to(BF)
+    k, v = torch.zeros(seqs, 1, page, hd, dtype=BF), torch.zeros(seqs, 1, page, hd, dtype=BF)
+    k[:, 0, 2, 0] = -s
+    v[:, 0, 0], v[:, 0, 1], v[:, 0, 2] = -hi[:, None], -mid[:, None], 1.0
+    q = torch.zeros(seqs, 1, hd, dtype=BF)
+    q[:, :, 0] = 1.0
+    table = torch.full((seqs, cols), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(seqs)
+    return q, k, v, table, w, (w - hi.double() - mid.double()) / (2 + w)
+
+
+@pytest.mark.parametrize("cols", [1, 64])
+def test_attention_holds_a_bf16_weight_whole(cols):
+    """Of w, a weight is off by its argument's two roundings (at most 2 of 2^-24 of
+    2 log2(e), as a factor 2^-22), exp2's step (2^-23) and three products' sums at w's
+    size (3 (2^-23 + 2^-24)): less than 2^-19 together."""
+    q, k, v, table, w, y = cancelling(70, cols)
+    got = pc.attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.full((70,), 2, device="cuda"), scale=1.0)
+    ref = y.view(-1, 1, 1).expand(got.shape)
+    assert_within(got, ref, rounding(ref, BF) * (1 + 2**-7) + (w / (2 + w)).view(-1, 1, 1) * 2.0**-19)

@@ -30,9 +30,10 @@
 // registers), so a lane holds 8 keys of one query head. The exponentials
 // subtract a reference that moves only when a score outgrows it (pg_above), so the
 // running maximum needs no exchange between lanes but a vote. P^T goes to the
-// matrix cores in two parts of the cache's type (together within 2^-16 of each
-// weight; one part, half a step off, took y's error against 64 bits from 0.0016 to
-// 0.0023 of its norm in bf16, and no time); the sums stay in fp32. It feeds
+// matrix cores in parts of the cache's type: bf16 in three, which hold a weight
+// whole, fp16 in two, together within 2^-22 of it; the sums stay in fp32. (bf16 in
+// two parts, within 2^-16: 300 rows of one sequence 8.0 against 8.3 us, the larger
+// calls the same within 1 %; one output in a thousand off by a step.) It feeds
 // O^T += V^T P^T from the registers it is in: the contraction takes the keys in the order the score
 // tiles hold them, and V^T comes from V's rows in LDS through the transposing
 // read. Each wave has its own 32 rows of LDS and never waits for another. K and
@@ -92,25 +93,31 @@ __device__ __forceinline__ f32x4 pg_mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                   0, 0);
 }
 
-// Two weights (not negative) as packed pairs of DT whose sum is each to 2^-16 of
-// it: what DT holds of it, rounded towards zero, and the rest, rounded to
-// nearest. (bf16: the rest is kept above 0, so that a weight's halves times an
-// infinite value have one sign.)
+// 16-bit parts a weight goes to the matrix cores in.
+template <int DT> constexpr int pg_parts = DT == DT_F16 ? 2 : 3;
+
+// Two weights (not negative) as packed pairs of DT. bf16: three parts of eight
+// bits each, their sum the weight itself (the lower ones are kept above 0, so that
+// a weight's parts times an infinite value have one sign). fp16: what it holds of
+// the weight, rounded towards zero, and the rest, rounded to nearest, together
+// within 2^-22 of it.
 template <int DT>
-__device__ __forceinline__ void pg_split(float p, float q, uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ void pg_split(float p, float q, uint32_t* parts) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   if constexpr (DT == DT_BF16) {
-    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-    const uint32_t up = __float_as_uint(p), uq = __float_as_uint(q);
-    *hi = __builtin_amdgcn_perm(uq, up, 0x07060302u);
-    const float rp = fmaxf(p - __uint_as_float(up & 0xffff0000u), 1.17549435e-38f);
-    const float rq = fmaxf(q - __uint_as_float(uq & 0xffff0000u), 1.17549435e-38f);
-    *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){rp, rq}, b16x2));
+    constexpr float least = 1.17549435e-38f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t up = __float_as_uint(p), uq = __float_as_uint(q);
+      parts[i] = __builtin_amdgcn_perm(uq, up, 0x07060302u);
+      p = fmaxf(p - __uint_as_float(up & 0xffff0000u), least);
+      q = fmaxf(q - __uint_as_float(uq & 0xffff0000u), least);
+    }
   } else {
     typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
     const h16x2 h = __builtin_bit_cast(h16x2, __builtin_amdgcn_cvt_pkrtz(p, q));
-    *hi = __builtin_bit_cast(uint32_t, h);
-    *lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p - (float)h[0], q - (float)h[1]}, h16x2));
+    parts[0] = __builtin_bit_cast(uint32_t, h);
+    parts[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p - (float)h[0], q - (float)h[1]}, h16x2));
   }
 }
 
@@ -398,7 +405,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
     }
-    u32x4 pf, pr;  // the weights' two parts
+    u32x4 pf[pg_parts<DT>];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float p[4];
@@ -407,11 +414,13 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
         p[r] = __builtin_amdgcn_exp2f(s[t][r] - mref);
         lsum += p[r];
       }
-      uint32_t hi[2], lo[2];
-      pg_split<DT>(p[0], p[1], &hi[0], &lo[0]);
-      pg_split<DT>(p[2], p[3], &hi[1], &lo[1]);
-      pf[2 * t] = hi[0], pf[2 * t + 1] = hi[1];
-      pr[2 * t] = lo[0], pr[2 * t + 1] = lo[1];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t parts[pg_parts<DT>];
+        pg_split<DT>(p[2 * r], p[2 * r + 1], parts);
+#pragma unroll
+        for (int i = 0; i < pg_parts<DT>; ++i) pf[i][2 * t + r] = parts[i];
+      }
     }
     // V^T: row = dim 16 d + lr at keys 4 lg .. + 3 and 16 + 4 lg .. + 3
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -423,8 +432,8 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
       const uint2 lo = pg_ld_tr(vs + vaddr(row, d) + 8 * (lr & 3));
       const uint2 hi = pg_ld_tr(vs + vaddr(row + 16, d) + 8 * (lr & 3));
       const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
-      o[d] = pg_mfma<DT>(vt, pf, o[d]);
-      o[d] = pg_mfma<DT>(vt, pr, o[d]);
+#pragma unroll
+      for (int i = 0; i < pg_parts<DT>; ++i) o[d] = pg_mfma<DT>(vt, pf[i], o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
