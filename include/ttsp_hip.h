@@ -75,7 +75,8 @@ enum { TTSP_FAST_SYNC_WORDS = 192, TTSP_FAST_SYNC_FAILED = 128 };
  * scores (fp32) and slot_pos (int32), each optional, hold per sequence, kv head
  * and slot the attention weight the slot has gathered and the position its row
  * came from: element (b, head, j) at scores + b*score_seq + head*score_head + j
- * (slot_pos with its own strides), cols * page_size of them a head. */
+ * (slot_pos with its own strides), cols * page_size of them a head, no two of
+ * which may share a word. */
 enum { TTSP_PAGED_MAX_SLOTS = 1 << 24, TTSP_PAGED_MAX_ROW_STRIDE = 1 << 24 };
 typedef struct ttsp_paged_cache {
   void* K;

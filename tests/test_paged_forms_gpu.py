@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.pageddata import assert_within, rounding
+from tests.pageddata import Case, assert_within, rounding
 from ttspipe_amd import pagedcache as pc
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,18 @@ def test_attention_holds_a_bf16_weight_whole(cols):
     got = pc.attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.full((70,), 2, device="cuda"), scale=1.0)
     ref = y.view(-1, 1, 1).expand(got.shape)
     assert_within(got, ref, rounding(ref, BF) * (1 + 2**-7) + (w / (2 + w)).view(-1, 1, 1) * 2.0**-19)
+
+
+def test_scores_and_positions_that_overlap_are_declined():
+    """Strides of at least a head's slots each, and sequence 1's first head in the place of sequence 0's second."""
+    c = Case([40, 40], 4, 2, 64, 16, BF, seed=1)
+    over, apart, wrong = (torch.zeros(6 * c.cap, dtype=t, device="cuda").as_strided((2, 2, c.cap), (c.cap, n * c.cap, 1))
+                          for t, n in ((torch.float32, 1), (torch.float32, 2), (torch.int32, 1)))
+    sp, pos = torch.zeros(c.scores.shape, dtype=torch.int32, device="cuda"), c.slots.clone()
+    assert pc.attention(c.q, *c.pools(), c.slots, scores=over) is None
+    assert pc.attention(c.q, *c.pools(), c.slots, scores=apart) is not None
+    assert pc.evict(*c.pools(), c.slots, over, sp, pos, 20) is None
+    assert pc.evict(*c.pools(), c.slots, c.scores, wrong, pos, 20) is None
+    rows = torch.zeros(2, 2, 64, dtype=BF, device="cuda")
+    assert pc.store(rows, rows, *c.pools(), c.slots, scores=over) is None
+    assert not over.any()

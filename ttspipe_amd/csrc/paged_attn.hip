@@ -697,7 +697,6 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
   if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p) || (long long)a.c.nkv * p.hgs > 65535 ||
       (long long)p.chunks * a.c.nkv * p.hgs + (long long)a.c.seqs * nh > PG_MAX_GRID)
     return (int)hipErrorInvalidValue;
-  if (tracked && ((a.c.seqs > 1 && !a.c.score_seq) || (a.c.nkv > 1 && !a.c.score_head))) return (int)hipErrorInvalidValue;
   if (p.parts + p.scores && (!work || (uintptr_t)work % 16)) return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;
   a.q_seq = q_seq_stride;

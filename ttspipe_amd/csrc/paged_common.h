@@ -42,6 +42,13 @@ struct Paged {
   }
 };
 
+// Whether the `cap` words of every (sequence, kv head) lie apart by these strides.
+// (A workgroup adds to its own words, or moves them, while others do to theirs.)
+inline bool words_apart(long long seq, long long head, int seqs, int nkv, long long cap) {
+  if (seq < (seqs > 1 ? cap : 0) || head < (nkv > 1 ? cap : 0)) return false;
+  return seqs == 1 || nkv == 1 || (seq - cap) / (nkv - 1) >= head || (head - cap) / (seqs - 1) >= seq;
+}
+
 // The kernels' form of `c` for head dim `hd`-wide rows; false where the fields
 // do not describe a cache these kernels take (the caller returns
 // hipErrorInvalidValue). Rows are read and written 16 bytes at a time.
@@ -56,9 +63,11 @@ inline bool paged_args(const ttsp_paged_cache* c, Paged* p) {
       c->table_stride < c->cols || c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
     return false;
   if ((c->head_dim != 64 && c->head_dim != 128) || (c->dtype != DT_F16 && c->dtype != DT_BF16)) return false;
-  if ((long long)c->cols * c->page_size > TTSP_PAGED_MAX_SLOTS) return false;
-  if ((c->scores && ((uintptr_t)c->scores % 4 || c->score_seq < 0 || c->score_head < 0)) ||
-      (c->slot_pos && ((uintptr_t)c->slot_pos % 4 || c->pos_seq < 0 || c->pos_head < 0)))
+  const long long cap = (long long)c->cols * c->page_size;
+  if (cap > TTSP_PAGED_MAX_SLOTS) return false;
+  if (c->scores && ((uintptr_t)c->scores % 4 || !words_apart(c->score_seq, c->score_head, c->seqs, c->n_kv, cap)))
+    return false;
+  if (c->slot_pos && ((uintptr_t)c->slot_pos % 4 || !words_apart(c->pos_seq, c->pos_head, c->seqs, c->n_kv, cap)))
     return false;
   *p = Paged{(uint16_t*)c->K, (uint16_t*)c->V, c->k_page, c->k_head, c->k_row, c->v_page, c->v_head, c->v_row,
              c->table, c->table_stride, c->seqs, c->cols, c->pages, __builtin_ctz((unsigned)c->page_size), c->n_kv,

@@ -642,8 +642,7 @@ extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* 
                                 int budget, int sinks, int recent, int* work, hipStream_t stream) {
   EvictArgs a{};
   if (!paged_args(cache, &a.c) || !a.c.scores || !a.c.slot_pos || !SLOT || !POS || budget < 1 || sinks < 0 ||
-      recent < 0 || sinks > budget - recent || (a.c.seqs > 1 && (!a.c.score_seq || !a.c.pos_seq)) ||
-      (a.c.nkv > 1 && (!a.c.score_head || !a.c.pos_head)))
+      recent < 0 || sinks > budget - recent)
     return (int)hipErrorInvalidValue;
   const long long cap = a.c.cap();
   if (cap <= budget) return 0;  // no table row holds more than the budget

@@ -7,8 +7,8 @@ keys and values in pages of one pool instead, so that a stream takes the pages
 it needs and gives them back. For D-wide heads (64 or 128) and 16-bit caches:
 
 * pools `k_pages`, `v_pages` (pages, n_local_heads, page size, D), the last
-  axis contiguous, any other strides that keep rows 16-byte aligned; the page
-  size a power of two from 16 to 4096;
+  axis contiguous, any other strides that keep rows 16-byte aligned and
+  apart; the page size a power of two from 16 to 4096;
 * `block_table` int32 (sequences, columns): row b names sequence b's pages, and
   slot j of the sequence is row j % page size of its page j // page size. An
   entry that is no page of the pool (-1) is a hole: its slots do not exist;
@@ -16,7 +16,8 @@ it needs and gives them back. For D-wide heads (64 or 128) and 16-bit caches:
   holds nothing;
 * `scores` fp32 and `slot_pos` int32 (sequences, n_local_heads, columns * page
   size), where a cache is evicted from: the attention weight each slot has
-  gathered and the position its row came from.
+  gathered and the position its row came from; a head's slots contiguous, any
+  strides that keep the heads apart.
 
 `qk_rope_kv` and `store` write rows, `attention` reads them, `evict` cuts a
 sequence down to a budget. `PageTable` hands the pages out and keeps the device
@@ -66,6 +67,13 @@ def _strides_ok(s, nkv, pages, hd) -> bool:
             and (nkv == 1 or s[1] >= hd) and (pages == 1 or s[0] >= hd))
 
 
+def _words_ok(s0, s1, last, seqs, nkv, cap) -> bool:
+    """Whether the cap words of every (sequence, head) are contiguous and lie apart, by their strides."""
+    if last != 1 or (seqs > 1 and s0 < cap) or (nkv > 1 and s1 < cap):
+        return False
+    return seqs == 1 or nkv == 1 or s0 >= (nkv - 1) * s1 + cap or s1 >= (seqs - 1) * s0 + cap
+
+
 def _pool(k_pages, v_pages, block_table, scores=None, slot_pos=None):
     """(the C-ABI's argument block, n_kv, page size, head dim, sequences, columns,
     the cache's dtype, its device's index) of these tensors, or None where the
@@ -98,14 +106,14 @@ def _pool(k_pages, v_pages, block_table, scores=None, slot_pos=None):
         if scores.dtype is not torch.float32 or scores.get_device() != dev or scores.shape != (seqs, nkv, cap):
             return None
         sc0, sc1, last = scores.stride()
-        if last != 1 or (seqs > 1 and sc0 < cap) or (nkv > 1 and sc1 < cap):
+        if not _words_ok(sc0, sc1, last, seqs, nkv, cap):
             return None
         scp = scores.data_ptr()
     if slot_pos is not None:
         if slot_pos.dtype is not torch.int32 or slot_pos.get_device() != dev or slot_pos.shape != (seqs, nkv, cap):
             return None
         sp0, sp1, last = slot_pos.stride()
-        if last != 1 or (seqs > 1 and sp0 < cap) or (nkv > 1 and sp1 < cap):
+        if not _words_ok(sp0, sp1, last, seqs, nkv, cap):
             return None
         spp = slot_pos.data_ptr()
     block = _BLOCK.pack(kp, vp, block_table.data_ptr(), scp, spp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
