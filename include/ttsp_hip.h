@@ -610,8 +610,10 @@ int ttsp_paged_store(const ttsp_paged_cache* cache, const void* K, long long k_r
                      const void* V, long long v_row_stride, long long v_head_stride, const long long* POS,
                      const int* SEQ, const long long* SLOT, int rows, void* stream);
 
-/* KiB of ttsp_paged_attention's workspace (host-only; 0: none is needed, -1:
- * over 2 TiB, or seqs * cols * page_size over 2^37); tracked: the cache has scores. */
+/* KiB of ttsp_paged_attention's workspace (host-only; 0: none is needed, -1: no
+ * such call is taken: sizes out of range, over 2 TiB, seqs * cols * page_size over
+ * 2^37, or more workgroups than a launch has, about seqs * nh of 2^24); tracked:
+ * the cache has scores. */
 int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size, int tracked);
 
 /* Attention of one new token per sequence over a paged cache: query (b, hd) at
@@ -627,7 +629,8 @@ int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long
                          const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
 
 /* KiB of ttsp_paged_evict's workspace (host-only; 0: none is needed, where no
- * sequence can have more than 256 rows to move, in caches of up to 8192 slots; -1: over 2 TiB). */
+ * sequence can have more than 256 rows to move, in caches of up to 8192 slots; -1: no
+ * such call is taken: sizes out of range or over 2 TiB). */
 int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int budget);
 
 /* Cut every sequence of more than `budget` rows (SLOT[b] + 1, int64) down to

@@ -58,3 +58,16 @@ def test_scores_and_positions_that_overlap_are_declined():
     rows = torch.zeros(2, 2, 64, dtype=BF, device="cuda")
     assert pc.store(rows, rows, *c.pools(), c.slots, scores=over) is None
     assert not over.any()
+
+
+def test_calls_of_more_heads_than_a_launch_has_workgroups_are_declined():
+    """65535 sequences of 256 heads (2 GB of q): sizes that every check of a tensor lets pass."""
+    seqs, nh, hd = 65535, 256, 64
+    k = torch.zeros(1, 1, 16, hd, dtype=BF, device="cuda")
+    table = torch.zeros(seqs, 1, dtype=torch.int32, device="cuda")
+    slots = torch.zeros(seqs, dtype=torch.int64, device="cuda")
+    q = torch.empty(seqs, nh, hd, dtype=BF, device="cuda")
+    before = pc.stats()["declined"]
+    assert pc.attention(q, k, k, table, slots) is None and pc.stats()["declined"] == before + 1
+    y = pc.attention(torch.zeros(seqs, 1, hd, dtype=BF, device="cuda"), k, k, table, slots)
+    assert y is not None and not y.any()

@@ -6,6 +6,7 @@ import pytest
 
 from tests.test_paged import _attention, _cache, _evict, _rope, _store
 from ttspipe_amd import _lib
+from ttspipe_amd import pagedcache as pc
 
 
 @pytest.mark.parametrize("kw", [dict(score_seq=64), dict(score_seq=192), dict(score_head=63), dict(pos_seq=64, pos_head=65),
@@ -25,3 +26,20 @@ def test_scores_whose_heads_lie_apart_are_taken():
                dict(n_kv=1, score_head=0, pos_head=3)):
         c = _cache(**kw)
         assert _evict(lib, c, budget=64) == 0 and _rope(lib, c, rows=0, rs=4096) == 0  # (nothing to launch)
+
+
+def test_workspace_queries_of_sizes_that_no_call_takes():
+    lib = _lib.load()
+    for seqs, nh, nkv, hd, cols, page, tracked in (
+            (65535, 256, 1, 64, 1, 16, 0), (65535, 4096, 8, 128, 1, 16, 0), (20000, 840, 1, 128, 100, 16, 0),  # workgroups
+            (1, 65535, 1, 64, 1 << 20, 16, 1),  # 4 TiB of scores
+            (65535, 1, 1, 64, 1 << 20, 16, 0), (1, 1, 1, 64, (1 << 20) + 1, 16, 0), (65536, 1, 1, 64, 1, 16, 0),
+            (1, 65536, 1, 64, 1, 16, 0), (1, 1, 1, 256, 1, 16, 0), *[(2**31 - 1,) * 6 + (t,) for t in (0, 1)],
+            (2**31 - 1, 2**31 - 1, 1, 128, 2**31 - 1, 16, 1)):
+        assert lib.ttsp_paged_attention_work_kib(seqs, nh, nkv, hd, cols, page, tracked) == -1, (seqs, nh, cols)
+        with pytest.raises(ValueError):
+            pc.attention_work(seqs, nh, nkv, hd, cols, page, bool(tracked))
+    assert lib.ttsp_paged_attention_work_kib(65535, 128, 1, 64, 1, 16, 0) == 0
+    for seqs, nkv, cols, page, budget in ((65536, 1, 64, 16, 5), (1, 4097, 64, 16, 5), (1, 1, (1 << 20) + 1, 16, 5),
+                                          (2**31 - 1, 2**31 - 1, 2**31 - 1, 2**31 - 1, 5)):
+        assert lib.ttsp_paged_evict_work_kib(seqs, nkv, cols, page, budget) == -1, (seqs, nkv, cols)

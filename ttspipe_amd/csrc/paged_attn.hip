@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
   }
 }
 
-// How a call is cut up; false where the workspace's size overflows.
+// How a call is cut up; false where the workspace, the rows or the launch are more than are counted.
 struct AttnPlan {
   int target, chunks, hgs;
   size_t parts, scores;  // floats
@@ -668,7 +668,7 @@ inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, bool tra
   // several workgroups of a kv head leave their sums for the gathering launch even so
   if (!one || (tracked && p->hgs > 1)) p->parts = (((size_t)p->chunks * nh * (2 + hd)) + 3) / 4 * 4;
   p->scores = tracked ? (size_t)seqs * nh * cap : 0;
-  return (p->parts + p->scores + 255) / 256 <= 0x7fffffff;
+  return (p->parts + p->scores + 255) / 256 <= 0x7fffffff && p->chunks * wide + (long long)seqs * nh <= PG_MAX_GRID;
 }
 
 }  // namespace ttsp
@@ -679,7 +679,10 @@ extern "C" int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head
                                              int tracked) {
   if (seqs < 1 || nkv < 1 || nh < nkv || cols < 1 || page_size < 1 || head_dim < 1) return 0;
   AttnPlan p;
-  if (!attn_plan(seqs, nh, nkv, head_dim, (long long)cols * page_size, tracked != 0, &p)) return -1;
+  const long long cap = (long long)cols * page_size;
+  if (seqs > 65535 || nh > 65535 || head_dim > 128 || cap > TTSP_PAGED_MAX_SLOTS ||
+      !attn_plan(seqs, nh, nkv, head_dim, cap, tracked != 0, &p))
+    return -1;
   return (int)((p.parts + p.scores + 255) / 256);
 }
 
@@ -694,9 +697,7 @@ extern "C" int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q
     return (int)hipErrorInvalidValue;
   const int hd = cache->head_dim;
   const bool tracked = a.c.scores != nullptr;
-  if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p) || (long long)a.c.nkv * p.hgs > 65535 ||
-      (long long)p.chunks * a.c.nkv * p.hgs + (long long)a.c.seqs * nh > PG_MAX_GRID)
-    return (int)hipErrorInvalidValue;
+  if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, a.c.cap(), tracked, &p)) return (int)hipErrorInvalidValue;
   if (p.parts + p.scores && (!work || (uintptr_t)work % 16)) return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;
   a.q_seq = q_seq_stride;

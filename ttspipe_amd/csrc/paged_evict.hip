@@ -633,6 +633,7 @@ extern "C" int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_s
   if (seqs < 1 || nkv < 1 || cols < 1 || page_size < 1 || budget < 1) return 0;
   const long long cap = (long long)cols * page_size;
   if (cap <= budget) return 0;
+  if (seqs > 65535 || nkv > 4096 || cap > TTSP_PAGED_MAX_SLOTS) return -1;
   const EvictPlan p = evict_plan(seqs, nkv, cap, budget);
   const size_t kib = ((p.lists + p.heads + p.counts + p.hists + p.cands) * 4 + 1023) / 1024;
   return kib > 0x7fffffffu ? -1 : (int)kib;

@@ -236,13 +236,17 @@ def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=No
 
 
 @functools.lru_cache(maxsize=256)
+def _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked) -> int:
+    return _lib.lib().ttsp_paged_attention_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
+                                                    int(tracked))
+
+
 def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, columns: int, page_size: int,
                    tracked: bool = False) -> int:
-    """fp32 elements of `attention`'s workspace."""
-    kib = _lib.lib().ttsp_paged_attention_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
-                                                   int(tracked))
+    """fp32 elements of `attention`'s workspace; ValueError where `attention` declines sizes like these."""
+    kib = _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked)
     if kib < 0:
-        raise ValueError("the table is too wide, or the workspace would take more than 2 TiB")
+        raise ValueError("too many heads or slots for one call, or the workspace would take more than 2 TiB")
     return kib * 256
 
 
@@ -284,11 +288,14 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
             or last != 1 or (nh > 1 and head_step != hd) or (seqs > 1 and (step < nh * hd or step % 8)) or qp % 16
             or not _vector(slots, torch.int64, seqs, dev)):
         return _declined()
+    kib = _attention_kib(seqs, nh, nkv, hd, cols, page, scores is not None)
+    if kib < 0:
+        return _declined()
     if out is None:
         out = q.new_empty(shape)
     elif not _out_ok(out, shape, dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
-    work = _workspace(work, attention_work(seqs, nh, nkv, hd, cols, page, scores is not None), torch.float32, q)
+    work = _workspace(work, kib * 256, torch.float32, q)
     _launch("ttsp_paged_attention", dev, block, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
             hd**-0.5 if scale is None else scale, 0 if work is None else work.data_ptr())
     _stats["attention"] += 1
