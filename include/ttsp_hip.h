@@ -641,8 +641,9 @@ int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int bu
  * the free slots below it, with their score and slot_pos; rows that stay, and
  * what slots from `budget` on hold, are not touched. The sequence's next slot is
  * then `budget` (the caller advances SLOT). sinks + recent <= budget. The
- * pages of such a sequence belong to it alone and have no holes below SLOT[b];
- * a row is not copied from or into a hole. work: ttsp_paged_evict_work_kib()
+ * pages of such a sequence belong to it alone and have no holes up to SLOT[b]
+ * (their slots would be ranked by what their scores hold; nothing moves from or
+ * into one). work: ttsp_paged_evict_work_kib()
  * KiB (0: may be NULL), 16-byte aligned, which calls that may overlap must not share. Replaces:
  * nothing (the reference's cache is as long as its longest stream). */
 int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS, int budget,

@@ -4,10 +4,12 @@ bounds of `tests/pageddata.py` unless a test derives its own."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from tests.pageddata import Case, assert_within, rounding
+from tests.gpuutil import bits
+from tests.pageddata import Case, assert_within, evict_ref, rounding
 from ttspipe_amd import pagedcache as pc
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +73,38 @@ def test_calls_of_more_heads_than_a_launch_has_workgroups_are_declined():
     assert pc.attention(q, k, k, table, slots) is None and pc.stats()["declined"] == before + 1
     y = pc.attention(torch.zeros(seqs, 1, hd, dtype=BF, device="cuda"), k, k, table, slots)
     assert y is not None and not y.any()
+
+
+# --------------------------------------------------------------- the eviction
+
+
+@pytest.mark.parametrize("n,budget,cols", [(103, 100, 8), (140, 100, 9), (700, 300, 44), (9000, 8000, 563), (2500, 1200, 157)])
+def test_evict_moves_nothing_from_or_into_a_hole(n, budget, cols):
+    """A hole among the slots below the budget and one above it, in every variant (a
+    few rows over, moved while ranking, listed, in parts): each move between pages
+    is whole, and of the others neither the row nor its score or position goes."""
+    c = Case([n], 2, 2, 64, 16, BF, seed=n, cols=cols)
+    g = torch.Generator().manual_seed(n)
+    s = torch.rand(1, 2, c.cap, generator=g)
+    low, high = 2, budget // 16 + 1 if n - budget > 16 else (n - 1) // 16
+    s[:, :, 16 * low:16 * low + 3] = -1.0  # some of the free slots are the hole's, and some movers
+    s[:, :, budget:][:, :, :2] += 2.0
+    sp = torch.arange(c.cap, dtype=torch.int32).expand(1, 2, -1).contiguous()
+    moves = [evict_ref(s[0, h].numpy(), sp[0, h].numpy(), n, n - 1, budget, 0, 0) for h in range(2)]
+    c.table[0, low] = c.table[0, high] = -1
+    holes = [sum(src // 16 == high or dst // 16 == low for src, dst in m) for m in moves]
+    assert all(holes), holes
+    k, v, s1, sp1 = c.k.clone(), c.v.clone(), s.clone(), sp.clone()
+    table = c.table.cpu().tolist()[0]
+    for h, m in enumerate(moves):
+        for src, dst in m:
+            p, q = table[src // 16], table[dst // 16]
+            if p < 0 or q < 0:
+                continue
+            for t in (k, v):
+                t[q, h, dst % 16] = t[p, h, src % 16]
+            s1[0, h, dst], sp1[0, h, dst] = s[0, h, src], sp[0, h, src]
+    s, sp = s.cuda(), sp.cuda()
+    assert pc.evict(*c.pools(), c.slots, s, sp, torch.tensor([n - 1], device="cuda"), budget)
+    assert torch.equal(s.cpu(), s1) and torch.equal(sp.cpu(), sp1)
+    assert np.array_equal(bits(c.k), bits(k)) and np.array_equal(bits(c.v), bits(v))

@@ -175,9 +175,16 @@ __device__ __forceinline__ void store_row(const Paged& c, int page, int h, int j
   *reinterpret_cast<u32x4*>(c.K + page * c.k_page + h * c.k_head + row * c.k_row + e) = r.k;
   *reinterpret_cast<u32x4*>(c.V + page * c.v_page + h * c.v_head + row * c.v_row + e) = r.v;
 }
-__device__ __forceinline__ void move_row(const Paged& c, int b, int h, int src, int dst, int lane) {
+// The row of slot src to slot dst with its score and position (sc, sp: the
+// sequence's and head's). Nothing of it where either is in a hole.
+__device__ __forceinline__ void move_row(const Paged& c, float* sc, int* sp, int b, int h, int src, int dst, int lane) {
   const int from = c.page(b, src), to = c.page(b, dst);
-  if (from >= 0 && to >= 0) store_row(c, to, h, dst, lane, load_row(c, from, h, src, lane));
+  if (from < 0 || to < 0) return;
+  if (lane == 0) {
+    sc[dst] = sc[src];
+    sp[dst] = sp[src];
+  }
+  store_row(c, to, h, dst, lane, load_row(c, from, h, src, lane));
 }
 
 // T threads holding eight keys each.
@@ -270,7 +277,8 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
       }
       if (!stays || dst < 0) return;
       const int to = a.c.page(b, dst);
-      if (row_page >= 0 && to >= 0) store_row(a.c, to, h, dst, tid % LH, row);
+      if (row_page < 0 || to < 0) return;
+      store_row(a.c, to, h, dst, tid % LH, row);
       if (tid % LH == 0) {
         sc[dst] = sc[over];
         sp[dst] = sp[over];
@@ -338,11 +346,7 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
     return;
   }
   __syncthreads();
-  for (int i = tid; i < moves; i += T) {
-    sc[dst[i]] = sc[src[i]];
-    sp[dst[i]] = sp[src[i]];
-  }
-  for (int i = tid / LH; i < moves; i += T / LH) move_row(a.c, b, h, src[i], dst[i], tid % LH);
+  for (int i = tid / LH; i < moves; i += T / LH) move_row(a.c, sc, sp, b, h, src[i], dst[i], tid % LH);
 }
 
 // What the launches over parts share: part blockIdx.x of (kv head blockIdx.y,
@@ -563,14 +567,8 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const EvictArgs a
   const int* work = a.work + ((size_t)b * a.c.nkv + h) * a.list_ints();
   const int i = blockIdx.x * ROWS + (int)threadIdx.x / LH;
   if (i >= work[0]) return;
-  const int src = work[1 + i], dst = work[1 + a.max_moves + i];
-  if (lane == 0) {
-    float* const sc = a.c.scores + b * a.c.score_seq + h * a.c.score_head;
-    int* const sp = a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head;
-    sc[dst] = sc[src];
-    sp[dst] = sp[src];
-  }
-  move_row(a.c, b, h, src, dst, lane);
+  move_row(a.c, a.c.scores + b * a.c.score_seq + h * a.c.score_head, a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head,
+           b, h, work[1 + i], work[1 + a.max_moves + i], lane);
 }
 
 // How a call is done; the workspace in ints.

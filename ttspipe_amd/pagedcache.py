@@ -322,7 +322,10 @@ def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, bud
     they were, and so are `slots`: the caller's next slot is `budget`
     (`PageTable.evicted`). True, or None when declined.
 
-    The pages of a sequence that is cut belong to it alone. `work`: an int32
+    The pages of a sequence that is cut belong to it alone, and it has no holes up
+    to its newest slot (as `PageTable` keeps it): a hole's slots would be ranked by
+    what their scores hold, and a row that would move from or into one stays where
+    it is, with its score and position. `work`: an int32
     workspace of `evict_work(...)` elements, else allocated per call."""
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget or budget > _lib.PAGED_MAX_SLOTS:
         raise ValueError("evict needs a budget of at least one row, 0 <= sinks, 0 <= recent and sinks + recent <= budget")
