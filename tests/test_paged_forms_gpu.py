@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from tests.gpuutil import bits
-from tests.pageddata import Case, assert_within, evict_ref, rounding
+from tests.pageddata import Case, assert_within, attention_check, evict_ref, rounding
 from ttspipe_amd import pagedcache as pc
 
 pytestmark = pytest.mark.gpu
@@ -73,6 +73,15 @@ def test_calls_of_more_heads_than_a_launch_has_workgroups_are_declined():
     assert pc.attention(q, k, k, table, slots) is None and pc.stats()["declined"] == before + 1
     y = pc.attention(torch.zeros(seqs, 1, hd, dtype=BF, device="cuda"), k, k, table, slots)
     assert y is not None and not y.any()
+
+
+@pytest.mark.parametrize("lens,track", [([131072], True), ([130941, 5], False), ([261000], False), ([196613, 0, 5], True)])
+def test_attention_of_one_kv_head_in_a_thousand_chunks(lens, track):
+    """One KV head, which its own chunks must fill the GPU with: 1024, 1023, 1020 and 769 to a sequence."""
+    c = Case(lens, 3, 1, 64, 4096, BF, seed=lens[0] % 97, tracked=track)
+    before = c.scores.clone() if track else None
+    y = pc.attention(c.q, *c.pools(), c.slots, scores=c.scores)
+    attention_check(c, y, c.scores, before)
 
 
 # --------------------------------------------------------------- the eviction

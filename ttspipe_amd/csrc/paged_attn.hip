@@ -541,10 +541,8 @@ template <int DT, int D>
 __device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, int head, int tid) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
   constexpr int AHEAD = 8;             // reads of a lane under way together
-  constexpr int WMAX = 1024;           // chunks whose weights are held at once
-  static_assert(WMAX % (ROWS * AHEAD) == 0, "weights change between rounds");
   __shared__ f32x4 part[256];
-  __shared__ float w_s[WMAX];
+  __shared__ float w_s[PG_WGS];        // the chunks' weights (chunk_len: a sequence has at most `target` chunks)
   const int e = tid % (D / 4), r0 = tid / (D / 4);
   f32x4 x[AHEAD];
   auto load = [&](int c0) {  // past the last chunk: the last one's, not used
@@ -558,19 +556,16 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, in
   float m, den;
   join_sums(a, ck, head, tid & 63, &m, &den);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = tid; c < ck.count; c += 256)  // (a chunk without a key: weight times zeros)
+    w_s[c] = __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c) * a.nh + head] - m);
+  __syncthreads();
   for (int c0 = 0; c0 < ck.count; c0 += ROWS * AHEAD) {
     if (c0) load(c0);
-    if (c0 % WMAX == 0) {
-      __syncthreads();
-      for (int c = tid; c < WMAX && c0 + c < ck.count; c += 256)  // (a chunk without a key: weight times zeros)
-        w_s[c] = __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c0 + c) * a.nh + head] - m);
-      __syncthreads();
-    }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int c = c0 + r0 + i * ROWS;
       if (c < ck.count) {
-        const float w = w_s[c % WMAX];
+        const float w = w_s[c];
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] += x[i][k] * w;
       }
