@@ -84,6 +84,36 @@ def test_attention_of_one_kv_head_in_a_thousand_chunks(lens, track):
     attention_check(c, y, c.scores, before)
 
 
+@pytest.mark.parametrize("seqs", [63, 64, 65, 256, 257, 300, 1000])
+@pytest.mark.parametrize("tracked", [False, True])
+def test_attention_counts_the_chunks_of_many_sequences(seqs, tracked):
+    """Tables wide enough to be cut, one sequence a lane of a wave and one to four a
+    thread of the workgroup, the last of them uneven; empty ones at both ends, in a
+    run of 70 and alone, a few long ones among short ones."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 25, (seqs,), generator=g).tolist()
+    for b, n in zip(torch.randperm(seqs, generator=g).tolist(), (1023, 700, 513, 129, 128, 400)):
+        lens[b] = n
+    lens[0] = lens[-1] = lens[seqs // 2] = 0
+    lens[-2] = 640
+    if seqs > 200:
+        lens[100:170] = [0] * 70
+    c = Case(lens, 4, 2, 64, 16, BF, seed=seqs, cols=64, tracked=tracked)
+    before = c.scores.clone() if tracked else None
+    y = pc.attention(c.q, *c.pools(), c.slots, scores=c.scores)
+    attention_check(c, y, c.scores, before)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,dtype", [(65, 1, 64, BF), (132, 2, 128, FP), (200, 1, 64, FP)])
+@pytest.mark.parametrize("cols", [20, 130])
+def test_weights_of_more_query_heads_than_are_gathered_at_once(nh, nkv, hd, dtype, cols):
+    """Over 64 query heads a KV head: their weights are added to a score in rounds."""
+    c = Case([300, 0, 1, 129, min(cols * 16, 2000)], nh, nkv, hd, 16, dtype, seed=nh, cols=cols)
+    before = c.scores.clone()
+    y = pc.attention(c.q, *c.pools(), c.slots, scores=c.scores)
+    attention_check(c, y, c.scores, before)
+
+
 # --------------------------------------------------------------- the eviction
 
 
