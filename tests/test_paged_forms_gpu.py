@@ -10,6 +10,7 @@ import torch
 
 from tests.gpuutil import bits
 from tests.pageddata import Case, assert_within, attention_check, evict_ref, rounding
+from tests.test_paged_gpu import _evict, _tracked
 from ttspipe_amd import pagedcache as pc
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +148,17 @@ def test_evict_moves_nothing_from_or_into_a_hole(n, budget, cols):
     assert pc.evict(*c.pools(), c.slots, s, sp, torch.tensor([n - 1], device="cuda"), budget)
     assert torch.equal(s.cpu(), s1) and torch.equal(sp.cpu(), sp1)
     assert np.array_equal(bits(c.k), bits(k)) and np.array_equal(bits(c.v), bits(v))
+
+
+@pytest.mark.parametrize("cap", [2048, 2064])
+@pytest.mark.parametrize("budget", [257, 1024, -257])
+@pytest.mark.parametrize("hd,dtype", [(64, FP), (128, BF)])
+@pytest.mark.parametrize("kind", ["exp", "few", "same", "every"])
+def test_evict_lists_the_moves_of_whole_caches(cap, budget, hd, dtype, kind):
+    """More moves than the ranking workgroup does by itself, at the last width of its
+    256-thread form and the first of its 1024-thread one."""
+    budget = budget if budget > 0 else cap + budget
+    lens = [cap, cap - 1, budget, budget + 1, budget + 4, budget + 5, 0, 1, (cap + budget) // 2]
+    c, s, sp = _tracked(lens, 2, hd, 16, dtype, seed=cap + budget, kind=kind, cols=cap // 16)
+    assert pc.evict_work(len(lens), 2, cap // 16, 16, budget) > 0
+    assert _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=17)
