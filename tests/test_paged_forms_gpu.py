@@ -9,8 +9,8 @@ import pytest
 import torch
 
 from tests.gpuutil import bits
-from tests.pageddata import Case, assert_within, attention_check, evict_ref, rounding
-from tests.test_paged_gpu import _evict, _tracked
+from tests.pageddata import Case, assert_within, attention64, attention_check, evict_ref, rounding
+from tests.test_paged_gpu import _evict, _freqs, _rope64, _tracked
 from ttspipe_amd import pagedcache as pc
 
 pytestmark = pytest.mark.gpu
@@ -162,3 +162,125 @@ def test_evict_lists_the_moves_of_whole_caches(cap, budget, hd, dtype, kind):
     c, s, sp = _tracked(lens, 2, hd, 16, dtype, seed=cap + budget, kind=kind, cols=cap // 16)
     assert pc.evict_work(len(lens), 2, cap // 16, 16, budget) > 0
     assert _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=17)
+
+
+# ------------------------------------------------------------------ the block
+
+
+def _streams(nkv, hd, lens, dtype, layers=1, **kw):
+    """A table with a stream of each length, and `layers` caches with seeded rows."""
+    table = pc.PageTable(len(lens) + 1, 128, 60, 16)
+    caches = [pc.PagedKVCache(table, nkv, hd, dtype=dtype, **kw) for _ in range(layers)]
+    for b, n in enumerate(lens):
+        assert table.admit(n) == b
+        for i, cache in enumerate(caches):
+            g = torch.Generator().manual_seed(100 * n + i)
+            assert cache.store(b, *(torch.randn(n, nkv, hd, generator=g).to(dtype).cuda() for _ in "kv"))
+    return table, caches
+
+
+def _same(a, b, what):
+    for name in ("k_pages", "v_pages", "scores", "slot_pos"):
+        x, y = getattr(a, name), getattr(b, name)
+        if x is None and y is None:
+            continue
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16)), (what, name)
+
+
+@pytest.mark.parametrize("lens,dtype", [((70,), BF), ((3, 47, 17, 64), FP), (tuple(range(1, 20)), BF)])
+@pytest.mark.parametrize("tracked", [False, True])
+def test_decode_batch_is_its_parts(lens, dtype, tracked):
+    """The block on a cache, tracked or not, against its steps called one by one on
+    a twin, bit for bit; of those steps the rows, the attention and the gathered
+    weights against 64 bits."""
+    from tests.test_fused_gpu import _block
+    from ttspipe_amd import fusedlayer, fusedops, nf4gemv
+
+    assert nf4gemv.install() and fusedops.install()
+    block, _ = _block(dtype, True, seed=len(lens))
+    a, ff, an, fn = block.attention, block.feed_forward, block.attention_norm, block.ffn_norm
+    nh, nkv, hd, rows = 4, 2, 128, len(lens) + 1
+    (ta, (ca,)), (tb, (cb,)) = (_streams(nkv, hd, lens, dtype, tracked=tracked) for _ in "ab")
+    ta.step(), tb.step()
+    x = torch.randn(rows, 1, 512, generator=torch.Generator().manual_seed(7)).to(dtype).cuda()
+    freqs = _freqs(128, hd)
+    got = fusedlayer.decode_batch(block, x, freqs, ca)
+    # the steps
+    if rows <= nf4gemv.FUSED_MAX_ROWS:
+        qkv = nf4gemv.matmul_fused(a.wqkv, x, norm_weight=an.weight, eps=an.eps)
+    else:
+        qkv = nf4gemv.matmul(a.wqkv, fusedops.rms_norm(x, an.weight, an.eps))
+    qkv = qkv.view(rows, -1)
+    q = cb.qk_rope_kv(qkv, nh, freqs, q_weight=a.q_norm.weight, k_weight=a.k_norm.weight, eps=a.q_norm.eps)
+    head = qkv.view(rows, -1, hd)
+    for b, n in enumerate(lens):
+        ref, bound = _rope64(head[b, :nh], a.q_norm.weight, freqs[n], 1e-6)
+        assert_within(q[b], ref, rounding(ref, dtype) * (1 + 2**-7) + bound, f"q {b}")
+        at, off = int(tb.block_table[b, n // 16]), n % 16
+        ref, bound = _rope64(head[b, nh:nh + nkv], a.k_norm.weight, freqs[n], 1e-6)
+        assert_within(cb.k_pages[at, :, off], ref, rounding(ref, dtype) * (1 + 2**-7) + bound, f"k {b}")
+        assert torch.equal(cb.v_pages[at, :, off], head[b, nh + nkv:])
+    before = cb.scores.clone() if tracked else None
+    y = cb.attention(q)
+    ref, p, yb, pb = attention64(q, cb.k_pages, cb.v_pages, tb.block_table, tb.slots)
+    assert_within(y, ref, rounding(ref, dtype) * (1 + 2**-7) + yb, "y")
+    if tracked:
+        new = before.double().cpu() + p
+        assert_within(cb.scores, new, new.abs() * 2.0**-24 + pb, "scores")
+        for b, n in enumerate(lens):
+            assert (ca.slot_pos[b, :, : n + 1].cpu() == torch.arange(n + 1)).all()
+    y = y.view(rows, 1, nh * hd)
+    hh = nf4gemv.matmul_norm(a.wo, y, fn.weight, fn.eps, epi=nf4gemv.EPI_RESIDUAL, operand=x)
+    h, hn = hh if hh is not None else (nf4gemv.matmul(a.wo, y, epi=nf4gemv.EPI_RESIDUAL, operand=x), None)
+    h, u = h.view(x.shape), None
+    if hn is None and rows <= nf4gemv.FUSED_MAX_ROWS:
+        u = nf4gemv.matmul_fused(ff.w1, h, norm_weight=fn.weight, eps=fn.eps, module3=ff.w3)
+    if u is None:
+        hn = fusedops.rms_norm(h, fn.weight, fn.eps) if hn is None else hn.view(x.shape)
+        u = nf4gemv.matmul_swiglu(ff.w1, ff.w3, hn)
+        if u is None:
+            u = nf4gemv.matmul(ff.w3, hn, epi=nf4gemv.EPI_SILU_GATE, operand=nf4gemv.matmul(ff.w1, hn))
+    want = nf4gemv.matmul(ff.w2, u, epi=nf4gemv.EPI_RESIDUAL, operand=h)
+    assert np.array_equal(bits(got).reshape(-1), bits(want).reshape(-1))
+    _same(ca, cb, "cache")
+
+
+def test_captured_decode_batch_equals_eager_steps():
+    """Two blocks on tracked caches and their eviction in one graph, replayed as the
+    streams grow past the budget and one ends, the table's own steps between."""
+    from tests.test_fused_gpu import _block
+    from ttspipe_amd import fusedlayer, fusedops, nf4gemv
+
+    assert nf4gemv.install() and fusedops.install()
+    blocks = [_block(BF, True, seed=i)[0] for i in (3, 4)]
+    budget, freqs = 30, _freqs(128, 128)
+    (ta, la), (tb, lb) = (_streams(2, 128, (20, 1, 29), BF, layers=2, tracked=True) for _ in "ab")
+
+    def step(caches, x):
+        for block, cache in zip(blocks, caches):
+            x = fusedlayer.decode_batch(block, x, freqs, cache)
+        for cache in caches:
+            assert cache.evict(budget, sinks=1, recent=6)
+        return x
+
+    g = torch.Generator().manual_seed(2)
+    xs = [torch.randn(4, 1, 512, generator=g).to(BF).cuda() for _ in range(18)]
+    x = xs[0].clone()
+    ta.step(), tb.step()
+    assert np.array_equal(bits(step(la, x)), bits(step(lb, xs[0])))
+    ta.evicted(budget), tb.evicted(budget)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(la, x)
+    for i, new in enumerate(xs[1:]):
+        if i == 7:
+            ta.release(2), tb.release(2)
+        ta.step(), tb.step()
+        x.copy_(new)
+        graph.replay()
+        assert np.array_equal(bits(got), bits(step(lb, new))), i
+        for p, q in zip(la, lb):
+            _same(p, q, i)
+        ta.evicted(budget), tb.evicted(budget)
+    assert ta.rows(0) == budget and ta.rows(1) == 19 and ta.rows(2) == 0
