@@ -164,6 +164,39 @@ def test_evict_lists_the_moves_of_whole_caches(cap, budget, hd, dtype, kind):
     assert _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=17)
 
 
+# ------------------------------------------------------------------ the table
+
+
+def test_the_page_table_waits_for_nothing():
+    """Streams that grow page by page, are cut and end while the GPU is still busy
+    with what was queued before: no call waits, and the tensors end up as the host has them."""
+    table = pc.PageTable(24, 400, 24 * 12, 16)
+    cache = pc.PagedKVCache(table, 1, 64)
+    rows = torch.zeros(20, 1, 64, dtype=BF, device="cuda")
+    a = torch.randn(4096, 4096, device="cuda")
+    states = []
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(20):
+            a = a @ a
+        for i in range(20):
+            assert table.admit(14 + i) == i
+        assert cache.store(3, rows[:17], rows[:17])
+        for step in range(90):
+            table.step()
+            if step in (40, 70):
+                table.evicted(30)
+            if step == 50:
+                table.release(5)
+                assert table.admit(33) == 5
+            states.append((table.block_table.clone(), table.slots.clone(), [list(x) for x in table._held], list(table._rows)))
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    for t, slots, held, n in states:
+        assert t.tolist() == [x + [-1] * (t.shape[1] - len(x)) for x in held] and slots.tolist() == [x - 1 for x in n]
+
+
 # ------------------------------------------------------------------ the block
 
 

@@ -351,8 +351,9 @@ class PageTable:
     position of each sequence, -1: none). One table serves every layer's pools.
 
     The host knows each sequence's row count and position without asking the
-    device: `admit` and `step` add rows, `evicted` cuts them, `release` drops
-    them. Running out of pages raises MemoryError and changes nothing; so does,
+    device, and changes the tensors by work queued on the current stream, which it
+    does not wait for: `admit` and `step` add rows, `evicted` cuts them, `release`
+    drops them. Running out of pages raises MemoryError and changes nothing; so does,
     with ValueError, a row past `max_len` rows or past `max_position` positions
     (the rotary table's rows: a sequence that is evicted from runs on while its
     rows stay few; None: not checked here)."""
@@ -389,13 +390,25 @@ class PageTable:
     def _missing(self, seq: int, rows: int) -> int:
         return max(0, -(-rows // self.page_size) - len(self._held[seq]))
 
-    def _grow(self, seq: int, rows: int) -> None:
-        held, n = self._held[seq], self._missing(seq, rows)
-        if n == 0:
+    def _grow(self, wanted) -> None:
+        """The pages that `wanted`, (sequence, rows) pairs, are missing (there are as many free), in one upload."""
+        new = []
+        for seq, rows in wanted:
+            held = self._held[seq]
+            for _ in range(self._missing(seq, rows)):
+                new.append((seq, len(held), self._free.pop()))
+                held.append(new[-1][2])
+        if not new:
             return
-        new = [self._free.pop() for _ in range(n)]
-        self.block_table[seq, len(held): len(held) + n] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
-        held += new
+        dev = self.block_table.device
+        up = torch.tensor(list(zip(*new)), dtype=torch.int64, pin_memory=dev.type == "cuda").to(dev, non_blocking=True)
+        self.block_table[up[0], up[1]] = up[2].to(torch.int32)
+
+    def _place(self, seq: int, newest: int, active: int) -> None:
+        # (fill_: a number assigned to one element is uploaded, and waited for)
+        self.slots[seq].fill_(newest)
+        self.positions[seq].fill_(newest)
+        self._active[seq].fill_(active)
 
     def admit(self, rows: int):
         """A free sequence with pages for `rows` rows (a prompt's, at positions
@@ -407,10 +420,9 @@ class PageTable:
             return None
         if self._missing(seq, rows) > len(self._free):
             raise MemoryError(f"{self._missing(seq, rows)} pages needed, {len(self._free)} free")
-        self._grow(seq, rows)
+        self._grow([(seq, rows)])
         self._rows[seq] = self._next[seq] = rows
-        self.slots[seq] = self.positions[seq] = rows - 1
-        self._active[seq] = 1
+        self._place(seq, rows - 1, 1)
         return seq
 
     def step(self) -> None:
@@ -423,8 +435,8 @@ class PageTable:
         need = sum(self._missing(i, self._rows[i] + 1) for i in live)
         if need > len(self._free):
             raise MemoryError(f"{need} pages needed, {len(self._free)} free")
+        self._grow((i, self._rows[i] + 1) for i in live)
         for i in live:
-            self._grow(i, self._rows[i] + 1)
             self._rows[i] += 1
             self._next[i] += 1
         self.slots += self._active
@@ -437,14 +449,15 @@ class PageTable:
             raise ValueError("a sequence keeps at least one row")
         self.slots.clamp_(max=budget - 1)
         keep = -(-(budget + 1) // self.page_size)
+        free = len(self._free)
         for seq, n in enumerate(self._rows):
             if n > budget:
                 self._rows[seq] = budget
                 held = self._held[seq]
-                if len(held) > keep:
-                    self.block_table[seq, keep:] = -1
-                    self._free += held[keep:][::-1]
-                    del held[keep:]
+                self._free += held[keep:][::-1]
+                del held[keep:]
+        if len(self._free) > free:  # (no sequence holds more than `keep` pages now)
+            self.block_table[:, keep:].fill_(-1)
 
     def release(self, seq: int) -> None:
         """Sequence `seq` ends: its pages go back to the pool."""
@@ -452,9 +465,8 @@ class PageTable:
             raise ValueError(f"there is no sequence {seq}")
         self._free += self._held[seq][::-1]
         self._held[seq], self._rows[seq], self._next[seq] = [], 0, 0
-        self.block_table[seq] = -1
-        self.slots[seq] = self.positions[seq] = -1
-        self._active[seq] = 0
+        self.block_table[seq].fill_(-1)
+        self._place(seq, -1, 0)
 
 
 class PagedKVCache(nn.Module):
