@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from tests.test_paged import _attention, _cache, _evict, _rope, _store
 from ttspipe_amd import _lib
@@ -43,3 +44,16 @@ def test_workspace_queries_of_sizes_that_no_call_takes():
     for seqs, nkv, cols, page, budget in ((65536, 1, 64, 16, 5), (1, 4097, 64, 16, 5), (1, 1, (1 << 20) + 1, 16, 5),
                                           (2**31 - 1, 2**31 - 1, 2**31 - 1, 2**31 - 1, 5)):
         assert lib.ttsp_paged_evict_work_kib(seqs, nkv, cols, page, budget) == -1, (seqs, nkv, cols)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.to(torch.float16), lambda m: m.to("cpu", torch.float16)])
+def test_a_cast_cache_keeps_its_scores_in_32_bits(cast):
+    """(In 16 bits every call on the cache would be declined.)"""
+    c = pc.PagedKVCache(pc.PageTable(2, 40, 5, 16, device="cpu"), 2, 64, tracked=True)
+    c.scores.copy_(torch.rand(c.scores.shape))
+    want = c.scores.clone()
+    assert cast(c) is c
+    assert c.k_pages.dtype is c.v_pages.dtype is torch.float16 and c.slot_pos.dtype is torch.int32
+    assert c.scores.dtype is torch.float32 and torch.equal(c.scores, want) and "scores" in dict(c.named_buffers())
+    plain = cast(pc.PagedKVCache(c.table, 2, 64))
+    assert plain.scores is None and plain.k_pages.dtype is torch.float16

@@ -484,6 +484,14 @@ class PagedKVCache(nn.Module):
         self.register_buffer("scores", torch.zeros(slots, dtype=torch.float32, device=dev) if tracked else None)
         self.register_buffer("slot_pos", torch.zeros(slots, dtype=torch.int32, device=dev) if tracked else None)
 
+    def _apply(self, fn, *args, **kw):
+        # a module's cast to 16 bits is for the pools: the gathered weights stay fp32
+        scores = self.scores
+        super()._apply(fn, *args, **kw)
+        if scores is not None and self.scores.dtype is not torch.float32:
+            self.scores = scores.to(self.scores.device)
+        return self
+
     def qk_rope_kv(self, qkv, n_head, freqs_cis, *, q_weight=None, k_weight=None, eps: float = 1e-6, out=None):
         """`qk_rope_kv` of each sequence's newest row (qkv: one row a sequence)."""
         t = self.table
