@@ -57,3 +57,14 @@ def test_a_cast_cache_keeps_its_scores_in_32_bits(cast):
     assert c.scores.dtype is torch.float32 and torch.equal(c.scores, want) and "scores" in dict(c.named_buffers())
     plain = cast(pc.PagedKVCache(c.table, 2, 64))
     assert plain.scores is None and plain.k_pages.dtype is torch.float16
+
+
+def test_a_position_past_the_rotary_table_is_refused_before_its_row_is_left_out():
+    t = pc.PageTable(2, 64, 8, 16, device="cpu")
+    c = pc.PagedKVCache(t, 2, 64)
+    t.admit(30)
+    qkv = torch.zeros(2, 8 * 64, dtype=torch.bfloat16)
+    for n in (0, 29):
+        with pytest.raises(ValueError):
+            c.qk_rope_kv(qkv, 4, torch.zeros(n, 32, 2))
+    assert c.qk_rope_kv(qkv, 4, torch.zeros(30, 32, 2)) is None  # (in range: declined, off the GPU)

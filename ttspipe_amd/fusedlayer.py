@@ -252,8 +252,6 @@ def decode_batch(block, x, freqs_cis, cache):
     for linear in (a.wqkv, a.wo, ff.w1, ff.w2, ff.w3):
         if getattr(linear, "bias", None) is not None or not nf4gemv.prepare(linear):
             return None
-    if table.positions_used > freqs_cis.shape[0]:
-        raise ValueError(f"decode_batch: position {table.positions_used - 1} lies past the rotary table")
     an, fn = block.attention_norm, block.ffn_norm
     rows, nh = x.shape[0], a.n_head
     qkv = None

@@ -493,8 +493,12 @@ class PagedKVCache(nn.Module):
         return self
 
     def qk_rope_kv(self, qkv, n_head, freqs_cis, *, q_weight=None, k_weight=None, eps: float = 1e-6, out=None):
-        """`qk_rope_kv` of each sequence's newest row (qkv: one row a sequence)."""
+        """`qk_rope_kv` of each sequence's newest row (qkv: one row a sequence).
+        ValueError where one's position lies past `freqs_cis`: its slot would stay
+        unwritten, and `attention` would read it."""
         t = self.table
+        if t.positions_used > freqs_cis.shape[0]:
+            raise ValueError(f"position {t.positions_used - 1} lies past the rotary table")
         return qk_rope_kv(qkv, n_head, self.k_pages, self.v_pages, t.block_table, t.slots, freqs_cis, t.positions,
                           q_weight=q_weight, k_weight=k_weight, eps=eps, scores=self.scores, slot_pos=self.slot_pos,
                           out=out)
