@@ -4,6 +4,8 @@ bounds of `tests/pageddata.py` unless a test derives its own."""
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -115,6 +117,75 @@ def test_weights_of_more_query_heads_than_are_gathered_at_once(nh, nkv, hd, dtyp
     attention_check(c, y, c.scores, before)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_attention_of_pages_that_sequences_share(page):
+    """A prefix of pages that three sequences read, one of them with a page twice:
+    each gathers weights of its own."""
+    c = Case([600, 600, 600], 8, 2, 128, page, FP, seed=page)
+    n = 320 // page
+    c.table[1, :n] = c.table[2, :n] = c.table[0, :n]
+    c.table[2, n] = c.table[2, 1]
+    before = c.scores.clone()
+    y = pc.attention(c.q, *c.pools(), c.slots, scores=c.scores)
+    attention_check(c, y, c.scores, before)
+
+
+def _longest():
+    """One sequence of the most slots there may be, pages in falling order."""
+    n, page, hd = 1 << 24, 4096, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(n // page, 1, page, hd, generator=g, device="cuda", dtype=FP) for _ in "kv")
+    table = torch.arange(n // page - 1, -1, -1, dtype=torch.int32, device="cuda").view(1, -1)
+    return n, page, hd, g, k, v, table
+
+
+def test_attention_of_the_longest_sequence():
+    """2^24 slots, 64 bits on the GPU. The bounds are those of `attention64`."""
+    n, page, hd, g, k, v, table = _longest()
+    q = torch.randn(1, 2, hd, generator=g, device="cuda", dtype=FP) * 3
+    scores = torch.zeros(1, 1, n, device="cuda")
+    y = pc.attention(q, k, v, table, torch.tensor([n - 1], device="cuda"), scores=scores)
+    K, V = (t.flip(0).reshape(n, hd) for t in (k, v))
+    dots, mag = torch.empty(2, n, dtype=torch.float64, device="cuda"), torch.zeros((), dtype=torch.float64, device="cuda")
+    step = 1 << 20
+    for i in range(0, n, step):
+        rows = K[i:i + step].double()
+        dots[:, i:i + step] = (rows @ q[0].double().t()).t() * hd**-0.5
+        mag = torch.maximum(mag, (rows.abs() @ q[0].double().abs().t()).max() * hd**-0.5)
+    w = torch.softmax(dots, 1)
+    ref, absolute, total = (torch.zeros(2, hd, dtype=torch.float64, device="cuda") for _ in "yab")
+    for i in range(0, n, step):
+        rows = V[i:i + step].double()
+        ref += w[:, i:i + step] @ rows
+        absolute += w[:, i:i + step] @ rows.abs()
+        total += rows.abs().sum(0)
+    e = 2 * (hd + 4) * 2.0**-24 * mag + 2.0**-20 + 2.0**-23 * (n / 8 / 1024 + 64)  # (1024 chunks' sums, then theirs)
+    assert_within(y[0], ref, rounding(ref, FP) * (1 + 2**-7) + absolute * (e + 2.0**-16) + 2.0**-38 * total, "y")
+    assert_within(scores[0, 0], w.sum(0), w.sum(0) * (e + 2.0**-23), "scores")
+
+
+@pytest.mark.parametrize("kind", ["exp", "same"])
+def test_evict_of_the_longest_sequence(kind):
+    n, page, hd, g, k, v, table = _longest()
+    budget, sinks, recent = (1 << 23) + 77, 100, 1000
+    s = torch.rand(1, 1, n, generator=g, device="cuda") if kind == "exp" else torch.ones(1, 1, n, device="cuda")
+    sp = torch.arange(n, dtype=torch.int32, device="cuda").view(1, 1, n).clone()
+    key = s[0, 0].clone()
+    key[:sinks] = key[n - recent:] = math.inf
+    kept = torch.zeros(n, dtype=torch.bool, device="cuda")
+    kept[torch.sort(key, descending=True, stable=True).indices[:budget]] = True
+    src = kept[budget:].nonzero()[:, 0] + budget
+    dst = (~kept[:budget]).nonzero()[:, 0]
+    want = [t.flip(0).reshape(n, hd) for t in (k, v)] + [s[0, 0].clone(), sp[0, 0].clone()]
+    for t in want:
+        t[dst] = t[src]
+    assert pc.evict(k, v, table, torch.tensor([n - 1], device="cuda"), s, sp, torch.tensor([n - 1], device="cuda"), budget,
+                    sinks=sinks, recent=recent)
+    assert len(src) and torch.equal(s[0, 0], want[2]) and torch.equal(sp[0, 0], want[3])
+    for t, w in zip((k, v), want):
+        assert torch.equal(t.flip(0).reshape(n, hd).view(torch.int16), w.view(torch.int16))
+
+
 # --------------------------------------------------------------- the eviction
 
 
@@ -162,6 +233,32 @@ def test_evict_lists_the_moves_of_whole_caches(cap, budget, hd, dtype, kind):
     c, s, sp = _tracked(lens, 2, hd, 16, dtype, seed=cap + budget, kind=kind, cols=cap // 16)
     assert pc.evict_work(len(lens), 2, cap // 16, 16, budget) > 0
     assert _evict(c, s, sp, sp.amax((1, 2)).long(), budget, sinks=3, recent=17)
+
+
+@pytest.mark.parametrize("n,budget", [(700, 300), (3000, 1000), (9000, 2000)])
+def test_captured_evict_in_every_form(n, budget):
+    """Moves listed by 256 and by 1024 threads and in parts, replayed at other lengths: a workspace that
+    earlier replays have used."""
+    c, s, sp = _tracked([n, n], 2, 64, 16, BF, seed=n)
+    first = [t.clone() for t in (c.k, c.v, s, sp)]
+    pos = sp.amax((1, 2)).long()
+    work = torch.full((pc.evict_work(2, 2, c.table.shape[1], 16, budget),), -1, dtype=torch.int32, device="cuda")
+    call = lambda: pc.evict(*c.pools(), c.slots, s, sp, pos, budget, sinks=2, recent=16, work=work)  # noqa: E731
+    assert len(work) and call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for lens in ((n, budget + 1), (5, n), (budget, budget + 40), (n - 1, n), (0, 1), (budget + 2, n // 2)):
+        for a, b in zip((c.k, c.v, s, sp), first):
+            a.copy_(b)
+        c.slots.copy_(torch.tensor([x - 1 for x in lens]))
+        g.replay()
+        k, v, s1, sp1 = (t.clone() for t in first)
+        assert pc.evict(k, v, c.table, c.slots, s1, sp1, pos, budget, sinks=2, recent=16)
+        torch.cuda.synchronize()
+        assert torch.equal(s, s1) and torch.equal(sp, sp1), lens
+        assert np.array_equal(bits(c.k), bits(k)) and np.array_equal(bits(c.v), bits(v)), lens
 
 
 # ------------------------------------------------------------------ the table
