@@ -150,18 +150,6 @@ __device__ __forceinline__ int chunk_size(int n, int count) {
   return count < 2 ? n : (int)((units(n) + count - 1) / count * PG_STEP);
 }
 
-// v plus the lower lanes' v, by shifts within the rows of 16 lanes and two row
-// broadcasts (lanes without a source add 0).
-__device__ __forceinline__ uint32_t lane_prefix(uint32_t v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return v;
-}
-
 // Rows of sequence b, 0 past the last.
 __device__ __forceinline__ int rows_of(const AttnArgs& a, int b) { return b < a.seqs ? a.c.rows(a.SLOT[b]) : 0; }
 

@@ -42,6 +42,18 @@ struct Paged {
   }
 };
 
+// v plus the lower lanes' v, by shifts within the rows of 16 lanes and two row
+// broadcasts (lanes without a source add 0).
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
 // Whether the `cap` words of every (sequence, kv head) lie apart by these strides.
 // (A workgroup adds to its own words, or moves them, while others do to theirs.)
 inline bool words_apart(long long seq, long long head, int seqs, int nkv, long long cap) {

@@ -121,13 +121,7 @@ __device__ __forceinline__ void find_digit(const int* hist, int* wsum, int* pick
     }
     mine += sum[k];
   }
-  int upto = mine;
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xF, 0xF, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xF, 0xF, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xF, 0xF, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xF, 0xF, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xA, 0xF, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xC, 0xF, false);
+  const int upto = (int)lane_prefix((uint32_t)mine);
   if (lane == 63) wsum[wave] = upto;
   __syncthreads();
   int before = upto - mine;
