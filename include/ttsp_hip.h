@@ -635,8 +635,9 @@ int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int bu
 
 /* Cut every sequence of more than `budget` rows (SLOT[b] + 1, int64) down to
  * it, in each kv head by itself: rows with slot_pos < sinks or slot_pos >
- * POS[b] - recent (POS[b], int64: the newest position) come first, then the
- * others by score (NaN lowest, as -inf), ties by the lowest slot, and the first
+ * POS[b] - recent (POS[b], int64: the newest position) come first, and with them
+ * scores of +inf; then the others by score (NaN lowest, as -inf), ties by the
+ * lowest slot, and the first
  * `budget` are kept. Kept rows in slots from `budget` on move, in order, into
  * the free slots below it, with their score and slot_pos; rows that stay, and
  * what slots from `budget` on hold, are not touched. The sequence's next slot is

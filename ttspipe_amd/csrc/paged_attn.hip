@@ -8,8 +8,8 @@
 // Memory bound: every cached row is read once for all the query heads of its
 // kv head (G = nh / nkv flop a byte), so what counts is how many bytes are under
 // way at once. One sequence of 130995 rows (8 kv heads of 128): the first launch
-// 84 us, 6.4 TB/s, the rate of a plain streaming read; 64 of 2048 to 5119: 161 us,
-// 5.9 TB/s; 32 of 200 to 2304, where a workgroup has only three rounds between its
+// 84 us, 6.4 TB/s, the rate of a plain streaming read; 64 of 2048 to 5119: 163 us,
+// 5.8 TB/s; 32 of 200 to 2304, where a workgroup has only three rounds between its
 // first dependent reads and its merge: 36 us, 4.7 TB/s. Cached rows are read past
 // the caches (plain loads: 97 and 181 us for the first two).
 //
@@ -58,7 +58,7 @@ constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of
 // and 8 kv heads of 128, bf16; 512 of them, one round: 49 / 200 / 88).
 constexpr int PG_WGS = 1024;
 // Caches of up to this many slots: a sequence is one chunk, and there is no
-// joining launch (300 rows, alone: 7.6 us; in three chunks and joined: 10.0).
+// joining launch (300 rows, alone: 8.3 us; in three chunks and joined: 10.2).
 constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score

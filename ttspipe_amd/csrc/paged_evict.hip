@@ -1,7 +1,7 @@
 // Eviction from a paged cache by gathered attention weight. For each
 // (sequence, kv head) of n > budget rows, the rows are ranked by
 //   key = +inf where slot_pos < sinks or slot_pos > position - recent,
-//         else the score (NaN counts as -inf),
+//         else the score (NaN counts as -inf; a score of +inf is as good as protected),
 // ties to the lowest slot; the first `budget` are kept. Attention does not
 // care about the order of the slots, so a kept row below `budget` stays where
 // it is, and the j-th kept row from slot `budget` on moves into the j-th free
@@ -19,11 +19,14 @@
 // Up to 8192 slots one workgroup ranks a (sequence, kv head), its keys read once
 // and held in registers, a wave's keys neighbouring slots, so that movers and
 // free slots are listed in order with ballots and one prefix over the waves. A
-// second launch moves the rows, a group of lanes each. Where the cache has
-// little room past the budget the first launch moves them itself; and a
-// sequence only a few rows over its budget, as after a decode step, has its
-// lowest keys taken out one by one instead, while the rows past the budget,
-// which may have to move, are on their way already.
+// second launch moves the rows, a group of lanes each. Where the budget or the
+// cache's room past it is at most EV_INLINE rows the first launch moves them
+// itself, and there a sequence only a few rows over its budget, as after a decode
+// step, has its lowest keys taken out one by one instead, while the rows past the
+// budget, which may have to move, are on their way already. A wider cache is ranked
+// in full for such a step too: 32 sequences of 1025 rows down to 1024 (8 heads)
+// take 4.9 us in tables of 1088 slots, 16.2 in 2304 to 8192, 41 in 16384 and 115 in
+// 65536.
 //
 // In longer caches one workgroup's instructions, not its bytes, set the time
 // (65531 rows a head: 74 us, 25 in parts), so they are ranked in parts of a few thousand
@@ -37,7 +40,9 @@
 // bytes at random places): 8 sequences of 1500 to 8192 rows down to 2048 (8 heads
 // of 128): 12.7 us of ranking, which one workgroup's chain of passes sets, and
 // 20 of moving, about 3.7 TB/s; one of 65531 down to 8192: 5.3 + 9.1 + 12.2 and 14
-// us; 32 of 1025 down to 1024: 5.3 us, a chain of dependent reads.
+// us (the second and third launch read their part twice, and each workgroup of the
+// third clears and scans its bins for every further digit); 32 of 1025 down to 1024
+// in a table of 1088: 5.3 us, a chain of dependent reads.
 #include "paged_common.h"
 
 namespace ttsp {

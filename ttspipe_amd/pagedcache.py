@@ -273,7 +273,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
 
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
-    `attention_work(...)` elements, else allocated per call."""
+    `attention_work(...)` elements, else allocated per call; with `scores` it holds
+    sequences * n_head * the table's slots, whatever the sequences hold."""
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores)
@@ -316,7 +317,9 @@ def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, bud
     """Cut every sequence of more than `budget` rows down to it, in place and in
     each KV head by itself: kept are rows of the first `sinks` positions and of
     the last `recent` ones (up to `positions[b]`, int64, the newest), then those
-    of the largest scores (NaN counts as -inf), ties to the lowest slot. A kept
+    of the largest scores (+inf is as good as protected, NaN counts as -inf), ties
+    to the lowest slot. Rows that no step has attended to yet, a prompt's after
+    `store`, have a score of 0: of those the lowest slots stay. A kept
     row below `budget` stays; the others move, in order, into the free slots
     below it with their score and position. Slots from `budget` on are left as
     they were, and so are `slots`: the caller's next slot is `budget`
