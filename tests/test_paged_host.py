@@ -35,7 +35,7 @@ def test_workspace_queries_of_sizes_that_no_call_takes():
             (65535, 256, 1, 64, 1, 16, 0), (65535, 4096, 8, 128, 1, 16, 0), (20000, 840, 1, 128, 100, 16, 0),  # workgroups
             (1, 65535, 1, 64, 1 << 20, 16, 1),  # 4 TiB of scores
             (65535, 1, 1, 64, 1 << 20, 16, 0), (1, 1, 1, 64, (1 << 20) + 1, 16, 0), (65536, 1, 1, 64, 1, 16, 0),
-            (1, 65536, 1, 64, 1, 16, 0), (1, 1, 1, 256, 1, 16, 0), *[(2**31 - 1,) * 6 + (t,) for t in (0, 1)],
+            (1, 65536, 1, 64, 1, 16, 0), (1, 1, 1, 256, 1, 16, 0), (1, 5000, 5000, 64, 1, 16, 0), *[(2**31 - 1,) * 6 + (t,) for t in (0, 1)],
             (2**31 - 1, 2**31 - 1, 1, 128, 2**31 - 1, 16, 1)):
         assert lib.ttsp_paged_attention_work_kib(seqs, nh, nkv, hd, cols, page, tracked) == -1, (seqs, nh, cols)
         with pytest.raises(ValueError):

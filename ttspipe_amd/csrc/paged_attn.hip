@@ -663,7 +663,7 @@ extern "C" int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head
   if (seqs < 1 || nkv < 1 || nh < nkv || cols < 1 || page_size < 1 || head_dim < 1) return 0;
   AttnPlan p;
   const long long cap = (long long)cols * page_size;
-  if (seqs > 65535 || nh > 65535 || head_dim > 128 || cap > TTSP_PAGED_MAX_SLOTS ||
+  if (seqs > 65535 || nh > 65535 || nkv > 4096 || head_dim > 128 || cap > TTSP_PAGED_MAX_SLOTS ||
       !attn_plan(seqs, nh, nkv, head_dim, cap, tracked != 0, &p))
     return -1;
   return (int)((p.parts + p.scores + 255) / 256);

@@ -224,7 +224,8 @@ def decode_batch(block, x, freqs_cis, cache):
     `freqs_cis` (positions, head_dim / 2, 2) is the whole rotary table and
     `cache` this layer's `pagedcache.PagedKVCache`. Returns the blocks' outputs,
     shaped as x; a row of the table that holds no sequence gives what its x
-    gives with an attention of zeros. None when declined.
+    gives with an attention of zeros. None when declined; ValueError where a
+    position lies past `freqs_cis`.
 
     RMSNorm, wqkv, `pagedcache.qk_rope_kv`, `pagedcache.attention` (a tracked
     cache gathers its weights), wo with the residual and the FFN norm, w1 and w3
@@ -238,8 +239,7 @@ def decode_batch(block, x, freqs_cis, cache):
     from ttspipe_amd import fusedops, nf4gemv
 
     a, ff = block.attention, block.feed_forward
-    table = cache.table
-    if not _lib.gpu_present() or x.dim() != 3 or x.shape[1] != 1 or x.shape[0] != table.slots.shape[0]:
+    if not _lib.gpu_present() or x.dim() != 3 or x.shape[1] != 1 or x.shape[0] != cache.table.slots.shape[0]:
         return None
     if x.dtype not in (torch.float16, torch.bfloat16) or x.device.type != "cuda" or not x.is_contiguous():
         return None
