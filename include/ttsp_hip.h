@@ -89,6 +89,28 @@ typedef struct ttsp_paged_cache {
   int seqs, cols, pages, page_size, n_kv, head_dim, dtype;
 } ttsp_paged_cache;
 
+/* What ttsp_penalize does to rows of logits (no counterpart in the reference).
+ * Each part may be NULL. HIST: the tokens seen, int32 or (hist_64) int64, `hist`
+ * entries a row, rows hist_row_stride apart; LEN: how many of each row's first
+ * entries count (int32, or int64 with len_64; cut to 0 .. hist; NULL: all); an
+ * entry outside [0, vocab) counts for no token. REP, FREQ, PRES (fp32): the
+ * penalties, one a row (*_rows != 0) or one for all rows. BIAS: bias_dtype
+ * TTSP_F32 or the logits' type, rows bias_row_stride apart (0: one for all).
+ * MASK: bit t % 32 of word t / 32 of a row (mask_row_stride words apart, 0: one
+ * for all) is 0 where token t is not allowed. Strides are in elements and not
+ * negative; every array has its elements' alignment. */
+typedef struct ttsp_penalties {
+  const void* HIST;
+  const void* LEN;
+  const float* REP;
+  const float* FREQ;
+  const float* PRES;
+  const void* BIAS;
+  const void* MASK;
+  long long hist_row_stride, bias_row_stride, mask_row_stride;
+  int hist, hist_64, len_64, rep_rows, freq_rows, pres_rows, bias_dtype;
+} ttsp_penalties;
+
 #ifndef TTSP_HIP_TYPES_ONLY
 
 /* Y[N][M] = epi(X[N][K] . dequant(W)^T). N == 1 runs the HBM-bound GEMV (rows
@@ -432,6 +454,17 @@ int ttsp_sample_max_top_k(void);
  * is that fallback for top_k above MAX_TOP_K). */
 int ttsp_sample_max_vocab(void);
 
+/* Penalties on `rows` rows of `vocab` logits (dtype TTSP_F16, TTSP_BF16 or
+ * TTSP_F32; row strides in elements): with c the times a token occurs in its
+ * row's history, x = X[row][t]; where c > 0, x = x / REP (x > 0) or x * REP, then
+ * x - (FREQ c + PRES); x + BIAS; -inf where the mask's bit is 0; fp32, one
+ * rounding an operation in this order, the last to dtype. Y may be X (with X's
+ * stride) and otherwise overlaps no input; nothing outside its rows is written.
+ * vocab <= 2^30. Replaces: nothing (the reference's sampler,
+ * app/engine/fusedsample.py:28-223, has temperature, top-k and top-p). */
+int ttsp_penalize(const ttsp_penalties* penalties, const void* X, long long x_row_stride, void* Y,
+                  long long y_row_stride, int rows, int vocab, int dtype, void* stream);
+
 /* Cache positions per attention chunk (64). Replaces: CHUNK,
  * app/engine/fusedlayer.py:40. */
 int ttsp_attn_chunk(void);
@@ -627,6 +660,18 @@ int ttsp_paged_attention_work_kib(int seqs, int nh, int nkv, int head_dim, int c
  * + attn_combine, app/engine/fusedlayer.py:95-159, for several sequences. */
 int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
                          const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
+
+/* ttsp_paged_attention through a sliding window: of the rows of sequence b the
+ * keys are those in slots j < sinks and j > SLOT[b] - window (window >= 1,
+ * sinks >= 0), and only they and their pages' table entries are read. Replaces:
+ * nothing (the reference's attention sees the whole cache). */
+int ttsp_paged_attention_window(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
+                                const long long* SLOT, void* Y, int nh, float scale, int window, int sinks,
+                                float* work, void* stream);
+
+/* KiB of ttsp_paged_attention_window's workspace, as ttsp_paged_attention_work_kib. */
+int ttsp_paged_attention_window_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size,
+                                         int window, int sinks, int tracked);
 
 /* KiB of ttsp_paged_evict's workspace (host-only; 0: none is needed, where no
  * sequence can have more than 256 rows to move, in caches of up to 8192 slots; -1: no

@@ -54,6 +54,14 @@ class PagedCache(ctypes.Structure):
                 *((name, _i) for name in ("seqs", "cols", "pages", "page_size", "n_kv", "head_dim", "dtype"))]
 
 
+class Penalties(ctypes.Structure):
+    """`ttsp_penalties`: what `ttsp_penalize` does to rows of logits."""
+
+    _fields_ = [*((name, _vp) for name in ("HIST", "LEN", "REP", "FREQ", "PRES", "BIAS", "MASK")),
+                *((name, _ll) for name in ("hist_row_stride", "bias_row_stride", "mask_row_stride")),
+                *((name, _i) for name in ("hist", "hist_64", "len_64", "rep_rows", "freq_rows", "pres_rows", "bias_dtype"))]
+
+
 #: Most slots a sequence of a paged cache has (`TTSP_PAGED_MAX_SLOTS`).
 PAGED_MAX_SLOTS = 1 << 24
 #: Longest row stride of its pools, in elements (`TTSP_PAGED_MAX_ROW_STRIDE`).
@@ -121,6 +129,8 @@ SIGNATURES: dict[str, list] = {
     "ttsp_sample_topk": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "ttsp_sample_max_top_k": [],
     "ttsp_sample_max_vocab": [],
+    # (the penalties: the address of a Penalties, or its bytes)
+    "ttsp_penalize": [_vp, _vp, _ll, _vp, _ll, _i, _i, _i, _vp],
     "ttsp_embed_sum": [_vp, _vp, _i, _i, _i, _vp, _i, _vp],
     "ttsp_embed_sum_rows": [_vp, _vp, _ll, _i, _i, _i, _i, _vp, _i, _vp],
     "ttsp_argmax": [_vp, _i, _i, _vp, _vp],
@@ -137,6 +147,8 @@ SIGNATURES: dict[str, list] = {
     "ttsp_paged_store": [_vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _vp],
     "ttsp_paged_attention_work_kib": [_i, _i, _i, _i, _i, _i, _i],
     "ttsp_paged_attention": [_vp, _vp, _ll, _vp, _vp, _i, _f, _vp, _vp],
+    "ttsp_paged_attention_window_work_kib": [_i, _i, _i, _i, _i, _i, _i, _i, _i],
+    "ttsp_paged_attention_window": [_vp, _vp, _ll, _vp, _vp, _i, _f, _i, _i, _vp, _vp],
     "ttsp_paged_evict_work_kib": [_i, _i, _i, _i, _i],
     "ttsp_paged_evict": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
 }
@@ -217,6 +229,19 @@ def stream() -> int:
     if all(get):
         _raw_stream = get
     return st
+
+
+def launch(what: str, dev: int, *args) -> None:
+    """`what` of the library on the current stream of device `dev`."""
+    import torch
+
+    fn = getattr(lib(), what)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream())
+    check(rc, what)
 
 
 def check(rc: int, what: str) -> None:

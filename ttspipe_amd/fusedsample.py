@@ -13,9 +13,15 @@ sampling from the truncated, tempered distribution (reference:
 fusedsample.py:1-19, 225-257). The cumulative mass is summed in fp32 where the
 fork's fp16 cumsum rounds, so a draw whose mass lands exactly on the top-p
 boundary can differ; the distribution is the same.
+
+`penalize` goes before it: penalties for the tokens that a row's history
+holds, biases and a grammar's mask, for the rows of several streams at once
+(the reference's sampler has none of them).
 """
 
 from __future__ import annotations
+
+import struct
 
 from ttspipe_amd import _lib
 
@@ -64,4 +70,113 @@ def sample(logits, temperature, top_p, top_k, uniform=None):
     rc = _lib.lib().ttsp_sample_topk(row.data_ptr(), row.numel(), dt, temp.data_ptr(), topp.data_ptr(),
                                      topk.data_ptr(), uniform.contiguous().data_ptr(), out.data_ptr(), _lib.stream())
     _lib.check(rc, "ttsp_sample_topk")
+    return out
+
+
+#: `ttsp_penalties`' fields in order (`_lib.Penalties` names them).
+_PENALTIES = struct.Struct("@7P3q7i4x")
+
+
+def pack_mask(allowed):
+    """The words `penalize` takes as `mask` (int32, (..., ceil(V / 32))) from a
+    boolean tensor (..., V): bit t % 32 of word t // 32 is allowed[..., t]. Torch
+    operations, for programs whose grammar does not write the words itself."""
+    import torch
+
+    v = allowed.shape[-1]
+    bits = torch.nn.functional.pad(allowed.to(torch.int64), (0, -v % 32)).unflatten(-1, (-1, 32))
+    words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+def _rows_of(t, shapes, what):
+    """(address, row stride) of a tensor of one of `shapes` with a contiguous last axis."""
+    if t.shape not in shapes or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} must have one of the shapes {[tuple(s) for s in shapes]} and a contiguous last axis")
+    return t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
+
+
+def penalize(logits, history=None, *, lengths=None, repetition=None, frequency=None, presence=None, bias=None,
+             mask=None, out=None):
+    """Logits (rows, V) or (V,) of 16 or 32 bits as the sampler should see them, in
+    one launch: with c the number of times token t occurs in its row's history,
+
+        x = logit;  where c > 0:  x = x / repetition if x > 0 else x * repetition,
+        x -= frequency * c + presence;  x += bias;  -inf where the mask forbids t
+
+    in fp32 with one rounding to the logits' type at the end. Every part may be
+    left out. `history` int32 or int64 (rows, H), or (H,) for all rows: a token
+    outside 0 .. V - 1 (-1 for padding) counts for none; `lengths` int32 or int64
+    (rows,): only so many of a row's first entries count (values outside
+    0 .. H are cut to it). `repetition`, `frequency`, `presence`: fp32, one value a
+    row or one in all, on the device, so that a captured graph's can be changed in
+    place. `bias` fp32 or of the logits' type, (rows, V) or (V,). `mask` int32
+    (rows, ceil(V / 32)) or (ceil(V / 32),): bit t % 32 of word t // 32 set where
+    t is allowed (`pack_mask`); a row that allows nothing is -inf throughout, which
+    `sample` has no draw for.
+
+    Returns the new logits, in `out` if given: the logits themselves, or a tensor
+    of their shape and type that overlaps no input. None where the kernel does not
+    take the logits (no GPU, another type, a last axis that is not contiguous);
+    ValueError for parts that do not fit them. Work is queued on the current
+    stream of the logits' device; with `out` nothing is allocated."""
+    import torch
+
+    dt = _lib.dtype_code(logits.dtype)
+    if not _lib.gpu_present() or dt is None or logits.dim() not in (1, 2) or logits.get_device() < 0:
+        return None
+    dev, vocab = logits.get_device(), logits.shape[-1]
+    rows = logits.shape[0] if logits.dim() == 2 else 1
+    x_row = logits.stride(0) if logits.dim() == 2 and rows > 1 else vocab
+    if vocab > 1 << 30 or rows > 1 << 24 or rows * -(-vocab // 1024) > 0xffffff or (vocab > 1 and logits.stride(-1) != 1):
+        return None
+    for t in (history, lengths, repetition, frequency, presence, bias, mask):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("every part must be on the logits' device")
+    hist = hp = hs = h64 = lp = l64 = 0
+    if history is not None:
+        if history.dtype not in (torch.int32, torch.int64) or history.dim() not in (1, 2):
+            raise ValueError("history must be an int32 or int64 tensor (rows, H) or (H,)")
+        hist, h64 = history.shape[-1], int(history.dtype is torch.int64)
+        hp, hs = _rows_of(history, ((rows, hist), (1, hist), (hist,)), "history")
+        if hist >= 1 << 31:
+            raise ValueError("a history holds at most 2^31 - 1 tokens")
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (rows,) or not lengths.is_contiguous():
+            raise ValueError("lengths must be a contiguous int32 or int64 tensor (rows,)")
+        lp, l64 = lengths.data_ptr(), int(lengths.dtype is torch.int64)
+    scalars = []
+    for t, what in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
+        if t is None:
+            scalars.append((0, 0))
+            continue
+        if t.dtype is not torch.float32 or t.dim() > 1 or t.numel() not in (rows, 1) or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous fp32 tensor of one value a row, or of one")
+        scalars.append((t.data_ptr(), int(t.numel() > 1)))
+    bp = bs = mp = ms = 0
+    if bias is not None:
+        if bias.dtype not in (torch.float32, logits.dtype):
+            raise ValueError("bias must be fp32 or of the logits' type")
+        bp, bs = _rows_of(bias, ((rows, vocab), (1, vocab), (vocab,)), "bias")
+    if mask is not None:
+        words = -(-vocab // 32)
+        if mask.dtype is not torch.int32:
+            raise ValueError("mask must hold int32 words")
+        mp, ms = _rows_of(mask, ((rows, words), (1, words), (words,)), "mask")
+    if out is None:
+        out = logits.new_empty(logits.shape)
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (vocab > 1 and out.stride(-1) != 1):
+        raise ValueError("out must have the logits' shape, type and device, and a contiguous last axis")
+    y_row = out.stride(0) if logits.dim() == 2 and rows > 1 else vocab
+    if not rows or not vocab:
+        return out
+    if rows > 1 and y_row < vocab:
+        raise ValueError("out's rows must not overlap")
+    xp, yp, size = logits.data_ptr(), out.data_ptr(), logits.element_size()
+    if (xp != yp or x_row != y_row) and xp < yp + ((rows - 1) * y_row + vocab) * size and yp < xp + ((rows - 1) * x_row + vocab) * size:
+        raise ValueError("out must be the logits themselves or not overlap them")
+    (rp, rr), (fp, fr), (pp, pr) = scalars
+    block = _PENALTIES.pack(hp, lp, rp, fp, pp, bp, mp, hs, bs, ms, hist, h64, l64, rr, fr, pr,
+                            dt if bias is None else _lib.dtype_code(bias.dtype))
+    _lib.launch("ttsp_penalize", dev, block, xp, x_row, yp, y_row, rows, vocab, dt)
     return out

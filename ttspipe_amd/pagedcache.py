@@ -126,18 +126,6 @@ def _vector(t, dtype, n, dev) -> bool:
     return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.get_device() == dev
 
 
-def _launch(what, dev, *args):
-    """`what` of the library on the current stream of device `dev`."""
-    fn = getattr(_lib.lib(), what)
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(*args, _lib.stream())
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _lib.stream())
-    if rc:
-        raise RuntimeError(f"{what} failed: hipError_t {rc}")
-
-
 def _out_ok(out, shape, dtype, dev) -> bool:
     return (out.shape == shape and out.dtype is dtype and out.get_device() == dev and out.is_contiguous()
             and not out.data_ptr() % 16)
@@ -199,7 +187,7 @@ def qk_rope_kv(qkv, n_head, k_pages, v_pages, block_table, slots, freqs_cis, pos
     elif not _out_ok(out, (rows, n_head, hd), dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (rows, n_head, head_dim) tensor of the cache's dtype")
     if rows:
-        _launch("ttsp_paged_qk_rope_kv", dev, block, qp, step if rows > 1 else width, qw, kw, eps, fp, ftype, n_freqs,
+        _lib.launch("ttsp_paged_qk_rope_kv", dev, block, qp, step if rows > 1 else width, qw, kw, eps, fp, ftype, n_freqs,
                 0 if positions is None else positions.data_ptr(), 0 if seqs is None else seqs.data_ptr(),
                 slots.data_ptr(), out.data_ptr(), n_head, rows)
         _stats["rows"] += 1
@@ -229,22 +217,32 @@ def store(k, v, k_pages, v_pages, block_table, slots, *, positions=None, seqs=No
     if kl != 1 or vl != 1 or kr % 8 or kh % 8 or vr % 8 or vh % 8 or kp % 16 or vp % 16:
         return _declined()
     if rows:
-        _launch("ttsp_paged_store", dev, block, kp, kr, kh, vp, vr, vh, 0 if positions is None else positions.data_ptr(),
+        _lib.launch("ttsp_paged_store", dev, block, kp, kr, kh, vp, vr, vh, 0 if positions is None else positions.data_ptr(),
                 0 if seqs is None else seqs.data_ptr(), slots.data_ptr(), rows)
         _stats["rows"] += 1
     return True
 
 
 @functools.lru_cache(maxsize=256)
-def _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked) -> int:
+def _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked, window=None, sinks=0) -> int:
+    if window is not None:
+        return _lib.lib().ttsp_paged_attention_window_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
+                                                               window, sinks, int(tracked))
     return _lib.lib().ttsp_paged_attention_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
                                                     int(tracked))
 
 
+def _window(window, sinks):
+    """A window and its sinks as the library takes them (a longer one than any table is wide changes nothing)."""
+    if sinks < 0 or (window is None and sinks) or (window is not None and window < 1):
+        raise ValueError("a window has at least one row, and its sinks are not negative")
+    return None if window is None else min(int(window), _lib.PAGED_MAX_SLOTS), min(int(sinks), _lib.PAGED_MAX_SLOTS)
+
+
 def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, columns: int, page_size: int,
-                   tracked: bool = False) -> int:
+                   tracked: bool = False, *, window: int | None = None, sinks: int = 0) -> int:
     """fp32 elements of `attention`'s workspace; ValueError where `attention` declines sizes like these."""
-    kib = _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked)
+    kib = _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked, *_window(window, sinks))
     if kib < 0:
         raise ValueError("too many heads or slots for one call, or the workspace would take more than 2 TiB")
     return kib * 256
@@ -261,7 +259,7 @@ def _workspace(work, need, dtype, like):
 
 
 def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = None, scores=None, out=None,
-              work=None):
+              work=None, window: int | None = None, sinks: int = 0):
     """One new token of each sequence over its cached rows: q (sequences, n_head,
     D), a sequence's heads contiguous, over slots 0 .. slots[b] (cut to the
     table's width), query head h with KV head h // (n_head / n_local_heads), the
@@ -271,10 +269,18 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     value in an fp16 cache, which may give NaN, and scores beyond 2e38, which
     count as infinite.
 
+    With a `window`, a sequence's token sees only slots j with j < sinks or
+    j > slots[b] - window: the first rows stay visible, the others slide out. Only
+    those rows and their pages' table entries are read, so the pages in between
+    may have been given back (`PageTable.slide`). Slots have to be in the order of
+    their positions: a cache that `evict` has moved rows in has no window.
+
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
     `attention_work(...)` elements, else allocated per call; with `scores` it holds
     sequences * n_head * the table's slots, whatever the sequences hold."""
+    if window is not None or sinks:
+        window, sinks = _window(window, sinks)
     if not _lib.gpu_present():
         return _declined()
     c = _pool(k_pages, v_pages, block_table, scores)
@@ -289,7 +295,7 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
             or last != 1 or (nh > 1 and head_step != hd) or (seqs > 1 and (step < nh * hd or step % 8)) or qp % 16
             or not _vector(slots, torch.int64, seqs, dev)):
         return _declined()
-    kib = _attention_kib(seqs, nh, nkv, hd, cols, page, scores is not None)
+    kib = _attention_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks)
     if kib < 0:
         return _declined()
     if out is None:
@@ -297,8 +303,11 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     elif not _out_ok(out, shape, dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
     work = _workspace(work, kib * 256, torch.float32, q)
-    _launch("ttsp_paged_attention", dev, block, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
-            hd**-0.5 if scale is None else scale, 0 if work is None else work.data_ptr())
+    what, form = "ttsp_paged_attention", ()
+    if window is not None:
+        what, form = "ttsp_paged_attention_window", (window, sinks)
+    _lib.launch(what, dev, block, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
+                hd**-0.5 if scale is None else scale, *form, 0 if work is None else work.data_ptr())
     _stats["attention"] += 1
     return out
 
@@ -342,7 +351,7 @@ def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, bud
         return _declined()
     if cols * page > budget:  # else no sequence can be longer
         work = _workspace(work, evict_work(seqs, nkv, cols, page, budget), torch.int32, k_pages)
-        _launch("ttsp_paged_evict", dev, block, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
+        _lib.launch("ttsp_paged_evict", dev, block, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
                 0 if work is None else work.data_ptr())
     _stats["evict"] += 1
     return True
