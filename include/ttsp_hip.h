@@ -89,6 +89,20 @@ typedef struct ttsp_paged_cache {
   int seqs, cols, pages, page_size, n_kv, head_dim, dtype;
 } ttsp_paged_cache;
 
+/* Prefixes that sequences of a paged cache share (no counterpart in the
+ * reference): row p of `table` (int32, table_stride apart, `cols` entries) names
+ * the pages of prefix p in the cache's pools, SLOT[p] (int64) is its newest slot
+ * (-1: it holds nothing), and OF[b] (int32) is the prefix of sequence b (outside
+ * [0, count): none). count is at most 256, cols * page_size at most
+ * TTSP_PAGED_MAX_SLOTS. */
+typedef struct ttsp_paged_prefix {
+  const int* table;
+  const long long* SLOT;
+  const int* OF;
+  long long table_stride;
+  int count, cols;
+} ttsp_paged_prefix;
+
 /* What ttsp_penalize does to rows of logits (no counterpart in the reference).
  * Each part may be NULL. HIST: the tokens seen, int32 or (hist_64) int64, `hist`
  * entries a row, rows hist_row_stride apart; LEN: how many of each row's first
@@ -530,6 +544,21 @@ int ttsp_prefill_attention_causal(const void* Q, long long q_seq_stride, long lo
                                   const long long* pos, void* Y, int S, int nh, int nkv, int L, float scale,
                                   int dtype, float* work, int splits, void* stream);
 
+/* ttsp_prefill_attention_causal through a sliding window with sinks: the row at
+ * position p sees keys j <= p with j < sinks or j > p - window (window >= 1,
+ * sinks >= 0), none at or past L; a row that sees none gives NaN. splits as
+ * ttsp_prefill_attention_window_splits says, or 1. Replaces: nothing (the
+ * reference's masks are causal, app/engine/fastpath.py:244-268). */
+int ttsp_prefill_attention_window(const void* Q, long long q_seq_stride, long long q_head_stride, const void* K,
+                                  long long k_seq_stride, long long k_head_stride, const void* V,
+                                  long long v_seq_stride, long long v_head_stride, const long long* pos, void* Y,
+                                  int S, int nh, int nkv, int L, int window, int sinks, float scale, int dtype,
+                                  float* work, int splits, void* stream);
+
+/* Key splits that ttsp_prefill_attention_window's workspace is for (host-only), as
+ * ttsp_prefill_attention_splits. */
+int ttsp_prefill_attention_window_splits(int S, int nkv, int L, int window, int sinks);
+
 /* out[d] = round(sum_{c < ntok} E[(c*vocab + tok[c]) * D + d]) (tok int32 on the
  * device, clamped into [0, vocab)). Replaces: the codebook-embedding lookup of
  * a decode step (app/engine/graphs.py:124-131 via the fork's _fast_embed /
@@ -672,6 +701,19 @@ int ttsp_paged_attention_window(const ttsp_paged_cache* cache, const void* Q, lo
 /* KiB of ttsp_paged_attention_window's workspace, as ttsp_paged_attention_work_kib. */
 int ttsp_paged_attention_window_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size,
                                          int window, int sinks, int tracked);
+
+/* ttsp_paged_attention where sequences share prefixes: sequence b attends over the
+ * rows of prefix OF[b] that lie in a page and over its own, the latter through the
+ * window where window > 0 (0: all of them; sinks >= 0). A prefix's rows are read
+ * once for the sequences that share them. With scores, the own slots' weights are
+ * added to them. work: ttsp_paged_attention_prefix_work_kib() KiB. Replaces: nothing. */
+int ttsp_paged_attention_prefix(const ttsp_paged_cache* cache, const ttsp_paged_prefix* prefix, const void* Q,
+                                long long q_seq_stride, const long long* SLOT, void* Y, int nh, float scale,
+                                int window, int sinks, float* work, void* stream);
+
+/* KiB of ttsp_paged_attention_prefix's workspace (host-only; -1: no such call is taken). */
+int ttsp_paged_attention_prefix_work_kib(int seqs, int nh, int nkv, int head_dim, int cols, int page_size,
+                                         int prefixes, int prefix_cols, int window, int sinks, int tracked);
 
 /* KiB of ttsp_paged_evict's workspace (host-only; 0: none is needed, where no
  * sequence can have more than 256 rows to move, in caches of up to 8192 slots; -1: no

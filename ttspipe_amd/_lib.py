@@ -54,6 +54,12 @@ class PagedCache(ctypes.Structure):
                 *((name, _i) for name in ("seqs", "cols", "pages", "page_size", "n_kv", "head_dim", "dtype"))]
 
 
+class PagedPrefix(ctypes.Structure):
+    """`ttsp_paged_prefix`: prefixes that a paged cache's sequences share."""
+
+    _fields_ = [("table", _vp), ("SLOT", _vp), ("OF", _vp), ("table_stride", _ll), ("count", _i), ("cols", _i)]
+
+
 class Penalties(ctypes.Structure):
     """`ttsp_penalties`: what `ttsp_penalize` does to rows of logits."""
 
@@ -66,6 +72,9 @@ class Penalties(ctypes.Structure):
 PAGED_MAX_SLOTS = 1 << 24
 #: Longest row stride of its pools, in elements (`TTSP_PAGED_MAX_ROW_STRIDE`).
 PAGED_MAX_ROW_STRIDE = 1 << 24
+
+#: Most prefixes its sequences may share in one call.
+PAGED_MAX_PREFIXES = 256
 
 #: `ttsp_fast_steps`' barrier words and the index of its failed-wait count.
 FAST_SYNC_WORDS, FAST_SYNC_FAILED = 192, 128
@@ -126,6 +135,9 @@ SIGNATURES: dict[str, list] = {
                                      _i, _vp, _i, _vp],
     "ttsp_prefill_attention_causal": [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i,
                                       _vp, _i, _vp],
+    "ttsp_prefill_attention_window": [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _f,
+                                      _i, _vp, _i, _vp],
+    "ttsp_prefill_attention_window_splits": [_i, _i, _i, _i, _i],
     "ttsp_sample_topk": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "ttsp_sample_max_top_k": [],
     "ttsp_sample_max_vocab": [],
@@ -149,6 +161,8 @@ SIGNATURES: dict[str, list] = {
     "ttsp_paged_attention": [_vp, _vp, _ll, _vp, _vp, _i, _f, _vp, _vp],
     "ttsp_paged_attention_window_work_kib": [_i, _i, _i, _i, _i, _i, _i, _i, _i],
     "ttsp_paged_attention_window": [_vp, _vp, _ll, _vp, _vp, _i, _f, _i, _i, _vp, _vp],
+    "ttsp_paged_attention_prefix_work_kib": [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i],
+    "ttsp_paged_attention_prefix": [_vp, _vp, _vp, _ll, _vp, _vp, _i, _f, _i, _i, _vp, _vp],
     "ttsp_paged_evict_work_kib": [_i, _i, _i, _i, _i],
     "ttsp_paged_evict": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
 }

@@ -47,13 +47,15 @@
 // runs of 16 slots are put side by side: a sequence then has fewer, virtual rows,
 // which chunks are cut from, and a gap of slots that is added to those behind the
 // sinks' runs before they become addresses; what the runs hold besides is masked.
+// Over shared prefixes (PG_PREFIX; paged_prefix.hip has their kernel): a sequence's
+// own rows leave partial sums only, which the second launch joins with its prefix's.
 #pragma once
 
 #include "paged_common.h"
 
 namespace ttsp {
 
-enum : int { PG_TRACK = 1, PG_WINDOW = 2 };
+enum : int { PG_TRACK = 1, PG_WINDOW = 2, PG_PREFIX = 4 };
 
 typedef __bf16 pg_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_f16x8 __attribute__((ext_vector_type(8)));
@@ -92,7 +94,36 @@ struct AttnArgs {
   float scale2;  // scale * log2(e)
   int nh, seqs, target;  // target: chunks that fill the GPU (0: chunk b is the whole sequence b)
   int window, sinks;     // PG_WINDOW: at least 1 and 0, at most the table's slots
+  // PG_PREFIX
+  const int* far_table;  // [prefixes][far_cols] by far_stride
+  long long far_stride;
+  const long long* FAR_SLOT;  // [prefixes]
+  const int* OF;              // [seqs]: the sequence's prefix, outside 0 .. prefixes - 1: none
+  int prefixes, far_cols, far_target, far_tile;  // far_tile: query rows of a kv head a prefix workgroup takes
+  size_t far_base;  // rows of PM, PL, PACC before the prefixes'
+  int4* DESC;       // [seqs]: where its prefix's sums are (Far), where it has one that holds a row
+
+  __device__ __forceinline__ int far_rows(int p) const {
+    const long long slot = FAR_SLOT[p];
+    const int cap = far_cols << c.shift;
+    return slot < 0 ? 0 : slot < cap ? (int)slot + 1 : cap;
+  }
 };
+
+// A sequence's prefix: `count` chunks, chunk k in item first + k * tiles + (its row / far_tile);
+// an item holds far_tile rows (the query heads of one sequence after the other's) of each kv head.
+struct Far {
+  int first, count, tiles, row;
+};
+__device__ __forceinline__ Far far_of(const AttnArgs& a, int b) {
+  Far f{0, 0, 1, 0};
+  const int p = a.OF[b];
+  if ((unsigned)p < (unsigned)a.prefixes && a.far_rows(p) > 0) {
+    const int4 d = a.DESC[b];
+    f = Far{d.x, d.y, d.z, d.w};
+  }
+  return f;
+}
 
 // What a window leaves of a sequence's rows: virtual row j is slot j + (j < sinks16 ? 0 : gap),
 // and rows m0 .. m1 - 1 are no keys (they share a run of 16 slots with one).
@@ -479,7 +510,7 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   for (int d = 0; d < DC; ++d) *reinterpret_cast<f32x4*>(os + lr * D + 16 * d + 4 * lg) = o[d];
   __syncthreads();
   const float* const all = reinterpret_cast<const float*>(lds);
-  const bool alone = ck.count == 1;
+  const bool alone = ck.count == 1 && !(FORM & PG_PREFIX);
   for (int i = tid; i < heads * D; i += 64 * PG_WAVES) {
     const int g = i / D, d = i % D;
     float m = PG_NONE;
@@ -540,17 +571,32 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   }
 }
 
-// The reference and sum of one query head over a sequence's chunks, by a wave;
+// Row of PM, PL and PACC of query head `head`'s c-th part: its own chunks', then its prefix's.
+template <int FORM>
+__device__ __forceinline__ size_t part_row(const AttnArgs& a, const Chunk& ck, const Far& far, int head, int c) {
+  if constexpr ((FORM & PG_PREFIX) != 0) {
+    if (c >= ck.count) {
+      const int group = a.nh / a.c.nkv, row = far.row + head % group;
+      const size_t item = far.first + (size_t)(c - ck.count) * far.tiles + row / a.far_tile;
+      return a.far_base + (item * a.c.nkv + head / group) * a.far_tile + row % a.far_tile;
+    }
+  }
+  return (size_t)(ck.first + c) * a.nh + head;
+}
+
+// The reference and sum of one query head over a sequence's `count` parts, by a wave;
 // uniform. den < 0: no key.
-__device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, int head, int lane, float* m, float* den) {
+template <int FORM>
+__device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, const Far& far, int count, int head, int lane,
+                                          float* m, float* den) {
   float mx = PG_NONE;
-  for (int c = lane; c < ck.count; c += 64) mx = fmaxf(mx, a.PM[(size_t)(ck.first + c) * a.nh + head]);
+  for (int c = lane; c < count; c += 64) mx = fmaxf(mx, a.PM[part_row<FORM>(a, ck, far, head, c)]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
   float l = 0.0f;
   bool any = false;
-  for (int c = lane; c < ck.count; c += 64) {
-    const size_t at = (size_t)(ck.first + c) * a.nh + head;
+  for (int c = lane; c < count; c += 64) {
+    const size_t at = part_row<FORM>(a, ck, far, head, c);
     const float x = a.PL[at];
     if (x < 0.0f) continue;
     l += x * __builtin_amdgcn_exp2f(a.PM[at] - mx);
@@ -562,37 +608,37 @@ __device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, in
   *den = __any(any) ? l : -1.0f;
 }
 
-// One query head's output from its sequence's chunks (two or more); all 256
+// One query head's output from its `count` parts (at least one); all 256
 // threads. The chunks' sums of the first round are on their way before the
 // joined reference is known.
-template <int DT, int D>
-__device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, int head, int tid) {
+template <int DT, int D, int FORM>
+__device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, const Far& far, int count, int head, int tid) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
   constexpr int AHEAD = 8;             // reads of a lane under way together
   __shared__ f32x4 part[256];
-  __shared__ float w_s[PG_WGS];        // the chunks' weights (chunk_len: a sequence has at most `target` chunks)
+  __shared__ float w_s[PG_WGS + (FORM & PG_PREFIX ? PG_WGS : 0)];  // the parts' weights (chunk_len: at most `target` of each kind)
   const int e = tid % (D / 4), r0 = tid / (D / 4);
   f32x4 x[AHEAD];
   auto load = [&](int c0) {  // past the last chunk: the last one's, not used
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const size_t at = (size_t)(ck.first + min(c0 + r0 + i * ROWS, ck.count - 1)) * a.nh + head;
+      const size_t at = part_row<FORM>(a, ck, far, head, min(c0 + r0 + i * ROWS, count - 1));
       x[i] = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
     }
   };
   load(0);
   float m, den;
-  join_sums(a, ck, head, tid & 63, &m, &den);
+  join_sums<FORM>(a, ck, far, count, head, tid & 63, &m, &den);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = tid; c < ck.count; c += 256)  // (a chunk without a key: weight times zeros)
-    w_s[c] = __builtin_amdgcn_exp2f(a.PM[(size_t)(ck.first + c) * a.nh + head] - m);
+  for (int c = tid; c < count; c += 256)  // (a chunk without a key: weight times zeros)
+    w_s[c] = __builtin_amdgcn_exp2f(a.PM[part_row<FORM>(a, ck, far, head, c)] - m);
   __syncthreads();
-  for (int c0 = 0; c0 < ck.count; c0 += ROWS * AHEAD) {
+  for (int c0 = 0; c0 < count; c0 += ROWS * AHEAD) {
     if (c0) load(c0);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int c = c0 + r0 + i * ROWS;
-      if (c < ck.count) {
+      if (c < count) {
         const float w = w_s[c];
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] += x[i][k] * w;
@@ -619,9 +665,12 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, in
 template <int DT, int D, int FORM>
 __device__ __forceinline__ void join_sequence(const AttnArgs& a, int b, int head, int tid) {
   const Chunk ck = sequence_chunks<FORM>(a, b, tid);
-  if (ck.count > 1)
-    join_head<DT, D>(a, ck, head, tid);
-  else if (ck.count == 0)  // no row, so no chunk. (In the first launch, stores that never ran took 10 % off its speed.)
+  Far far{0, 0, 1, 0};
+  if constexpr ((FORM & PG_PREFIX) != 0) far = far_of(a, b);
+  const int count = ck.count + far.count;
+  if (count > (FORM & PG_PREFIX ? 0 : 1))
+    join_head<DT, D, FORM>(a, ck, far, count, head, tid);
+  else if (count == 0)  // no row, so no chunk. (In the first launch, stores that never ran took 10 % off its speed.)
     for (int i = tid; i < D / 8; i += 256)
       reinterpret_cast<u32x4*>(a.Y + ((size_t)b * a.nh + head) * D)[i] = u32x4{0u, 0u, 0u, 0u};
 }
@@ -647,7 +696,9 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
   }
   const int h = blockIdx.x % a.c.nkv, group = a.nh / a.c.nkv;
   const Chunk ck = find_chunk<FORM>(a, blockIdx.x / a.c.nkv, tid);
-  if (ck.b < 0 || (ck.count == 1 && group <= PG_HEADS)) return;  // (finished by the first launch)
+  if (ck.b < 0 || (!(FORM & PG_PREFIX) && ck.count == 1 && group <= PG_HEADS)) return;  // (finished by the first launch)
+  Far far{0, 0, 1, 0};
+  if constexpr ((FORM & PG_PREFIX) != 0) far = far_of(a, ck.b);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   constexpr bool WINDOW = (FORM & PG_WINDOW) != 0;
   const Window win = window_of<FORM>(a, WINDOW ? a.c.rows(a.SLOT[ck.b]) : 0);
@@ -658,7 +709,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
     __syncthreads();
     for (int g = wave; g < gs; g += 4) {
       float m, den;
-      join_sums(a, ck, h * group + g0 + g, lane, &m, &den);
+      join_sums<FORM>(a, ck, far, ck.count + far.count, h * group + g0 + g, lane, &m, &den);
       if (lane == 0) m_s[g] = m, l_s[g] = den;
     }
     __syncthreads();
@@ -678,15 +729,16 @@ struct AttnPlan {
   int target, chunks, hgs;
   size_t parts, scores;  // floats
 };
-// rows: the most a sequence has (of the table's cap slots; fewer through a window).
-inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, long long rows, bool tracked, AttnPlan* p) {
+// rows: the most a sequence has (of the table's cap slots; fewer through a window); joined: there is
+// a second launch in any case.
+inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, long long rows, bool tracked, bool joined, AttnPlan* p) {
   const int group = nh / nkv;
   p->hgs = (group + PG_HEADS - 1) / PG_HEADS;
   const long long wide = (long long)nkv * p->hgs;
   p->target = (int)(wide < PG_WGS ? PG_WGS / wide : 1);
   p->parts = p->scores = 0;
   if ((long long)seqs * ((rows + PG_STEP - 1) / PG_STEP) > 0x3fffffff) return false;  // (more rows than any memory holds)
-  const bool one = rows <= PG_SHORT;
+  const bool one = rows <= PG_SHORT && !joined;
   if (one) p->target = 0;
   // a sequence adds at most one partly filled chunk to those the rows fill
   const long long most = (long long)seqs * ((rows + PG_STEP - 1) / PG_STEP);

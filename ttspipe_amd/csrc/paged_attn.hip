@@ -11,7 +11,7 @@ static int attention_kib(int seqs, int nh, int nkv, int head_dim, int cols, int 
   AttnPlan p;
   const long long cap = (long long)cols * page_size;
   if (seqs > 65535 || nh > 65535 || nkv > 4096 || head_dim > 128 || cap > TTSP_PAGED_MAX_SLOTS ||
-      !attn_plan(seqs, nh, nkv, head_dim, cap, window < 0 ? cap : window_rows(cap, window, sinks), tracked != 0, &p))
+      !attn_plan(seqs, nh, nkv, head_dim, cap, window < 0 ? cap : window_rows(cap, window, sinks), tracked != 0, false, &p))
     return -1;
   return (int)((p.parts + p.scores + 255) / 256);
 }
@@ -33,7 +33,8 @@ static int attention_launch(const ttsp_paged_cache* cache, const void* Q, long l
     a.window = window < cap ? window : cap;
     a.sinks = sinks < cap ? sinks : cap;
   }
-  if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, cap, FORM & PG_WINDOW ? window_rows(cap, a.window, a.sinks) : cap, tracked, &p))
+  if (!attn_plan(a.c.seqs, nh, a.c.nkv, hd, cap, FORM & PG_WINDOW ? window_rows(cap, a.window, a.sinks) : cap, tracked,
+                 false, &p))
     return (int)hipErrorInvalidValue;
   if (p.parts + p.scores && (!work || (uintptr_t)work % 16)) return (int)hipErrorInvalidValue;
   a.Q = (const uint16_t*)Q;

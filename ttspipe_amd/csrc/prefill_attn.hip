@@ -130,6 +130,7 @@ struct PrefillArgs {
   float scale2;  // scale * log2(e): scores in log2 units
   float* WO;     // SPLIT: unnormalised O [z][i][head][128], then m, l [z][i][head]
   const long long* POS;  // CAUSAL: the S query rows' positions (M unused)
+  int window, sinks;     // WINDOW: at least 1 and 0, at most L
 };
 
 // LDS of one staged key block: K rows, V rows, mask tile (bytes)
@@ -148,10 +149,13 @@ constexpr int PA_BLK = PA_KT + PA_VT + PA_MT;
 // (and the first key some row may not see) from its own 32 position loads.
 // The same keys are masked and the same blocks flagged whole as with the
 // causal mask's bytes, so the results are those bits.
+// WINDOW (CAUSAL): a row at position p does not see keys from `sinks` to
+// p - window. The blocks that no row of the workgroup sees are left out: block b
+// is the b-th of those that hold a sink or a key of some row's window.
 // GW: the query heads a workgroup takes, of the G that share a kv head
 // (G / GW workgroups a kv head and query block, each staging the kv head's
 // keys for its own heads).
-template <int DT, int G, int NS, bool SPLIT, bool CAUSAL = false, int GW = G>
+template <int DT, int G, int NS, bool SPLIT, bool CAUSAL = false, int GW = G, bool WINDOW = false>
 __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const PrefillArgs a) {
   static_assert(G % GW == 0, "a kv head's query heads split evenly over its workgroups");
   static_assert((NS & (NS - 1)) == 0, "the key splits merge in halving rounds");
@@ -179,6 +183,10 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   const int L = a.L;
   const int z = blockIdx.z;
   int kb0 = 0;  // first key of this workgroup's run (SPLIT: set after the mask scan)
+  // WINDOW: blocks of sinks, and the blocks left out behind them (keys)
+  const int sink_keys = WINDOW ? (a.sinks + PA_KB - 1) / PA_KB * PA_KB : 0;
+  int gap = 0;
+  auto key_at = [&](int j) { return WINDOW && j >= sink_keys ? j + gap : j; };
   const __amdgpu_buffer_rsrc_t kr = pa_rsrc(a.K + (size_t)kh * a.k_sh, (uint32_t)((L - 1) * a.k_ss + HD) * 2);
   const __amdgpu_buffer_rsrc_t vr = pa_rsrc(a.V + (size_t)kh * a.v_sh, (uint32_t)((L - 1) * a.v_ss + HD) * 2);
   // the mask buffer ends with the 16-byte piece holding the last row's byte
@@ -220,13 +228,13 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
 #pragma unroll
     for (int n = 0; n < KPT; ++n) {
       const int p = min(tid + n * NT, NKP - 1), blk = p / (PA_KB * (HD / 8)), q = p % (PA_KB * (HD / 8));
-      const int j = min(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8), L - 1), e = (q % (HD / 8)) * 8;
+      const int j = min(key_at(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8)), L - 1), e = (q % (HD / 8)) * 8;
       r.k[n] = pa_ld16(kr, (uint32_t)(j * a.k_ss + e) * 2);
     }
 #pragma unroll
     for (int n = 0; n < VPT; ++n) {
       const int p = min(tid + n * NT, NVP - 1), blk = p / (PA_KB * (HD / 8)), q = p % (PA_KB * (HD / 8));
-      const int j = min(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8), L - 1), e = (q % (HD / 8)) * 8;
+      const int j = min(key_at(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8)), L - 1), e = (q % (HD / 8)) * 8;
       r.v[n] = pa_ld16(vr, (uint32_t)(j * a.v_ss + e) * 2);
     }
     if constexpr (!CAUSAL) {
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       }
     }
   };
-  if constexpr (!SPLIT) {
+  if constexpr (!SPLIT && !WINDOW) {
     load(rs[0], 0);
     __builtin_amdgcn_sched_barrier(0);
     load(rs[1], 1);
@@ -282,8 +290,22 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   int hit = -1;
   // CAUSAL: the last key this lane's row sees (-1: none), and the lowest such
   // key over the workgroup's rows, below which every block is whole
-  const int klast = CAUSAL ? (int)min(pos_i, (long long)L - 1) : 0;
+  const int klast = CAUSAL ? (int)max(min(pos_i, (long long)L - 1), -1LL) : 0;
   int kwhole = 0;
+  // WINDOW: the first key of this lane's row's window, and the highest such key
+  // over the workgroup's rows, from which on no block is cut by one
+  const int klow = WINDOW ? (int)min(max(pos_i - a.window + 1, 0LL), (long long)L) : 0;
+  int low = 0;
+  if constexpr (WINDOW) {
+    int first = ql < nq ? klow : L;
+    low = ql < nq ? klow : 0;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      first = min(first, __shfl_xor(first, o, 64));
+      low = max(low, __shfl_xor(low, o, 64));
+    }
+    gap = max(first / PA_KB * PA_KB - sink_keys, 0);
+  }
   if constexpr (CAUSAL) {
     hit = klast;
     kwhole = ql < nq ? klast : L;
@@ -313,12 +335,14 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   }
   // this workgroup's key blocks: all blocks holding keys 0 .. last, or split
   // z's run of them
-  const int live = (last + PA_KB) / PA_KB;
+  const int live = max(last + PA_KB - gap, 0) / PA_KB;
   int nkb = live;
   if constexpr (SPLIT) {
     const int bps = (live + (int)gridDim.z - 1) / (int)gridDim.z;
     kb0 = z * bps * PA_KB;
     nkb = max(0, min(live, (z + 1) * bps) - z * bps);
+  }
+  if constexpr (SPLIT || WINDOW) {
     load(rs[0], 0);
     __builtin_amdgcn_sched_barrier(0);
     load(rs[1], 1);
@@ -352,7 +376,9 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       // (CAUSAL: the group's blocks whole when its last key is below every row's
       // last key, as the causal mask's tiles are then all set)
       const int gend = kb0 + (NS * t + NS) * PA_KB - 1;
-      const bool all = CAUSAL ? gend <= kwhole : __builtin_amdgcn_readfirstlane(full[t % 3]) != 0;
+      // (WINDOW: and none of them between the sinks and the last row's window)
+      const bool all = CAUSAL ? key_at(gend) <= kwhole && (!WINDOW || key_at(kb0 + NS * t * PA_KB) >= low || key_at(gend) < a.sinks)
+                              : __builtin_amdgcn_readfirstlane(full[t % 3]) != 0;
       // S^T = K Q^T for keys 32 b .. 32 b + 31
       pa_f32x16 s;
 #pragma unroll
@@ -383,12 +409,13 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       // lane and lane ^ 32, in log2 units
       if (!all) {
         if constexpr (CAUSAL) {
-          const int k0 = kb0 + b * PA_KB + 4 * h;  // key of s[0]
+          const int k0 = key_at(kb0 + b * PA_KB) + 4 * h;  // key of s[0]
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (k0 + 8 * g + c > klast) s[4 * g + c] = -__builtin_inff();
+              if (k0 + 8 * g + c > klast || (WINDOW && k0 + 8 * g + c >= a.sinks && k0 + 8 * g + c < klow))
+                s[4 * g + c] = -__builtin_inff();
         } else {
           const uint8_t* mrow = ms + ql * PA_MROW + 4 * h;
 #pragma unroll
@@ -605,22 +632,22 @@ extern "C" int ttsp_prefill_max_groups() { return PA_MAX_GROUPS; }
 // half the serial key steps, for twice the key staging (512 causal rows,
 // 32 / 8 heads: 14.5 against 15.9 us; with fewer rows, or with key splits,
 // the staging costs more than it saves).
-template <int DT, bool CAUSAL>
+template <int DT, bool CAUSAL, bool WINDOW = false>
 static int prefill_dispatch(int groups, dim3 grid, int splits, const PrefillArgs& a, hipStream_t stream) {
   if constexpr (CAUSAL) {
     if (groups == 4 && splits == 1 && (long long)grid.x * grid.y >= 128) {
       grid.x *= 2;
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, 4, 4, false, true, 2>), grid, dim3(64 * 2 * 4), 0, stream, a);
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, 4, 4, false, true, 2, WINDOW>), grid, dim3(64 * 2 * 4), 0, stream, a);
       return 0;
     }
   }
 #define TTSP_PA_G(G)                                                                                         \
   case G:                                                                                                    \
     if (splits > 1)                                                                                          \
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), true, CAUSAL>), grid,                     \
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), true, CAUSAL, G, WINDOW>), grid,                     \
                          dim3(64 * G * PA_SPLITS(G)), 0, stream, a);                                         \
     else                                                                                                     \
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), false, CAUSAL>), grid,                    \
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), false, CAUSAL, G, WINDOW>), grid,                    \
                          dim3(64 * G * PA_SPLITS(G)), 0, stream, a);                                         \
     return 0;
   switch (groups) {
@@ -639,12 +666,13 @@ static int prefill_dispatch(int groups, dim3 grid, int splits, const PrefillArgs
 }
 
 // mask: bool rows (mask_row_stride bytes apart), or null with pos, the S
-// rows' positions, for the causal mask at those positions
+// rows' positions, for the causal mask at those positions; window > 0: through a
+// window with sinks
 static int prefill_launch(const void* Q, long long q_seq_stride, long long q_head_stride, const void* K,
                           long long k_seq_stride, long long k_head_stride, const void* V, long long v_seq_stride,
                           long long v_head_stride, const void* mask, long long mask_row_stride, const long long* pos,
                           void* Y, int S, int nh, int nkv, int L, float scale, int dtype, float* work, int splits,
-                          hipStream_t stream) {
+                          hipStream_t stream, int window = 0, int sinks = 0) {
   const bool causal = pos != nullptr;
   if (causal) mask = nullptr, mask_row_stride = 0;
   if (!Q || !K || !V || (!causal && !mask) || !Y || S <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || L <= 0 ||
@@ -666,11 +694,15 @@ static int prefill_launch(const void* Q, long long q_seq_stride, long long q_hea
   PrefillArgs a{(const uint16_t*)Q, (const uint16_t*)K, (const uint16_t*)V, (const uint8_t*)mask, (uint16_t*)Y,
                 q_seq_stride, q_head_stride, (int)k_seq_stride, (int)k_head_stride, (int)v_seq_stride,
                 (int)v_head_stride, (int)mask_row_stride, S, nh, nkv, L, scale * PA_LOG2E,
-                splits > 1 ? work : nullptr, pos};
+                splits > 1 ? work : nullptr, pos, window < L ? window : L, sinks < L ? sinks : L};
   const int groups = nh / nkv;
   const dim3 grid(nkv, (S + PA_QB - 1) / PA_QB, splits);
   int rc;
-  if (dtype == DT_F16)
+  if (window > 0 && dtype == DT_F16)
+    rc = prefill_dispatch<DT_F16, true, true>(groups, grid, splits, a, stream);
+  else if (window > 0 && dtype == DT_BF16)
+    rc = prefill_dispatch<DT_BF16, true, true>(groups, grid, splits, a, stream);
+  else if (dtype == DT_F16)
     rc = causal ? prefill_dispatch<DT_F16, true>(groups, grid, splits, a, stream)
                 : prefill_dispatch<DT_F16, false>(groups, grid, splits, a, stream);
   else if (dtype == DT_BF16)
@@ -738,4 +770,27 @@ extern "C" int ttsp_prefill_attention_causal(const void* Q, long long q_seq_stri
   if (!pos) return (int)hipErrorInvalidValue;
   return prefill_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride,
                         v_head_stride, nullptr, 0, pos, Y, S, nh, nkv, L, scale, dtype, work, splits, stream);
+}
+
+// Keys the rows of a workgroup see at most.
+static int window_keys(int S, int L, int window, int sinks) {
+  const long long n = (long long)window + sinks + S;
+  return n < L ? (int)n : L;
+}
+
+extern "C" int ttsp_prefill_attention_window_splits(int S, int nkv, int L, int window, int sinks) {
+  if (S <= 0 || nkv <= 0 || L <= 0 || window <= 0 || sinks < 0) return 1;
+  return prefill_splits(S, nkv, window_keys(S, L, window, sinks));
+}
+
+extern "C" int ttsp_prefill_attention_window(const void* Q, long long q_seq_stride, long long q_head_stride,
+                                             const void* K, long long k_seq_stride, long long k_head_stride,
+                                             const void* V, long long v_seq_stride, long long v_head_stride,
+                                             const long long* pos, void* Y, int S, int nh, int nkv, int L, int window,
+                                             int sinks, float scale, int dtype, float* work, int splits,
+                                             hipStream_t stream) {
+  if (!pos || window < 1 || sinks < 0) return (int)hipErrorInvalidValue;
+  return prefill_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride,
+                        v_head_stride, nullptr, 0, pos, Y, S, nh, nkv, L, scale, dtype, work, splits, stream, window,
+                        sinks);
 }

@@ -60,7 +60,8 @@ def _prefill_eligible(q, k, v, mask, n_head, n_local_heads, head_dim, positions=
     return mask.stride(3) == 1 and mask.stride(2) % 16 == 0 and mask.stride(2) >= L and mask.data_ptr() % 16 == 0
 
 
-def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, work=None, positions=None):
+def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, work=None, positions=None, window=None,
+                      sinks=0):
     """`decode_attention` in one launch: q (1, n_head, S, 128), k/v (1,
     n_local_heads, L, 128) with the last dim contiguous (any seq/head strides
     that keep rows 16-byte aligned, e.g. the KV cache sliced to L), mask bool
@@ -78,11 +79,18 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     result is bit for bit the one `mask` = those causal rows gives, except
     where the kernel takes four in-workgroup key splits (4 query heads per kv
     head, no split over workgroups, at least 128 (kv head, 32-row block)
-    pairs), whose merge order rounds differently."""
+    pairs), whose merge order rounds differently.
+    `window` (with `positions`): row i sees keys j <= positions[i] with j < sinks
+    or j > positions[i] - window only, and key blocks that no row of a workgroup
+    sees are not read (their workspace: `prefill_splits(...)`)."""
     import torch
 
     from ttspipe_amd import _lib
 
+    if window is not None and positions is None:
+        raise ValueError("a window goes by the rows' positions")
+    if sinks < 0 or (window is None and sinks) or (window is not None and window < 1):
+        raise ValueError("a window has at least one key, and its sinks are not negative")
     if not _lib.gpu_present() or not _prefill_eligible(q, k, v, mask, n_head, n_local_heads, head_dim, positions):
         _stats["prefill_declined"] += 1
         return None
@@ -92,7 +100,9 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     elif out.shape != (1, seqlen, n_head * head_dim) or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous (1, S, n_head * head_dim) tensor of q's dtype")
     lib = _lib.lib()
-    splits = lib.ttsp_prefill_attention_splits(seqlen, n_local_heads, L)
+    if window is not None:
+        window, sinks = min(int(window), L), min(int(sinks), L)
+    splits = prefill_splits(seqlen, n_local_heads, L, window, sinks)
     need = prefill_work_floats(seqlen, n_head, splits)
     if splits > 1 and work is None:
         work = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -100,7 +110,12 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
                          or work.data_ptr() % 16):
         raise ValueError(f"work must be a contiguous 16-byte aligned fp32 tensor of at least {need} elements")
     wp = work.data_ptr() if splits > 1 else None
-    if positions is not None:
+    if window is not None:
+        _lib.launch("ttsp_prefill_attention_window", q.get_device(), q.data_ptr(), q.stride(2), q.stride(1), k.data_ptr(),
+                    k.stride(2), k.stride(1), v.data_ptr(), v.stride(2), v.stride(1), positions.data_ptr(), out.data_ptr(),
+                    seqlen, n_head, n_local_heads, L, window, sinks, float(head_dim**-0.5), _lib.dtype_code(q.dtype), wp,
+                    splits)
+    elif positions is not None:
         rc = lib.ttsp_prefill_attention_causal(
             q.data_ptr(), q.stride(2), q.stride(1), k.data_ptr(), k.stride(2), k.stride(1), v.data_ptr(),
             v.stride(2), v.stride(1), positions.data_ptr(), out.data_ptr(), seqlen, n_head, n_local_heads, L,
@@ -202,6 +217,16 @@ def causal_rows_attention_qkv(qkv, q_weight, k_weight, eps, freqs_cis, input_pos
     _lib.check(rc, "ttsp_attn_decode_qkv_rows")
     _stats["causal_rows"] += 1
     return y
+
+
+def prefill_splits(seqlen: int, n_local_heads: int, width: int, window: int | None = None, sinks: int = 0) -> int:
+    """Key splits of `prefill_attention` over `width` keys (its workspace: `prefill_work_floats`)."""
+    from ttspipe_amd import _lib
+
+    if window is None:
+        return _lib.lib().ttsp_prefill_attention_splits(seqlen, n_local_heads, width)
+    return _lib.lib().ttsp_prefill_attention_window_splits(seqlen, n_local_heads, width, min(window, width),
+                                                           min(sinks, width))
 
 
 def prefill_work_floats(seqlen: int, n_head: int, splits: int) -> int:

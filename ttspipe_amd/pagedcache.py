@@ -37,6 +37,7 @@ from __future__ import annotations
 
 import functools
 import struct
+from typing import NamedTuple
 
 import torch
 from torch import nn
@@ -60,6 +61,18 @@ def _declined():
 
 #: `ttsp_paged_cache`'s fields in order (`_lib.PagedCache` names them).
 _BLOCK = struct.Struct("@5P11q7i4x")
+#: `ttsp_paged_prefix`'s (`_lib.PagedPrefix`).
+_PREFIX = struct.Struct("@3Pq2i")
+
+
+class Prefix(NamedTuple):
+    """Prefixes that sequences share, in pages of the same pools: `table` int32
+    (prefixes, columns) and `slots` int64 (prefixes,) as a block table and its
+    newest slots; `of` int32 (sequences,) names each sequence's, -1 for none."""
+
+    table: torch.Tensor
+    slots: torch.Tensor
+    of: torch.Tensor
 
 
 def _strides_ok(s, nkv, pages, hd) -> bool:
@@ -239,10 +252,19 @@ def _window(window, sinks):
     return None if window is None else min(int(window), _lib.PAGED_MAX_SLOTS), min(int(sinks), _lib.PAGED_MAX_SLOTS)
 
 
+@functools.lru_cache(maxsize=256)
+def _prefix_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked, window, sinks, prefixes, wide) -> int:
+    return _lib.lib().ttsp_paged_attention_prefix_work_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size,
+                                                           prefixes, wide, window or 0, sinks, int(tracked))
+
+
 def attention_work(seqs: int, n_head: int, n_local_heads: int, head_dim: int, columns: int, page_size: int,
-                   tracked: bool = False, *, window: int | None = None, sinks: int = 0) -> int:
-    """fp32 elements of `attention`'s workspace; ValueError where `attention` declines sizes like these."""
-    kib = _attention_kib(seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked, *_window(window, sinks))
+                   tracked: bool = False, *, window: int | None = None, sinks: int = 0, prefixes: int = 0,
+                   prefix_columns: int = 0) -> int:
+    """fp32 elements of `attention`'s workspace (`prefixes` and `prefix_columns`: the
+    shape of `prefix.table`); ValueError where `attention` declines sizes like these."""
+    sizes = seqs, n_head, n_local_heads, head_dim, columns, page_size, tracked, *_window(window, sinks)
+    kib = _prefix_kib(*sizes, prefixes, prefix_columns) if prefixes else _attention_kib(*sizes)
     if kib < 0:
         raise ValueError("too many heads or slots for one call, or the workspace would take more than 2 TiB")
     return kib * 256
@@ -258,8 +280,21 @@ def _workspace(work, need, dtype, like):
     return work
 
 
+def _prefix_block(prefix, seqs, page, dev):
+    """The C-ABI's argument block of a `Prefix`, or None where the kernels do not take it."""
+    table, slots, of = prefix
+    if (table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != dev
+            or not _vector(slots, torch.int64, table.shape[0], dev) or not _vector(of, torch.int32, seqs, dev)):
+        return None
+    (count, cols), (t0, t1) = table.shape, table.stride()
+    if (not 1 <= count <= _lib.PAGED_MAX_PREFIXES or not 1 <= cols <= _lib.PAGED_MAX_SLOTS // page or (t1 != 1 and cols > 1)
+            or (count > 1 and t0 < cols)):
+        return None
+    return _PREFIX.pack(table.data_ptr(), slots.data_ptr(), of.data_ptr(), max(t0, cols), count, cols)
+
+
 def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = None, scores=None, out=None,
-              work=None, window: int | None = None, sinks: int = 0):
+              work=None, window: int | None = None, sinks: int = 0, prefix: Prefix | None = None):
     """One new token of each sequence over its cached rows: q (sequences, n_head,
     D), a sequence's heads contiguous, over slots 0 .. slots[b] (cut to the
     table's width), query head h with KV head h // (n_head / n_local_heads), the
@@ -274,6 +309,10 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     those rows and their pages' table entries are read, so the pages in between
     may have been given back (`PageTable.slide`). Slots have to be in the order of
     their positions: a cache that `evict` has moved rows in has no window.
+
+    With a `prefix`, sequence b also sees all rows of prefix `prefix.of[b]`, whose
+    pages are read once for all sequences that have it. The window and the scores
+    are those of its own rows.
 
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
@@ -295,7 +334,13 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
             or last != 1 or (nh > 1 and head_step != hd) or (seqs > 1 and (step < nh * hd or step % 8)) or qp % 16
             or not _vector(slots, torch.int64, seqs, dev)):
         return _declined()
-    kib = _attention_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks)
+    if prefix is None:
+        kib = _attention_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks)
+    else:
+        far = _prefix_block(prefix, seqs, page, dev)
+        if far is None:
+            return _declined()
+        kib = _prefix_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks, *prefix.table.shape)
     if kib < 0:
         return _declined()
     if out is None:
@@ -303,10 +348,12 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     elif not _out_ok(out, shape, dtype, dev):
         raise ValueError("out must be a contiguous, 16-byte aligned (sequences, n_head, head_dim) tensor of q's dtype")
     work = _workspace(work, kib * 256, torch.float32, q)
-    what, form = "ttsp_paged_attention", ()
-    if window is not None:
+    what, pools, form = "ttsp_paged_attention", (block,), ()
+    if prefix is not None:
+        what, pools, form = "ttsp_paged_attention_prefix", (block, far), (window or 0, sinks)
+    elif window is not None:
         what, form = "ttsp_paged_attention_window", (window, sinks)
-    _lib.launch(what, dev, block, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
+    _lib.launch(what, dev, *pools, qp, step if seqs > 1 else nh * hd, slots.data_ptr(), out.data_ptr(), nh,
                 hd**-0.5 if scale is None else scale, *form, 0 if work is None else work.data_ptr())
     _stats["attention"] += 1
     return out
