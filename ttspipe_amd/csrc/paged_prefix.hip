@@ -4,19 +4,34 @@
 // rows are read here once for all the sequences that share them, and a last launch
 // joins both.
 //
-// A workgroup takes a chunk of a prefix's rows, one kv head, and 16 T query rows:
-// the query heads of the kv head of T 16 / group sequences that have the prefix.
-// The same rows for every column of the matrix cores' tiles: that is a matrix
-// product with 16 T columns where a sequence by itself has group of them. Four waves
-// each take every fourth run of 32 rows as in paged_attn.h, each with all the
-// workgroup's query rows, so every row of K and V goes from memory into one wave's
-// registers, and once through its LDS to be transposed, for 16 T query rows.
-#include "paged_attn.h"
+// A workgroup takes a chunk of a prefix's rows, one kv head, and up to 32 RG query
+// rows: that kv head's query heads of some of the sequences that have the prefix, one
+// sequence's after the other's (tile_attn.h: the same keys for all of them, where a
+// sequence by itself has group rows for a key). The chunks are cut on the device from
+// the prefixes' lengths and the number of sequences that have each.
+#include "tile_attn.h"
 
 namespace ttsp {
 
 constexpr int PF_MAX = 256;   // prefixes of a call (one a thread)
-constexpr int PF_WGS = 512;   // workgroups the chunks are meant to make
+constexpr int PF_WGS = 256;   // workgroups the chunks are meant to make, one a CU
+constexpr int PF_PARTS = 2;
+
+// The sum of v over the workgroup's threads, and over those before this one.
+__device__ __forceinline__ uint32_t pf_prefix(uint32_t v, uint32_t* sums, int tid, uint32_t* total) {
+  const uint32_t upto = lane_prefix(v);
+  __syncthreads();
+  if ((tid & 63) == 63) sums[tid >> 6] = upto;
+  __syncthreads();
+  uint32_t before = upto - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < TA_WAVES; ++w) {
+    if (w < (tid >> 6)) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before;
+}
 
 // Item gx of the call: a chunk of a prefix and a tile of its query rows.
 struct Item {
@@ -27,15 +42,16 @@ struct Item {
   int members;       // sequences that have it
 };
 
-// All 256 threads; the result is uniform.
+// All threads; the result is uniform.
 __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
-  __shared__ int cnt[PF_MAX];
-  __shared__ uint32_t sums[PG_T / 64];
-  __shared__ int found[8];
+  __shared__ int cnt[TA_T];
+  __shared__ uint32_t sums[TA_WAVES];
+  __shared__ int found[6];
+  static_assert(PF_MAX <= TA_T, "a thread a prefix");
   const int group = a.nh / a.c.nkv;
   cnt[tid] = 0;
   __syncthreads();
-  for (int b = tid; b < a.seqs; b += PG_T) {
+  for (int b = tid; b < a.seqs; b += TA_T) {
     const int p = a.OF[b];
     if ((unsigned)p < (unsigned)a.prefixes) atomicAdd(&cnt[p], 1);
   }
@@ -43,10 +59,10 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
   const int m = cnt[tid], n = m ? a.far_rows(tid) : 0;
   const uint32_t tiles = n ? (uint32_t)((m * group + a.far_tile - 1) / a.far_tile) : 0;
   uint32_t total;
-  block_prefix(tiles * units(n), sums, tid, &total);
+  pf_prefix(tiles * units(n), sums, tid, &total);
   const uint32_t len = max((total + a.far_target - 1) / (uint32_t)a.far_target, 1u);
   const int count = n ? chunk_count(n, len) : 0;
-  const int first = (int)block_prefix(tiles * count, sums, tid, &total);
+  const int first = (int)pf_prefix(tiles * count, sums, tid, &total);
   Item it{-1, 0, 0, 0, 0, 1, 0, 0};
   if ((uint32_t)gx >= total) return it;
   if (gx >= first && gx < first + (int)tiles * count) {  // one thread
@@ -64,19 +80,17 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
   return it;
 }
 
-template <int DT, int D, int T>
-__global__ __launch_bounds__(64 * PG_WAVES, 2) void paged_prefix_kernel(const AttnArgs a) {
-  constexpr int QT = 16 * T;                    // query rows of the workgroup
-  constexpr int QROW = D + 8;                   // their stride in LDS (elements)
-  constexpr int KC = D / 32, DC = D / 16, VPL = PG_KEYS * D * 2 / 1024, VR = 1024 / (D * 2);
-  constexpr int REGION = PG_KEYS * D * 2;       // a wave's LDS: V rows, at the end 16 fp32 rows of O
-  __shared__ __align__(16) uint8_t lds[PG_WAVES * REGION];
-  __shared__ __align__(16) uint16_t qs[QT * QROW];
-  __shared__ float m_s[PG_WAVES][16], l_s[PG_WAVES][16];
-  __shared__ int seq_s[QT + 2], wcnt[PG_WAVES];
+template <int DT, int D, int RG>
+__global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef Tile<D, RG> C;
+  constexpr int QT = 32 * RG;
+  __shared__ __align__(256) uint8_t ring0[C::STAGE];
+  __shared__ __align__(256) uint8_t ring1[C::STAGE];
+  __shared__ __align__(256) uint8_t ring2[C::ST > 2 ? C::STAGE : 16];
+  __shared__ int seq_s[QT + 2], wcnt[TA_WAVES];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 15, lg = lane >> 4;
   const int group = a.nh / a.c.nkv, h = blockIdx.x % a.c.nkv, gx = blockIdx.x / a.c.nkv;
   const Item it = find_item(a, gx, tid);
   if (it.p < 0) return;
@@ -84,7 +98,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, 2) void paged_prefix_kernel(const At
 
   // the tile's sequences: the o0-th of the prefix's to the one before the o1-th
   const int o0 = row0 / group, o1 = (row0 + rows - 1) / group + 1;
-  for (int b0 = 0, before = 0; b0 < a.seqs && before < o1; b0 += PG_T) {
+  for (int b0 = 0, before = 0; b0 < a.seqs && before < o1; b0 += TA_T) {
     const int b = b0 + tid;
     const bool has = b < a.seqs && a.OF[b] == it.p;
     const unsigned long long bits = __ballot(has);
@@ -92,7 +106,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, 2) void paged_prefix_kernel(const At
     __syncthreads();
     int at = before + __popcll(bits & ((1ull << lane) - 1));
 #pragma unroll
-    for (int w = 0; w < PG_WAVES; ++w) {
+    for (int w = 0; w < TA_WAVES; ++w) {
       at += w < wave ? wcnt[w] : 0;
       before += wcnt[w];
     }
@@ -100,198 +114,109 @@ __global__ __launch_bounds__(64 * PG_WAVES, 2) void paged_prefix_kernel(const At
     __syncthreads();
   }
   if (it.c == 0 && h == 0)  // for the joining launch: where a sequence's parts are
-    for (int i = tid; i < o1 - o0; i += PG_T)
+    for (int i = tid; i < o1 - o0; i += TA_T)
       if ((o0 + i) * group >= row0)
         a.DESC[seq_s[i]] = make_int4(it.first, it.count, it.tiles, (o0 + i) * group);
-  for (int i = tid; i < QT * (D / 8); i += PG_T) {
-    const int r = i / (D / 8), e = (i % (D / 8)) * 8;
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (r < rows)
-      v = *reinterpret_cast<const u32x4*>(a.Q + seq_s[(row0 + r) / group - o0] * a.q_seq +
-                                          (size_t)(h * group + (row0 + r) % group) * D + e);
-    *reinterpret_cast<u32x4*>(qs + r * QROW + e) = v;
+
+  const int rg = wave % RG, kg = wave / RG;
+  const int myrow = 32 * rg + (lane & 31);  // this lane's query row of the tile
+  TaWave<DT, D, PF_PARTS> w;
+  w.init(lane);
+  {
+    const int r = row0 + min(myrow, rows - 1);  // (rows past the tile's: its last one's, not written)
+    const uint16_t* const q = a.Q + seq_s[r / group - o0] * a.q_seq + (size_t)(h * group + r % group) * D + 8 * (lane >> 5);
+    const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and its absolute value)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) w.q[i] = *reinterpret_cast<const u32x4*>(q + 16 * i) ^ flip;
   }
-  __syncthreads();
+  const float scale2 = a.scale2 == 0.0f ? 1e-30f : fabsf(a.scale2);  // (0: -inf times it is to stay so)
 
   const int size = chunk_size(it.n, it.count), k0 = it.c * size, k1 = min(k0 + size, it.n);
   const int mask = (1 << a.c.shift) - 1;
-  const int* const trow = a.far_table + it.p * a.far_stride;
+  // (constant memory while the kernel runs: scalar loads, which the ring's waits do not count)
+  typedef const __attribute__((address_space(4))) int* table_ptr;
+  const table_ptr trow = (table_ptr)(a.far_table + it.p * a.far_stride);
   auto page_at = [&](int j) {
     const int p = j < k1 ? trow[j >> a.c.shift] : -1;
     return (unsigned)p < (unsigned)a.c.pages ? p : -1;
   };
-  uint8_t* const vs = lds + wave * REGION;
-  const uint32_t ko = (uint32_t)(lr * (int)a.c.k_row + 8 * lg) * 2;
-  const uint32_t vo = (uint32_t)((lane / (64 / VR)) * (int)a.c.v_row + (lane % (64 / VR)) * 8) * 2;
-  u32x4 kf[2][KC], vf[VPL];
-  auto load = [&](int j, int p0, int p1) {
+  // Pages asked for a tile ahead of their use: of this wave's loads, of what has
+  // landed, and of the runs it computes.
+  int pn[C::PER], pl[C::PER], pc[C::SB][2];
+  // this wave's loads of a tile: PER runs of RPI rows from row PER RPI wave on; a hole reads page 0
+  uint32_t ko[C::PER], vo[C::PER];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int p = max(s ? p1 : p0, 0), row = (j + 16 * s) & mask;
-      const uint8_t* kb = (const uint8_t*)(a.c.K + p * a.c.k_page + h * a.c.k_head + row * a.c.k_row);
-#pragma unroll
-      for (int i = 0; i < KC; ++i) kf[s][i] = *reinterpret_cast<const u32x4*>(kb + 64 * i + ko);
-      const uint8_t* vb = (const uint8_t*)(a.c.V + p * a.c.v_page + h * a.c.v_head + row * a.c.v_row);
-#pragma unroll
-      for (int i = 0; i < VPL / 2; ++i)
-        vf[s * (VPL / 2) + i] = *reinterpret_cast<const u32x4*>(vb + (size_t)i * VR * a.c.v_row * 2 + vo);
-    }
-  };
-  auto vaddr = [&](int row, int blk) {
-    const int sw = D == 128 ? row & 7 : (row >> 1) & 3;
-    return row * (D * 2) + ((blk ^ sw) << 5);
-  };
-
-  f32x4 o[T][DC];
-  float mref[T], lsum[T];
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    mref[t] = PG_NONE, lsum[t] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DC; ++d) o[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < C::PER; ++i) {
+    const int lrow = lane / C::PPR, piece = (lane % C::PPR) ^ ta_swz<D>((wave * C::PER + i) * C::RPI + lrow);
+    ko[i] = (uint32_t)(lrow * (int)a.c.k_row) * 2 + piece * 16;
+    vo[i] = (uint32_t)(lrow * (int)a.c.v_row) * 2 + piece * 16;
   }
+  const int lr0 = k0 + wave * C::PER * C::RPI, cr0 = k0 + 32 * C::SB * kg;
+  auto pages_loaded = [&](int t, int (&p)[C::PER]) {
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) p[i] = page_at(lr0 + t * C::KEYS + i * C::RPI);
+  };
+  auto pages_run = [&](int t) {
+#pragma unroll
+    for (int b = 0; b < C::SB; ++b)
+      pc[b][0] = page_at(cr0 + t * C::KEYS + 32 * b), pc[b][1] = page_at(cr0 + t * C::KEYS + 32 * b + 16);
+  };
+  pages_loaded(0, pn);
+  pages_loaded(0, pl);
+  pages_run(0);
+  auto load = [&](int t, uint8_t* ring) {
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+      const int row = (wave * C::PER + i) * C::RPI, p = max(pn[i], 0);
+      const long long r = (lr0 + t * C::KEYS + i * C::RPI) & mask;
+      ta_load(a.c.K + p * a.c.k_page + h * a.c.k_head + r * a.c.k_row, ko[i], ring + row * C::ROWB);
+      ta_load(a.c.V + p * a.c.v_page + h * a.c.v_head + r * a.c.v_row, vo[i], ring + C::HALF + row * C::ROWB);
+    }
+    pages_loaded(t + 1, pn);
+  };
+  // V rows that are no keys are zeros (what they hold may be NaN)
+  auto landed = [&](int t, uint8_t* ring) {
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+      const int j = lr0 + t * C::KEYS + i * C::RPI;
+      if (pl[i] < 0 || j + C::RPI > k1)
+        if (pl[i] < 0 || j + lane / C::PPR >= k1)
+          *reinterpret_cast<u32x4*>(ring + C::HALF + (wave * C::PER + i) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+    pages_loaded(t + 1, pl);
+  };
   bool seen = false;
+  auto compute = [&](int t, uint8_t* ring) {
+#pragma unroll
+    for (int b = 0; b < C::SB; ++b) {
+      const int row = 32 * (C::SB * kg + b), j = k0 + t * C::KEYS + row, p0 = pc[b][0], p1 = pc[b][1];
+      if (j >= k1) continue;
+      seen = seen || p0 >= 0 || p1 >= 0;
+      w.run(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, j + 32 > k1 || p0 < 0 || p1 < 0,
+            [&](int i) { return j + i >= k1 || (i < 16 ? p0 : p1) < 0; });
+    }
+    pages_run(t + 1);
+  };
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(w.q[i]));  // (waited for here, not among the loop's loads)
+  ta_tiles<C>((k1 - k0 + C::KEYS - 1) / C::KEYS, ring0, ring1, ring2, load, landed, compute);
+  ta_join<C>(w, seen, ring0, ring1, ring2, rg, kg, lane);
 
-  int j = k0 + PG_KEYS * wave;
-  int p0 = page_at(j), p1 = page_at(j + 16);
-  if (j < k1) load(j, p0, p1);
-  int n0 = page_at(j + PG_STEP), n1 = page_at(j + PG_STEP + 16);
-  for (; j < k1; j += PG_STEP) {
-    const bool whole = j + PG_KEYS <= k1 && p0 >= 0 && p1 >= 0;
-    seen = seen || p0 >= 0 || p1 >= 0;
-    f32x4 s[T][2];
+  if (kg == 0 && myrow < rows) {
+    const size_t at = a.far_base + ((size_t)gx * a.c.nkv + h) * QT + myrow;
+    const int h4 = 4 * (lane >> 5);
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const u32x4 qf = *reinterpret_cast<const u32x4*>(qs + (16 * t + lr) * QROW + 32 * i + 8 * lg);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s[t][u] = pg_mfma<DT>(kf[u][i], qf, s[t][u]);
-      }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(a.PACC + at * D + 32 * d + 8 * g + h4) =
+            f32x4{w.o[d][4 * g], w.o[d][4 * g + 1], w.o[d][4 * g + 2], w.o[d][4 * g + 3]};
+    if (lane < 32) {
+      a.PM[at] = w.m;
+      a.PL[at] = seen ? w.l : -1.0f;
     }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int row = i * VR + lane / (64 / VR), c16 = lane % (64 / VR);
-      *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = vf[i];
-    }
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int row = i * VR + lane / (64 / VR), c16 = lane % (64 / VR);
-        if (j + row >= k1 || (row < 16 ? p0 : p1) < 0)
-          *reinterpret_cast<u32x4*>(vs + vaddr(row, c16 >> 1) + (c16 & 1) * 16) = u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-    const int c0 = p0, c1 = p1;
-    p0 = n0, p1 = n1;
-    if (j + PG_STEP < k1) load(j + PG_STEP, p0, p1);
-    n0 = page_at(j + 2 * PG_STEP), n1 = page_at(j + 2 * PG_STEP + 16);
-
-    u32x4 pf[T][pg_parts<DT>];
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      bool over = false;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = s[t][u][r] * a.scale2;
-          if (!whole && (j + 16 * u + 4 * lg + r >= k1 || (u ? c1 : c0) < 0)) x = -__builtin_inff();
-          s[t][u][r] = x;
-          over = over || x > mref[t] + pg_above<DT>;
-        }
-      if (__any(over)) {
-        float bm = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                         fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-        bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-        bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-        const float mnew = bm > mref[t] + pg_above<DT> ? bm - pg_below<DT> : mref[t];
-        const float alpha = __builtin_amdgcn_exp2f(mref[t] - mnew);
-        mref[t] = mnew;
-        lsum[t] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DC; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[t][d][r] *= alpha;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(s[t][u][r] - mref[t]);
-          lsum[t] += p[r];
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t parts[pg_parts<DT>];
-          pg_split<DT>(p[2 * r], p[2 * r + 1], parts);
-#pragma unroll
-          for (int i = 0; i < pg_parts<DT>; ++i) pf[t][i][2 * u + r] = parts[i];
-        }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int d = 0; d < DC; ++d) {
-      const int row = 4 * lg + (lr >> 2);
-      const uint2 lo = pg_ld_tr(vs + vaddr(row, d) + 8 * (lr & 3));
-      const uint2 hi = pg_ld_tr(vs + vaddr(row + 16, d) + 8 * (lr & 3));
-      const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int i = 0; i < pg_parts<DT>; ++i) o[t][d] = pg_mfma<DT>(vt, pf[t][i], o[t][d]);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
-
-  // the waves' parts, 16 query rows at a time
-  float* const os = reinterpret_cast<float*>(vs);
-  const float* const all = reinterpret_cast<const float*>(lds);
-  const size_t out0 = a.far_base + ((size_t)gx * a.c.nkv + h) * QT;
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    float l = lsum[t];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (lane < 16) {
-      m_s[wave][lane] = mref[t];
-      l_s[wave][lane] = seen ? l : -1.0f;
-    }
-#pragma unroll
-    for (int d = 0; d < DC; ++d) *reinterpret_cast<f32x4*>(os + lr * D + 16 * d + 4 * lg) = o[t][d];
-    __syncthreads();
-    for (int i = tid; i < min(16, rows - 16 * t) * D; i += PG_T) {
-      const int g = i / D, d = i % D;
-      float m = PG_NONE;
-#pragma unroll
-      for (int w = 0; w < PG_WAVES; ++w) m = fmaxf(m, m_s[w][g]);
-      float num = 0.0f, den = 0.0f;
-      bool any = false;
-#pragma unroll
-      for (int w = 0; w < PG_WAVES; ++w) {
-        const float lw = l_s[w][g], e = __builtin_amdgcn_exp2f(m_s[w][g] - m);
-        const bool none = lw < 0.0f;
-        den += (none ? 0.0f : lw) * e;
-        num += all[(size_t)w * (REGION / 4) + g * D + d] * e;
-        any = any || !none;
-      }
-      const size_t at = out0 + 16 * t + g;
-      a.PACC[at * D + d] = num;
-      if (d == 0) {
-        a.PM[at] = m;
-        a.PL[at] = any ? den : -1.0f;
-      }
-    }
-    __syncthreads();
-  }
+#endif
 }
 
 // How the prefixes' part of a call is cut up; false where it is more than is counted.
@@ -301,7 +226,7 @@ struct PrefixPlan {
 };
 inline bool prefix_plan(int seqs, int nh, int nkv, int prefixes, long long far_cap, PrefixPlan* p) {
   const long long group = nh / nkv, rows = seqs * group;
-  p->tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p->tile = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
   p->target = nkv < PF_WGS ? PF_WGS / nkv : 1;
   // each prefix that a sequence has may end with a tile that is not full
   const long long tiles = rows / p->tile + (prefixes < seqs ? prefixes : seqs);
@@ -358,9 +283,9 @@ static int prefix_launch(const AttnArgs& a, const PrefixWork& w, int hd, int dty
   const int gathers = w.own.chunks * a.c.nkv;
 #define TTSP_PFX(DTV, DV)                                                                                              \
   do {                                                                                                                 \
-    if (w.far.tile == 16) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 1>), far, dim3(PG_T), 0, stream, a);         \
-    else if (w.far.tile == 32) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 2>), far, dim3(PG_T), 0, stream, a);    \
-    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4>), far, dim3(PG_T), 0, stream, a);                          \
+    if (w.far.tile == 64) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 2>), far, dim3(TA_T), 0, stream, a);         \
+    else if (w.far.tile == 128) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4>), far, dim3(TA_T), 0, stream, a);   \
+    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 8>), far, dim3(TA_T), 0, stream, a);                          \
     hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, FORM>), own, dim3(64 * PG_WAVES), 0, stream, a);                     \
     if (FORM & PG_TRACK)                                                                                               \
       hipLaunchKernelGGL((paged_gather_kernel<DTV, DV, FORM>), dim3(gathers + a.seqs * a.nh), dim3(256), 0, stream, a,  \

@@ -1,0 +1,234 @@
+// Attention of many query rows over the same keys, the core of the kernels that have
+// such rows: sequences that share a prefix (paged_prefix.hip) and a prompt's rows
+// through a window (prefill_window.hip).
+//
+// A workgroup of eight waves takes 32 RG query rows of one kv head. Its keys come in
+// tiles through a ring in LDS, straight from memory (buffer loads to LDS, so that no
+// register holds what is on its way): RG waves take 32 rows each of the same 32 keys,
+// and 8 / RG such groups of waves every (8 / RG)-th run of 32 keys; the groups' sums
+// join in LDS at the end. The fewer the rows, the more keys are under way.
+//
+// A wave's 32 keys: S^T = K Q^T on the matrix cores (Q stays in registers), so that a
+// lane holds 16 keys of one query row; the exponentials subtract a reference that
+// moves only when a score outgrows it (pg_above), so the running maximum needs no
+// exchange between lanes but a vote; P^T goes back to the matrix cores from the
+// registers it is in, in PARTS of the cache's type: O^T += V^T P^T, V^T through the
+// transposing LDS read. Two waves a SIMD: one's exponentials run beside the other's
+// products.
+//
+// K and V rows lie in LDS as in memory, their 16-byte pieces swizzled by row (ta_swz):
+// sixteen rows' same piece lies in sixteen different bank groups (K's reads), and the
+// same 64 bytes of four neighbouring rows in four (V's transposing reads).
+//
+// MFMA 32x32x16: lane l supplies row (l % 32) of A and column (l % 32) of B at
+// k = 8 (l / 32) .. + 7; accumulator r of lane l is D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32].
+#pragma once
+
+#include "nf4_mfma.h"
+#include "paged_attn.h"
+
+namespace ttsp {
+
+typedef __attribute__((address_space(3))) void* ta_lds_ptr;
+
+constexpr int TA_WAVES = 8, TA_T = 64 * TA_WAVES;
+
+template <int D, int RG>
+struct Tile {
+  static constexpr int KG = TA_WAVES / RG, SB = RG == 8 ? 2 : 1;  // key groups; runs of 32 keys a wave takes of a tile
+  static constexpr int KEYS = 32 * KG * SB, ROWB = D * 2, PPR = ROWB / 16;
+  static constexpr int HALF = KEYS * ROWB, STAGE = 2 * HALF, ST = RG == 2 ? 2 : 3;  // K, then V; stages of the ring
+  static constexpr int RPI = 1024 / ROWB, PER = KEYS / RPI / TA_WAVES;  // rows a load covers, loads of K (and of V) a wave
+};
+
+// The swizzle of row r: its 16-byte piece p lies at piece p ^ ta_swz(r).
+template <int D>
+__device__ __forceinline__ int ta_swz(int r) {
+  return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+// Two weights (not negative) in PARTS of DT as packed pairs. One part: rounded to
+// nearest. Two: fp16 as pg_split, within 2^-22; bf16 the upper eight bits and the rest
+// rounded to eight, within 2^-16 (the lower part is kept above 0, as in pg_split).
+template <int DT, int PARTS>
+__device__ __forceinline__ void ta_split(float p, float q, uint32_t* parts) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (PARTS == 1) {
+    if constexpr (DT == DT_BF16) parts[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p, q}, b16x2));
+    else parts[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p, q}, h16x2));
+  } else if constexpr (DT == DT_F16) {
+    pg_split<DT>(p, q, parts);
+  } else {
+    constexpr float least = 1.17549435e-38f;
+    const uint32_t up = __float_as_uint(p), uq = __float_as_uint(q);
+    parts[0] = __builtin_amdgcn_perm(uq, up, 0x07060302u);
+    const f32x2 rest = {fmaxf(p - __uint_as_float(up & 0xffff0000u), least), fmaxf(q - __uint_as_float(uq & 0xffff0000u), least)};
+    parts[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, b16x2));
+  }
+}
+
+// A wave's 32 query rows.
+template <int DT, int D, int PARTS>
+struct TaWave {
+  u32x4 q[D / 16];      // Q^T: column = query row lane % 32, dims 16 i + 8 (lane / 32) .. + 7
+  f32x16_v o[D / 32];   // O^T
+  float m, l;           // reference (log2 units) and this lane's keys' sum of exp2(s - m)
+  uint32_t kb, vb;      // this lane's first bytes of K and of V in a run of 32 keys
+
+  __device__ __forceinline__ void init(int lane) {
+    const int h = lane >> 5, ql = lane & 31, g = lane >> 4, li = lane & 15;
+    m = PG_NONE, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    kb = ql * (D * 2) + ((h ^ ta_swz<D>(ql)) << 4);
+    const int row = 4 * (g >> 1) + (li >> 2), piece = 2 * (g & 1) + ((li & 3) >> 1);
+    vb = row * (D * 2) + ((piece ^ ta_swz<D>(row)) << 4) + (li & 1) * 8;
+  }
+
+  // 32 keys: K and V rows at k and v. masked (uniform): key j of the run is none where gone(j).
+  template <typename F>
+  __device__ __forceinline__ void run(const uint8_t* k, const uint8_t* v, float scale2, bool masked, F gone) {
+    f32x16_v s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma32<DT>(*reinterpret_cast<const u32x4*>(k + (kb ^ (i << 5))), q[i], s);
+    if (masked) {
+      const int h4 = (threadIdx.x & 63) >> 5 << 2;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (gone(8 * (r / 4) + h4 + r % 4)) s[r] = -__builtin_inff();
+    }
+    float bm = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+    bm *= scale2;
+    if (__any(bm > m + pg_above<DT>)) {
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+      const float mnew = bm > m + pg_above<DT> ? bm - pg_below<DT> : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+      m = mnew;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    u32x4 pf[2][PARTS];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + 2 * u], scale2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + 2 * u + 1], scale2, -m));
+        l += p0;
+        l += p1;
+        uint32_t parts[PARTS];
+        ta_split<DT, PARTS>(p0, p1, parts);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) pf[c][i][u] = parts[i];
+      }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint8_t* const p = v + 16 * c * (D * 2) + (vb ^ (d << 6));
+        const uint8_t* const p8 = v + (16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32);
+        const uint2 lo = pg_ld_tr(p), hi = pg_ld_tr(p8);
+        const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) o[d] = mfma32<DT>(vt, pf[c][i], o[d]);
+      }
+  }
+};
+
+// n tiles through the ring: load(t, ring) issues this wave's 2 PER loads of tile t (any
+// t: past the last it may load what it likes), landed(t, ring) may touch up the rows
+// that this wave loaded, compute(t, ring) reads tile t.
+template <typename C, typename F, typename G, typename H>
+__device__ __forceinline__ void ta_tiles(int n, uint8_t* ring0, uint8_t* ring1, uint8_t* ring2, F load, G landed, H compute) {
+  constexpr int L = 2 * C::PER;
+  if (n <= 0) return;
+  load(0, ring0);
+  if constexpr (C::ST > 2) load(1, ring1);
+  // step t: tile t has landed and every wave is past tile t - 1, whose place tile t + ST - 1 takes
+  auto one = [&](int t, uint8_t* rd, uint8_t* dst) {
+    TTSP_WAIT_VM_LGKM0((C::ST - 2) * L);
+    landed(t, rd);
+    TTSP_WAIT_LGKM0();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load(t + C::ST - 1, dst);
+    compute(t, rd);
+  };
+  int t = 0;
+  if constexpr (C::ST == 2) {
+    for (; t + 2 <= n; t += 2) {
+      one(t, ring0, ring1);
+      one(t + 1, ring1, ring0);
+    }
+    if (t < n) one(t, ring0, ring1);
+  } else {
+    for (; t + 3 <= n; t += 3) {
+      one(t, ring0, ring2);
+      one(t + 1, ring1, ring0);
+      one(t + 2, ring2, ring1);
+    }
+    if (t < n) one(t, ring0, ring2);
+    if (t + 1 < n) one(t + 1, ring1, ring0);
+  }
+  TTSP_WAIT_VM_LGKM0(0);
+  __syncthreads();
+}
+
+// The key groups' sums joined into the first group's waves (the ring is free). seen:
+// whether the wave has had a key; the first group's get the groups'.
+template <typename C, int DT, int D, int PARTS>
+__device__ __forceinline__ void ta_join(TaWave<DT, D, PARTS>& w, bool& seen, uint8_t* ring0, uint8_t* ring1, uint8_t* ring2, int rg,
+                                        int kg, int lane) {
+  constexpr int RG = TA_WAVES / C::KG;
+  w.l += __shfl_xor(w.l, 32, 64);
+#pragma unroll
+  for (int st = C::KG / 2; st >= 1; st /= 2) {
+    const bool give = kg >= st && kg < 2 * st, take = kg < st;
+    const int slot = (give ? kg - st : kg) * RG + rg;
+    auto part = [&](int d) {  // 4 KB of the slot's O
+      const int at = (slot * (D / 32) + d) * 4096;
+      return reinterpret_cast<float*>(at < C::STAGE ? ring0 + at : ring1 + (at - C::STAGE)) + lane;
+    };
+    float* const ml = reinterpret_cast<float*>(C::ST > 2 ? ring2 : ring1) + slot * 192 + lane;
+    if (give) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part(d)[64 * r] = w.o[d][r];
+      ml[0] = w.m, ml[64] = w.l, ml[128] = seen ? 1.0f : 0.0f;
+    }
+    __syncthreads();
+    if (take) {
+      const float m2 = ml[0], mm = fmaxf(w.m, m2);
+      const float f1 = __builtin_amdgcn_exp2f(w.m - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
+      w.l = w.l * f1 + ml[64] * f2;
+      w.m = mm;
+      seen = seen || ml[128] != 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.o[d][r] = w.o[d][r] * f1 + part(d)[64 * r] * f2;
+    }
+    __syncthreads();
+  }
+}
+
+// One load of 1024 bytes of rows from base into LDS at dst, lane l's 16 bytes from byte voff.
+__device__ __forceinline__ void ta_load(const void* base, uint32_t voff, uint8_t* dst) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, -1, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ta_lds_ptr)dst, 16, voff, 0, 0, 0);
+}
+
+}  // namespace ttsp
