@@ -73,6 +73,8 @@ constexpr int PG_WGS = 1024;
 // joining launch (300 rows, alone: 8.3 us; in three chunks and joined: 10.2).
 constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
+// Rows a prefix's chunk has at most (their runs' places are held in LDS), and so its most chunks.
+constexpr int PF_CHUNK = 8192, PF_CHUNKS = TTSP_PAGED_MAX_SLOTS / PF_CHUNK;
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 // A moved reference lies `pg_below` under the largest score and moves again when a
 // score is `pg_above` over it. bf16 weights have room on both sides. fp16 ones end
@@ -101,7 +103,9 @@ struct AttnArgs {
   const int* OF;              // [seqs]: the sequence's prefix, outside 0 .. prefixes - 1: none
   int prefixes, far_cols, far_target, far_tile;  // far_tile: query rows of a kv head a prefix workgroup takes
   size_t far_base;  // rows of PM, PL, PACC before the prefixes'
-  int4* DESC;       // [seqs]: where its prefix's sums are (Far), where it has one that holds a row
+  // [2 seqs], written by the first launch for the last: a sequence's own chunks (first, count, whether
+  // it has a prefix that holds a row), and behind them, where it has, its prefix's sums (Far)
+  int4* DESC;
 
   __device__ __forceinline__ int far_rows(int p) const {
     const long long slot = FAR_SLOT[p];
@@ -115,15 +119,6 @@ struct AttnArgs {
 struct Far {
   int first, count, tiles, row;
 };
-__device__ __forceinline__ Far far_of(const AttnArgs& a, int b) {
-  Far f{0, 0, 1, 0};
-  const int p = a.OF[b];
-  if ((unsigned)p < (unsigned)a.prefixes && a.far_rows(p) > 0) {
-    const int4 d = a.DESC[b];
-    f = Far{d.x, d.y, d.z, d.w};
-  }
-  return f;
-}
 
 // What a window leaves of a sequence's rows: virtual row j is slot j + (j < sinks16 ? 0 : gap),
 // and rows m0 .. m1 - 1 are no keys (they share a run of 16 slots with one).
@@ -248,11 +243,9 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* sums, int
   return before;
 }
 
-// Chunk `gx` of the call; the result is uniform.
+// Chunk `gx` of the call; the result is uniform. sums, found: PG_T / 64 and 4 words of LDS.
 template <int FORM>
-__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int tid) {
-  __shared__ uint32_t sums[PG_T / 64];
-  __shared__ int found[4];
+__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, int gx, int tid, uint32_t* sums, int* found) {
   const int lane = tid & 63;
   if (a.target == 0) {
     const int n = rows_of<FORM>(a, gx);
@@ -327,27 +320,39 @@ __device__ __forceinline__ Chunk sequence_chunks(const AttnArgs& a, int b, int t
   return k;
 }
 
+// The LDS of four waves: a region a wave for V's rows (at the end 16 fp32 rows of O), and small things.
+template <int D>
+struct AttnLds {
+  static constexpr int REGION = PG_KEYS * D * 2;
+  float m_s[PG_WAVES][PG_HEADS], l_s[PG_WAVES][PG_HEADS];
+  uint32_t sums[PG_T / 64];
+  int found[4];
+};
+
+// Chunk gx, kv head and 16 of its query heads `part` (none past the last), by PG_T threads.
 template <int DT, int D, int FORM>
-__global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attend_chunk(const AttnArgs& a, int gx, int part, int tid, uint8_t* lds, AttnLds<D>& sh) {
   constexpr bool TRACK = (FORM & PG_TRACK) != 0, WINDOW = (FORM & PG_WINDOW) != 0;
   constexpr int KC = D / 32, DC = D / 16;       // 32-wide steps of q . k, 16-wide tiles of V^T
   constexpr int VPL = PG_KEYS * D * 2 / 1024;   // 16-byte pieces of the 32 V rows a lane
   constexpr int VR = 1024 / (D * 2);            // V rows a load of the wave covers
-  constexpr int REGION = PG_KEYS * D * 2;       // a wave's LDS: V rows, at the end 16 fp32 rows of O
+  constexpr int REGION = AttnLds<D>::REGION;
   static_assert(REGION == PG_HEADS * D * 4, "the output tile takes the V rows' place");
-  __shared__ __align__(16) uint8_t lds[PG_WAVES * REGION];
-  __shared__ float m_s[PG_WAVES][PG_HEADS], l_s[PG_WAVES][PG_HEADS];
+  auto& m_s = sh.m_s;
+  auto& l_s = sh.l_s;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int group = a.nh / a.c.nkv, hgs = (group + PG_HEADS - 1) / PG_HEADS;
-  const int wide = a.c.nkv * hgs, part = blockIdx.x % wide, gx = blockIdx.x / wide;
+  // (a part past the last: the last one's addresses, no head and no key)
+  const bool idle = (FORM & PG_PREFIX) != 0 && part >= a.c.nkv * hgs;
+  if (idle) part = a.c.nkv * hgs - 1;
   const int h = part / hgs, head0 = h * group + (part % hgs) * PG_HEADS;
-  const int heads = min(PG_HEADS, (h + 1) * group - head0);
-  const Chunk ck = find_chunk<FORM>(a, gx, tid);
+  const int heads = idle ? 0 : min(PG_HEADS, (h + 1) * group - head0);
+  const Chunk ck = find_chunk<FORM>(a, gx, tid, sh.sums, sh.found);
   if (ck.b < 0) return;  // (a sequence without a row has no chunk; with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
-  const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
+  const int k0 = ck.c * ck.size, k1 = idle ? k0 : min(k0 + ck.size, ck.n);
   const int mask = (1 << a.c.shift) - 1;
   const Window win = window_of<FORM>(a, WINDOW ? __builtin_amdgcn_readfirstlane(a.c.rows(a.SLOT[b])) : 0);
   uint8_t* const vs = lds + wave * REGION;
@@ -571,32 +576,49 @@ __global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArg
   }
 }
 
-// Row of PM, PL and PACC of query head `head`'s c-th part: its own chunks', then its prefix's.
-template <int FORM>
-__device__ __forceinline__ size_t part_row(const AttnArgs& a, const Chunk& ck, const Far& far, int head, int c) {
-  if constexpr ((FORM & PG_PREFIX) != 0) {
-    if (c >= ck.count) {
-      const int group = a.nh / a.c.nkv, row = far.row + head % group;
-      const size_t item = far.first + (size_t)(c - ck.count) * far.tiles + row / a.far_tile;
-      return a.far_base + (item * a.c.nkv + head / group) * a.far_tile + row % a.far_tile;
-    }
+template <int DT, int D, int FORM>
+__global__ __launch_bounds__(64 * PG_WAVES) void paged_attn_kernel(const AttnArgs a) {
+  __shared__ __align__(16) uint8_t lds[PG_WAVES * AttnLds<D>::REGION];
+  __shared__ AttnLds<D> sh;
+  const int group = a.nh / a.c.nkv, wide = a.c.nkv * ((group + PG_HEADS - 1) / PG_HEADS);
+  attend_chunk<DT, D, FORM>(a, blockIdx.x / wide, blockIdx.x % wide, threadIdx.x, lds, sh);
+}
+
+// Rows of PM, PL and PACC that hold query head `head`'s parts: its own chunks', then its prefix's.
+struct Parts {
+  int count, own;        // how many, and how many of them its own chunks'
+  size_t own0, far0;     // the first of each
+  size_t step, far_step;
+  __device__ __forceinline__ size_t row(int c) const {
+    return c < own ? own0 + c * step : far0 + (size_t)(c - own) * far_step;
   }
-  return (size_t)(ck.first + c) * a.nh + head;
+};
+template <int FORM>
+__device__ __forceinline__ Parts parts_of(const AttnArgs& a, const Chunk& ck, const Far& far, int head) {
+  Parts p{ck.count, ck.count, (size_t)ck.first * a.nh + head, 0, (size_t)a.nh, 0};
+  if constexpr ((FORM & PG_PREFIX) != 0) {
+    const int group = a.nh / a.c.nkv, h = head / group, r = far.row + head - h * group, tile = r / a.far_tile;
+    p.count += far.count;
+    p.far0 = a.far_base + ((size_t)(far.first + tile) * a.c.nkv + h) * a.far_tile + (r - tile * a.far_tile);
+    p.far_step = (size_t)far.tiles * a.c.nkv * a.far_tile;
+  } else {
+    p.own = 0x7fffffff;
+  }
+  return p;
 }
 
 // The reference and sum of one query head over a sequence's `count` parts, by a wave;
 // uniform. den < 0: no key.
-template <int FORM>
-__device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, const Far& far, int count, int head, int lane,
-                                          float* m, float* den) {
+__device__ __forceinline__ void join_sums(const AttnArgs& a, const Parts& parts, int lane, float* m, float* den) {
+  const int count = parts.count;
   float mx = PG_NONE;
-  for (int c = lane; c < count; c += 64) mx = fmaxf(mx, a.PM[part_row<FORM>(a, ck, far, head, c)]);
+  for (int c = lane; c < count; c += 64) mx = fmaxf(mx, a.PM[parts.row(c)]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
   float l = 0.0f;
   bool any = false;
   for (int c = lane; c < count; c += 64) {
-    const size_t at = part_row<FORM>(a, ck, far, head, c);
+    const size_t at = parts.row(c);
     const float x = a.PL[at];
     if (x < 0.0f) continue;
     l += x * __builtin_amdgcn_exp2f(a.PM[at] - mx);
@@ -612,26 +634,27 @@ __device__ __forceinline__ void join_sums(const AttnArgs& a, const Chunk& ck, co
 // threads. The chunks' sums of the first round are on their way before the
 // joined reference is known.
 template <int DT, int D, int FORM>
-__device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, const Far& far, int count, int head, int tid) {
+__device__ __forceinline__ void join_head(const AttnArgs& a, const Parts& parts, int b, int head, int tid) {
   constexpr int ROWS = 256 / (D / 4);  // chunks read at once, four elements a lane
   constexpr int AHEAD = 8;             // reads of a lane under way together
   __shared__ f32x4 part[256];
-  __shared__ float w_s[PG_WGS + (FORM & PG_PREFIX ? PG_WGS : 0)];  // the parts' weights (chunk_len: at most `target` of each kind)
+  const int count = parts.count;
+  __shared__ float w_s[PG_WGS + (FORM & PG_PREFIX ? PF_CHUNKS : 0)];  // the parts' weights (chunk_len: at most `target` chunks)
   const int e = tid % (D / 4), r0 = tid / (D / 4);
   f32x4 x[AHEAD];
   auto load = [&](int c0) {  // past the last chunk: the last one's, not used
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const size_t at = part_row<FORM>(a, ck, far, head, min(c0 + r0 + i * ROWS, count - 1));
+      const size_t at = parts.row(min(c0 + r0 + i * ROWS, count - 1));
       x[i] = reinterpret_cast<const f32x4*>(a.PACC + at * D)[e];
     }
   };
   load(0);
   float m, den;
-  join_sums<FORM>(a, ck, far, count, head, tid & 63, &m, &den);
+  join_sums(a, parts, tid & 63, &m, &den);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int c = tid; c < count; c += 256)  // (a chunk without a key: weight times zeros)
-    w_s[c] = __builtin_amdgcn_exp2f(a.PM[part_row<FORM>(a, ck, far, head, c)] - m);
+    w_s[c] = __builtin_amdgcn_exp2f(a.PM[parts.row(c)] - m);
   __syncthreads();
   for (int c0 = 0; c0 < count; c0 += ROWS * AHEAD) {
     if (c0) load(c0);
@@ -657,20 +680,31 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, const Chunk& ck, co
     for (int i = 0; i < 4; ++i) q[i] = den < 0.0f ? 0.0f : quotient(acc[i], den);
     out.x = Elem<DT>::store(q[0]) | (uint32_t)Elem<DT>::store(q[1]) << 16;
     out.y = Elem<DT>::store(q[2]) | (uint32_t)Elem<DT>::store(q[3]) << 16;
-    reinterpret_cast<uint2*>(a.Y + ((size_t)ck.b * a.nh + head) * D)[tid] = out;
+    reinterpret_cast<uint2*>(a.Y + ((size_t)b * a.nh + head) * D)[tid] = out;
   }
+}
+
+// The chunks of sequence b and its prefix's; all 256 threads.
+template <int FORM>
+__device__ __forceinline__ Chunk chunks_of(const AttnArgs& a, int b, int tid, Far* far) {
+  *far = Far{0, 0, 1, 0};
+  if constexpr ((FORM & PG_PREFIX) != 0) {
+    const int4 own = a.DESC[b], pre = a.DESC[a.seqs + b];
+    if (own.z) *far = Far{pre.x, pre.y, pre.z, pre.w};
+    return Chunk{b, 0, 0, own.y, own.x, 0};
+  }
+  return sequence_chunks<FORM>(a, b, tid);
 }
 
 // Query head `head` of sequence b, where the first launch has not finished it.
 template <int DT, int D, int FORM>
 __device__ __forceinline__ void join_sequence(const AttnArgs& a, int b, int head, int tid) {
-  const Chunk ck = sequence_chunks<FORM>(a, b, tid);
-  Far far{0, 0, 1, 0};
-  if constexpr ((FORM & PG_PREFIX) != 0) far = far_of(a, b);
-  const int count = ck.count + far.count;
-  if (count > (FORM & PG_PREFIX ? 0 : 1))
-    join_head<DT, D, FORM>(a, ck, far, count, head, tid);
-  else if (count == 0)  // no row, so no chunk. (In the first launch, stores that never ran took 10 % off its speed.)
+  Far far;
+  const Chunk ck = chunks_of<FORM>(a, b, tid, &far);
+  const Parts parts = parts_of<FORM>(a, ck, far, head);
+  if (parts.count > (FORM & PG_PREFIX ? 0 : 1))
+    join_head<DT, D, FORM>(a, parts, b, head, tid);
+  else if (parts.count == 0)  // no row, so no chunk. (In the first launch, stores that never ran took 10 % off its speed.)
     for (int i = tid; i < D / 8; i += 256)
       reinterpret_cast<u32x4*>(a.Y + ((size_t)b * a.nh + head) * D)[i] = u32x4{0u, 0u, 0u, 0u};
 }
@@ -695,10 +729,12 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
     return;
   }
   const int h = blockIdx.x % a.c.nkv, group = a.nh / a.c.nkv;
-  const Chunk ck = find_chunk<FORM>(a, blockIdx.x / a.c.nkv, tid);
+  __shared__ uint32_t sums[PG_T / 64];
+  __shared__ int found[4];
+  const Chunk ck = find_chunk<FORM>(a, blockIdx.x / a.c.nkv, tid, sums, found);
   if (ck.b < 0 || (!(FORM & PG_PREFIX) && ck.count == 1 && group <= PG_HEADS)) return;  // (finished by the first launch)
   Far far{0, 0, 1, 0};
-  if constexpr ((FORM & PG_PREFIX) != 0) far = far_of(a, ck.b);
+  if constexpr ((FORM & PG_PREFIX) != 0) chunks_of<FORM>(a, ck.b, tid, &far);
   const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   constexpr bool WINDOW = (FORM & PG_WINDOW) != 0;
   const Window win = window_of<FORM>(a, WINDOW ? a.c.rows(a.SLOT[ck.b]) : 0);
@@ -709,7 +745,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const AttnArgs a, int
     __syncthreads();
     for (int g = wave; g < gs; g += 4) {
       float m, den;
-      join_sums<FORM>(a, ck, far, ck.count + far.count, h * group + g0 + g, lane, &m, &den);
+      join_sums(a, parts_of<FORM>(a, ck, far, h * group + g0 + g), lane, &m, &den);
       if (lane == 0) m_s[g] = m, l_s[g] = den;
     }
     __syncthreads();

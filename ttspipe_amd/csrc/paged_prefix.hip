@@ -60,7 +60,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
   const uint32_t tiles = n ? (uint32_t)((m * group + a.far_tile - 1) / a.far_tile) : 0;
   uint32_t total;
   pf_prefix(tiles * units(n), sums, tid, &total);
-  const uint32_t len = max((total + a.far_target - 1) / (uint32_t)a.far_target, 1u);
+  const uint32_t len = min(max((total + a.far_target - 1) / (uint32_t)a.far_target, 1u), PF_CHUNK / PG_STEP);
   const int count = n ? chunk_count(n, len) : 0;
   const int first = (int)pf_prefix(tiles * count, sums, tid, &total);
   Item it{-1, 0, 0, 0, 0, 1, 0, 0};
@@ -80,8 +80,28 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
   return it;
 }
 
-template <int DT, int D, int RG>
-__global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a) {
+// The sequences' own chunks as the own rows' kernel cuts them, for the joining launch
+// (one workgroup).
+template <int FORM>
+__device__ __forceinline__ void describe(const AttnArgs& a, int tid) {
+  __shared__ uint32_t sums[TA_WAVES];
+  const int per = (a.seqs + TA_T - 1) / TA_T, b0 = tid * per;
+  uint32_t mine = 0, total;
+  for (int i = 0; i < per; ++i) mine += units(rows_of<FORM>(a, b0 + i));
+  pf_prefix(mine, sums, tid, &total);
+  const uint32_t len = chunk_len(a, total);
+  mine = 0;
+  for (int i = 0; i < per; ++i) mine += chunk_count(rows_of<FORM>(a, b0 + i), len);
+  int first = (int)pf_prefix(mine, sums, tid, &total);
+  for (int i = 0; i < per && b0 + i < a.seqs; ++i) {
+    const int b = b0 + i, count = chunk_count(rows_of<FORM>(a, b), len), p = a.OF[b];
+    a.DESC[b] = make_int4(first, count, (unsigned)p < (unsigned)a.prefixes && a.far_rows(p) > 0, 0);
+    first += count;
+  }
+}
+
+template <int DT, int D, int RG, int FORM>
+__global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a, int items) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef Tile<D, RG> C;
   constexpr int QT = 32 * RG;
@@ -89,9 +109,24 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a)
   __shared__ __align__(256) uint8_t ring1[C::STAGE];
   __shared__ __align__(256) uint8_t ring2[C::ST > 2 ? C::STAGE : 16];
   __shared__ int seq_s[QT + 2], wcnt[TA_WAVES];
+  __shared__ __align__(16) unsigned long long run_s[PF_CHUNK / 16][2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = a.nh / a.c.nkv, h = blockIdx.x % a.c.nkv, gx = blockIdx.x / a.c.nkv;
+  if ((int)blockIdx.x >= items) {
+    const int i = blockIdx.x - items;
+    if (i == 0) {
+      describe<FORM>(a, tid);
+      return;
+    }
+    // the sequences' own rows: neighbouring heads of one chunk side by side, four waves each
+    __shared__ AttnLds<D> sh[2];
+    const int half = __builtin_amdgcn_readfirstlane(tid >> 8), wide = a.c.nkv * ((group + PG_HEADS - 1) / PG_HEADS);
+    const int pairs = (wide + 1) / 2, part = 2 * ((i - 1) % pairs) + half;
+    static_assert(2 * PG_T == TA_T && PG_WAVES * AttnLds<D>::REGION <= C::STAGE, "two halves, a stage of the ring each");
+    attend_chunk<DT, D, FORM>(a, (i - 1) / pairs, part, tid & (PG_T - 1), half ? ring1 : ring0, sh[half]);
+    return;
+  }
   const Item it = find_item(a, gx, tid);
   if (it.p < 0) return;
   const int row0 = it.tile * QT, rows = min(QT, it.members * group - row0);
@@ -116,7 +151,7 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a)
   if (it.c == 0 && h == 0)  // for the joining launch: where a sequence's parts are
     for (int i = tid; i < o1 - o0; i += TA_T)
       if ((o0 + i) * group >= row0)
-        a.DESC[seq_s[i]] = make_int4(it.first, it.count, it.tiles, (o0 + i) * group);
+        a.DESC[a.seqs + seq_s[i]] = make_int4(it.first, it.count, it.tiles, (o0 + i) * group);
 
   const int rg = wave % RG, kg = wave / RG;
   const int myrow = 32 * rg + (lane & 31);  // this lane's query row of the tile
@@ -131,75 +166,72 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a)
   }
   const float scale2 = a.scale2 == 0.0f ? 1e-30f : fabsf(a.scale2);  // (0: -inf times it is to stay so)
 
-  const int size = chunk_size(it.n, it.count), k0 = it.c * size, k1 = min(k0 + size, it.n);
-  const int mask = (1 << a.c.shift) - 1;
-  // (constant memory while the kernel runs: scalar loads, which the ring's waits do not count)
-  typedef const __attribute__((address_space(4))) int* table_ptr;
-  const table_ptr trow = (table_ptr)(a.far_table + it.p * a.far_stride);
-  auto page_at = [&](int j) {
-    const int p = j < k1 ? trow[j >> a.c.shift] : -1;
-    return (unsigned)p < (unsigned)a.c.pages ? p : -1;
-  };
-  // Pages asked for a tile ahead of their use: of this wave's loads, of what has
-  // landed, and of the runs it computes.
-  int pn[C::PER], pl[C::PER], pc[C::SB][2];
-  // this wave's loads of a tile: PER runs of RPI rows from row PER RPI wave on; a hole reads page 0
+  const int size = chunk_size(it.n, it.count), k0 = min(it.c * size, it.n), k1 = min(k0 + size, it.n);
+  // Where the chunk's runs of 16 rows lie (bit 0 of V's address: a hole, for which page 0's are read).
+  const int mask = (1 << a.c.shift) - 1, runs = (k1 - k0 + 15) / 16;
+  bool holes = false;
+  for (int i = tid; i < runs; i += TA_T) {
+    const int j = k0 + 16 * i, page = a.far_table[it.p * a.far_stride + (j >> a.c.shift)];
+    const bool hole = (unsigned)page >= (unsigned)a.c.pages;
+    const long long q = hole ? 0 : page, r = j & mask;
+    run_s[i][0] = (unsigned long long)(a.c.K + q * a.c.k_page + h * a.c.k_head + r * a.c.k_row);
+    run_s[i][1] = (unsigned long long)(a.c.V + q * a.c.v_page + h * a.c.v_head + r * a.c.v_row) | hole;
+    holes = holes || hole;
+  }
+  holes = __syncthreads_or(holes);
+  // this wave's loads of a tile: PER of RPI rows from row PER RPI wave on, all in one run
   uint32_t ko[C::PER], vo[C::PER];
 #pragma unroll
   for (int i = 0; i < C::PER; ++i) {
-    const int lrow = lane / C::PPR, piece = (lane % C::PPR) ^ ta_swz<D>((wave * C::PER + i) * C::RPI + lrow);
-    ko[i] = (uint32_t)(lrow * (int)a.c.k_row) * 2 + piece * 16;
-    vo[i] = (uint32_t)(lrow * (int)a.c.v_row) * 2 + piece * 16;
+    const int lrow = lane / C::PPR, row = (wave * C::PER + i) * C::RPI;
+    const int piece = (lane % C::PPR) ^ ta_swz<D>(row + lrow);
+    ko[i] = (uint32_t)((row % 16 + lrow) * (int)a.c.k_row) * 2 + piece * 16;
+    vo[i] = (uint32_t)((row % 16 + lrow) * (int)a.c.v_row) * 2 + piece * 16;
   }
-  const int lr0 = k0 + wave * C::PER * C::RPI, cr0 = k0 + 32 * C::SB * kg;
-  auto pages_loaded = [&](int t, int (&p)[C::PER]) {
-#pragma unroll
-    for (int i = 0; i < C::PER; ++i) p[i] = page_at(lr0 + t * C::KEYS + i * C::RPI);
-  };
-  auto pages_run = [&](int t) {
-#pragma unroll
-    for (int b = 0; b < C::SB; ++b)
-      pc[b][0] = page_at(cr0 + t * C::KEYS + 32 * b), pc[b][1] = page_at(cr0 + t * C::KEYS + 32 * b + 16);
-  };
-  pages_loaded(0, pn);
-  pages_loaded(0, pl);
-  pages_run(0);
+  static_assert(C::PER * C::RPI <= 16, "a wave's rows of a tile lie in one run");
+  const int lr0 = wave * C::PER * C::RPI, last = max(runs - 1, 0);
+  auto run_at = [&](int t) { return *reinterpret_cast<const u32x4*>(run_s[min((t * C::KEYS + lr0) / 16, last)]); };
+  u32x4 next = run_at(0);  // (asked for a tile ahead)
   auto load = [&](int t, uint8_t* ring) {
+    uint32_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = __builtin_amdgcn_readfirstlane(next[i]);
+    const void* const kp = (const void*)((unsigned long long)at[1] << 32 | at[0]);
+    const void* const vp = (const void*)((unsigned long long)at[3] << 32 | (at[2] & ~1u));
 #pragma unroll
     for (int i = 0; i < C::PER; ++i) {
-      const int row = (wave * C::PER + i) * C::RPI, p = max(pn[i], 0);
-      const long long r = (lr0 + t * C::KEYS + i * C::RPI) & mask;
-      ta_load(a.c.K + p * a.c.k_page + h * a.c.k_head + r * a.c.k_row, ko[i], ring + row * C::ROWB);
-      ta_load(a.c.V + p * a.c.v_page + h * a.c.v_head + r * a.c.v_row, vo[i], ring + C::HALF + row * C::ROWB);
+      ta_load(kp, ko[i], ring + (wave * C::PER + i) * 1024);
+      ta_load(vp, vo[i], ring + C::HALF + (wave * C::PER + i) * 1024);
     }
-    pages_loaded(t + 1, pn);
+    next = run_at(t + 1);
   };
+  auto hole_at = [&](int r) { return holes && (run_s[min(r / 16, last)][1] & 1); };  // row r of the chunk
+  const int n = k1 - k0;
   // V rows that are no keys are zeros (what they hold may be NaN)
   auto landed = [&](int t, uint8_t* ring) {
+    const int r0 = t * C::KEYS + lr0;
+    if (!holes && r0 + C::PER * C::RPI <= n) return;
+    const bool hole = hole_at(r0);
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) {
-      const int j = lr0 + t * C::KEYS + i * C::RPI;
-      if (pl[i] < 0 || j + C::RPI > k1)
-        if (pl[i] < 0 || j + lane / C::PPR >= k1)
-          *reinterpret_cast<u32x4*>(ring + C::HALF + (wave * C::PER + i) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
-    }
-    pages_loaded(t + 1, pl);
+    for (int i = 0; i < C::PER; ++i)
+      if (hole || r0 + i * C::RPI + lane / C::PPR >= n)
+        *reinterpret_cast<u32x4*>(ring + C::HALF + (wave * C::PER + i) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
   };
   bool seen = false;
   auto compute = [&](int t, uint8_t* ring) {
 #pragma unroll
     for (int b = 0; b < C::SB; ++b) {
-      const int row = 32 * (C::SB * kg + b), j = k0 + t * C::KEYS + row, p0 = pc[b][0], p1 = pc[b][1];
-      if (j >= k1) continue;
-      seen = seen || p0 >= 0 || p1 >= 0;
-      w.run(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, j + 32 > k1 || p0 < 0 || p1 < 0,
-            [&](int i) { return j + i >= k1 || (i < 16 ? p0 : p1) < 0; });
+      const int row = 32 * (C::SB * kg + b), r0 = t * C::KEYS + row;
+      if (r0 >= n) continue;
+      const bool h0 = hole_at(r0), h1 = hole_at(r0 + 16);
+      seen = seen || !h0 || (!h1 && r0 + 16 < n);
+      w.run(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, r0 + 32 > n || h0 || h1,
+            [&](int i) { return r0 + i >= n || (i < 16 ? h0 : h1); });
     }
-    pages_run(t + 1);
   };
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(w.q[i]));  // (waited for here, not among the loop's loads)
-  ta_tiles<C>((k1 - k0 + C::KEYS - 1) / C::KEYS, ring0, ring1, ring2, load, landed, compute);
+  ta_tiles<C>((n + C::KEYS - 1) / C::KEYS, ring0, ring1, ring2, load, landed, compute);
   ta_join<C>(w, seen, ring0, ring1, ring2, rg, kg, lane);
 
   if (kg == 0 && myrow < rows) {
@@ -232,7 +264,9 @@ inline bool prefix_plan(int seqs, int nh, int nkv, int prefixes, long long far_c
   const long long tiles = rows / p->tile + (prefixes < seqs ? prefixes : seqs);
   const long long units = (far_cap + PG_STEP - 1) / PG_STEP;
   if (tiles * units > 0x3fffffff) return false;
-  const long long items = p->target + tiles < tiles * units ? p->target + tiles : tiles * units;
+  // chunks of the length that makes `target` of them, or of the longest
+  const long long most = tiles + (p->target > tiles * units / (PF_CHUNK / PG_STEP) ? p->target : tiles * units / (PF_CHUNK / PG_STEP));
+  const long long items = most < tiles * units ? most : tiles * units;
   if (items * nkv > PG_MAX_GRID) return false;
   p->items = (int)items;
   p->rows = (size_t)items * nkv * p->tile;
@@ -253,11 +287,12 @@ struct PrefixWork {
 static bool prefix_work(int seqs, int nh, int nkv, int hd, long long cap, long long rows, int prefixes, long long far_cap,
                         bool tracked, PrefixWork* w) {
   if (!attn_plan(seqs, nh, nkv, hd, cap, rows, tracked, true, &w->own) ||
-      !prefix_plan(seqs, nh, nkv, prefixes, far_cap, &w->far))
-    return false;
+      !prefix_plan(seqs, nh, nkv, prefixes, far_cap, &w->far) ||
+      (long long)w->far.items * nkv + 1 + (long long)w->own.chunks * nkv * w->own.hgs > PG_MAX_GRID / 2)
+    return false;  // (workgroups of 512 threads)
   w->rows = (size_t)w->own.chunks * nh + w->far.rows;
   w->desc = (w->rows * (2 + hd) + 3) / 4 * 4;
-  w->scores = w->desc + (size_t)seqs * 4;
+  w->scores = w->desc + (size_t)seqs * 8;
   w->total = w->scores + w->own.scores;
   return (w->total + 255) / 256 <= 0x7fffffff;
 }
@@ -279,14 +314,14 @@ extern "C" int ttsp_paged_attention_prefix_work_kib(int seqs, int nh, int nkv, i
 
 template <int FORM>
 static int prefix_launch(const AttnArgs& a, const PrefixWork& w, int hd, int dtype, hipStream_t stream) {
-  const dim3 far((unsigned)(w.far.items * a.c.nkv)), own((unsigned)(w.own.chunks * a.c.nkv * w.own.hgs));
+  const int items = w.far.items * a.c.nkv;
+  const dim3 grid((unsigned)(items + 1 + w.own.chunks * ((a.c.nkv * w.own.hgs + 1) / 2)));
   const int gathers = w.own.chunks * a.c.nkv;
 #define TTSP_PFX(DTV, DV)                                                                                              \
   do {                                                                                                                 \
-    if (w.far.tile == 64) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 2>), far, dim3(TA_T), 0, stream, a);         \
-    else if (w.far.tile == 128) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4>), far, dim3(TA_T), 0, stream, a);   \
-    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 8>), far, dim3(TA_T), 0, stream, a);                          \
-    hipLaunchKernelGGL((paged_attn_kernel<DTV, DV, FORM>), own, dim3(64 * PG_WAVES), 0, stream, a);                     \
+    if (w.far.tile == 64) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 2, FORM>), grid, dim3(TA_T), 0, stream, a, items);         \
+    else if (w.far.tile == 128) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4, FORM>), grid, dim3(TA_T), 0, stream, a, items);   \
+    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 8, FORM>), grid, dim3(TA_T), 0, stream, a, items);                          \
     if (FORM & PG_TRACK)                                                                                               \
       hipLaunchKernelGGL((paged_gather_kernel<DTV, DV, FORM>), dim3(gathers + a.seqs * a.nh), dim3(256), 0, stream, a,  \
                          gathers);                                                                                     \

@@ -103,11 +103,24 @@ struct TaWave {
       for (int r = 0; r < 16; ++r)
         if (gone(8 * (r / 4) + h4 + r % 4)) s[r] = -__builtin_inff();
     }
-    float bm = s[0];
+    // The weights with the reference as it is, and only where they come out too large
+    // (sixteen of 2^8 and less sum up to no more than 4096) the maximum, a new reference and the
+    // weights again. fp16 weights have no room for that: their maximum is looked at first.
+    float p[16], sum = 0.0f;
+    auto weigh = [&]() {
+      sum = 0.0f;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
-    bm *= scale2;
-    if (__any(bm > m + pg_above<DT>)) {
+      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -m));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += p[r];
+    };
+    auto largest = [&]() {
+      float bm = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+      return bm * scale2;
+    };
+    auto move = [&](float bm) {
       bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
       const float mnew = bm > m + pg_above<DT> ? bm - pg_below<DT> : m;
       const float alpha = __builtin_amdgcn_exp2f(m - mnew);
@@ -117,18 +130,26 @@ struct TaWave {
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    };
+    if constexpr (DT == DT_F16) {
+      const float bm = largest();
+      if (__any(bm > m + pg_above<DT>)) move(bm);
+      weigh();
+    } else {
+      weigh();
+      if (__any(!(sum <= 4096.0f))) {
+        move(largest());
+        weigh();
+      }
     }
+    l += sum;
     u32x4 pf[2][PARTS];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + 2 * u], scale2, -m));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + 2 * u + 1], scale2, -m));
-        l += p0;
-        l += p1;
         uint32_t parts[PARTS];
-        ta_split<DT, PARTS>(p0, p1, parts);
+        ta_split<DT, PARTS>(p[8 * c + 2 * u], p[8 * c + 2 * u + 1], parts);
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) pf[c][i][u] = parts[i];
       }
@@ -136,9 +157,8 @@ struct TaWave {
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint8_t* const p = v + 16 * c * (D * 2) + (vb ^ (d << 6));
-        const uint8_t* const p8 = v + (16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32);
-        const uint2 lo = pg_ld_tr(p), hi = pg_ld_tr(p8);
+        const uint2 lo = pg_ld_tr(v + 16 * c * (D * 2) + (vb ^ (d << 6)));
+        const uint2 hi = pg_ld_tr(v + (16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32));
         const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) o[d] = mfma32<DT>(vt, pf[c][i], o[d]);
