@@ -74,6 +74,7 @@ constexpr int PG_WGS = 1024;
 constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 // Rows a prefix's chunk has at most (their runs' places are held in LDS), and so its most chunks.
+constexpr int PF_OWN = 512;
 constexpr int PF_CHUNK = 8192, PF_CHUNKS = TTSP_PAGED_MAX_SLOTS / PF_CHUNK;
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 // A moved reference lies `pg_below` under the largest score and moves again when a
@@ -329,7 +330,7 @@ struct AttnLds {
   int found[4];
 };
 
-// Chunk gx, kv head and 16 of its query heads `part` (none past the last), by PG_T threads.
+// Chunk gx, kv head and 16 of its query heads `part` , by PG_T threads.
 template <int DT, int D, int FORM>
 __device__ __forceinline__ void attend_chunk(const AttnArgs& a, int gx, int part, int tid, uint8_t* lds, AttnLds<D>& sh) {
   constexpr bool TRACK = (FORM & PG_TRACK) != 0, WINDOW = (FORM & PG_WINDOW) != 0;
@@ -344,15 +345,12 @@ __device__ __forceinline__ void attend_chunk(const AttnArgs& a, int gx, int part
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int group = a.nh / a.c.nkv, hgs = (group + PG_HEADS - 1) / PG_HEADS;
-  // (a part past the last: the last one's addresses, no head and no key)
-  const bool idle = (FORM & PG_PREFIX) != 0 && part >= a.c.nkv * hgs;
-  if (idle) part = a.c.nkv * hgs - 1;
   const int h = part / hgs, head0 = h * group + (part % hgs) * PG_HEADS;
-  const int heads = idle ? 0 : min(PG_HEADS, (h + 1) * group - head0);
+  const int heads = min(PG_HEADS, (h + 1) * group - head0);
   const Chunk ck = find_chunk<FORM>(a, gx, tid, sh.sums, sh.found);
   if (ck.b < 0) return;  // (a sequence without a row has no chunk; with target == 0 an empty one)
   const int b = __builtin_amdgcn_readfirstlane(ck.b);
-  const int k0 = ck.c * ck.size, k1 = idle ? k0 : min(k0 + ck.size, ck.n);
+  const int k0 = ck.c * ck.size, k1 = min(k0 + ck.size, ck.n);
   const int mask = (1 << a.c.shift) - 1;
   const Window win = window_of<FORM>(a, WINDOW ? __builtin_amdgcn_readfirstlane(a.c.rows(a.SLOT[b])) : 0);
   uint8_t* const vs = lds + wave * REGION;
@@ -771,7 +769,8 @@ inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, long lon
   const int group = nh / nkv;
   p->hgs = (group + PG_HEADS - 1) / PG_HEADS;
   const long long wide = (long long)nkv * p->hgs;
-  p->target = (int)(wide < PG_WGS ? PG_WGS / wide : 1);
+  const int wgs = joined ? PF_OWN : PG_WGS;
+  p->target = (int)(wide < wgs ? wgs / wide : 1);
   p->parts = p->scores = 0;
   if ((long long)seqs * ((rows + PG_STEP - 1) / PG_STEP) > 0x3fffffff) return false;  // (more rows than any memory holds)
   const bool one = rows <= PG_SHORT && !joined;

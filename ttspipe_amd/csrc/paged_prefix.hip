@@ -14,24 +14,8 @@
 namespace ttsp {
 
 constexpr int PF_MAX = 256;   // prefixes of a call (one a thread)
-constexpr int PF_WGS = 256;   // workgroups the chunks are meant to make, one a CU
+constexpr int PF_WGS = 512;   // workgroups the chunks are meant to make, two a CU
 constexpr int PF_PARTS = 2;
-
-// The sum of v over the workgroup's threads, and over those before this one.
-__device__ __forceinline__ uint32_t pf_prefix(uint32_t v, uint32_t* sums, int tid, uint32_t* total) {
-  const uint32_t upto = lane_prefix(v);
-  __syncthreads();
-  if ((tid & 63) == 63) sums[tid >> 6] = upto;
-  __syncthreads();
-  uint32_t before = upto - v, all = 0;
-#pragma unroll
-  for (int w = 0; w < TA_WAVES; ++w) {
-    if (w < (tid >> 6)) before += sums[w];
-    all += sums[w];
-  }
-  *total = all;
-  return before;
-}
 
 // Item gx of the call: a chunk of a prefix and a tile of its query rows.
 struct Item {
@@ -49,6 +33,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
   __shared__ int found[6];
   static_assert(PF_MAX <= TA_T, "a thread a prefix");
   const int group = a.nh / a.c.nkv;
+  const int all = tid < a.prefixes ? a.far_rows(tid) : 0;  // (asked for before what it waits for)
   cnt[tid] = 0;
   __syncthreads();
   for (int b = tid; b < a.seqs; b += TA_T) {
@@ -56,13 +41,13 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, int gx, int tid) {
     if ((unsigned)p < (unsigned)a.prefixes) atomicAdd(&cnt[p], 1);
   }
   __syncthreads();
-  const int m = cnt[tid], n = m ? a.far_rows(tid) : 0;
+  const int m = cnt[tid], n = m ? all : 0;
   const uint32_t tiles = n ? (uint32_t)((m * group + a.far_tile - 1) / a.far_tile) : 0;
   uint32_t total;
-  pf_prefix(tiles * units(n), sums, tid, &total);
+  block_prefix(tiles * units(n), sums, tid, &total);
   const uint32_t len = min(max((total + a.far_target - 1) / (uint32_t)a.far_target, 1u), PF_CHUNK / PG_STEP);
   const int count = n ? chunk_count(n, len) : 0;
-  const int first = (int)pf_prefix(tiles * count, sums, tid, &total);
+  const int first = (int)block_prefix(tiles * count, sums, tid, &total);
   Item it{-1, 0, 0, 0, 0, 1, 0, 0};
   if ((uint32_t)gx >= total) return it;
   if (gx >= first && gx < first + (int)tiles * count) {  // one thread
@@ -88,11 +73,11 @@ __device__ __forceinline__ void describe(const AttnArgs& a, int tid) {
   const int per = (a.seqs + TA_T - 1) / TA_T, b0 = tid * per;
   uint32_t mine = 0, total;
   for (int i = 0; i < per; ++i) mine += units(rows_of<FORM>(a, b0 + i));
-  pf_prefix(mine, sums, tid, &total);
+  block_prefix(mine, sums, tid, &total);
   const uint32_t len = chunk_len(a, total);
   mine = 0;
   for (int i = 0; i < per; ++i) mine += chunk_count(rows_of<FORM>(a, b0 + i), len);
-  int first = (int)pf_prefix(mine, sums, tid, &total);
+  int first = (int)block_prefix(mine, sums, tid, &total);
   for (int i = 0; i < per && b0 + i < a.seqs; ++i) {
     const int b = b0 + i, count = chunk_count(rows_of<FORM>(a, b), len), p = a.OF[b];
     a.DESC[b] = make_int4(first, count, (unsigned)p < (unsigned)a.prefixes && a.far_rows(p) > 0, 0);
@@ -107,7 +92,6 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a,
   constexpr int QT = 32 * RG;
   __shared__ __align__(256) uint8_t ring0[C::STAGE];
   __shared__ __align__(256) uint8_t ring1[C::STAGE];
-  __shared__ __align__(256) uint8_t ring2[C::ST > 2 ? C::STAGE : 16];
   __shared__ int seq_s[QT + 2], wcnt[TA_WAVES];
   __shared__ __align__(16) unsigned long long run_s[PF_CHUNK / 16][2];
 
@@ -119,12 +103,10 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a,
       describe<FORM>(a, tid);
       return;
     }
-    // the sequences' own rows: neighbouring heads of one chunk side by side, four waves each
-    __shared__ AttnLds<D> sh[2];
-    const int half = __builtin_amdgcn_readfirstlane(tid >> 8), wide = a.c.nkv * ((group + PG_HEADS - 1) / PG_HEADS);
-    const int pairs = (wide + 1) / 2, part = 2 * ((i - 1) % pairs) + half;
-    static_assert(2 * PG_T == TA_T && PG_WAVES * AttnLds<D>::REGION <= C::STAGE, "two halves, a stage of the ring each");
-    attend_chunk<DT, D, FORM>(a, (i - 1) / pairs, part, tid & (PG_T - 1), half ? ring1 : ring0, sh[half]);
+    __shared__ AttnLds<D> sh;  // the sequences' own rows
+    const int wide = a.c.nkv * ((group + PG_HEADS - 1) / PG_HEADS);
+    static_assert(PG_T == TA_T && PG_WAVES * AttnLds<D>::REGION <= C::STAGE, "the same waves, and their V rows in a stage");
+    attend_chunk<DT, D, FORM>(a, (i - 1) / wide, (i - 1) % wide, tid, ring0, sh);
     return;
   }
   const Item it = find_item(a, gx, tid);
@@ -219,20 +201,24 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a,
   };
   bool seen = false;
   auto compute = [&](int t, uint8_t* ring) {
-#pragma unroll
-    for (int b = 0; b < C::SB; ++b) {
-      const int row = 32 * (C::SB * kg + b), r0 = t * C::KEYS + row;
-      if (r0 >= n) continue;
-      const bool h0 = hole_at(r0), h1 = hole_at(r0 + 16);
-      seen = seen || !h0 || (!h1 && r0 + 16 < n);
-      w.run(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, r0 + 32 > n || h0 || h1,
-            [&](int i) { return r0 + i >= n || (i < 16 ? h0 : h1); });
-    }
+    const int row = 32 * C::SB * kg, r0 = t * C::KEYS + row;
+    if (r0 >= n) return;
+    uint32_t gone = 0;  // the holes among its runs of 16 rows
+    if (holes)
+      for (int i = 0; i < 2 * C::SB; ++i) {
+        const bool hole = hole_at(r0 + 16 * i);
+        gone |= hole << i;
+        seen = seen || (!hole && r0 + 16 * i < n);
+      }
+    else
+      seen = true;
+    w.template run<C::SB>(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, gone || r0 + 32 * C::SB > n,
+                          [&](int i) { return r0 + i >= n || (gone >> (i / 16) & 1); });
   };
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(w.q[i]));  // (waited for here, not among the loop's loads)
-  ta_tiles<C>((n + C::KEYS - 1) / C::KEYS, ring0, ring1, ring2, load, landed, compute);
-  ta_join<C>(w, seen, ring0, ring1, ring2, rg, kg, lane);
+  ta_tiles<C>((n + C::KEYS - 1) / C::KEYS, ring0, ring1, load, landed, compute);
+  ta_join<C>(w, seen, ring0, ring1, rg, kg, lane);
 
   if (kg == 0 && myrow < rows) {
     const size_t at = a.far_base + ((size_t)gx * a.c.nkv + h) * QT + myrow;
@@ -258,7 +244,7 @@ struct PrefixPlan {
 };
 inline bool prefix_plan(int seqs, int nh, int nkv, int prefixes, long long far_cap, PrefixPlan* p) {
   const long long group = nh / nkv, rows = seqs * group;
-  p->tile = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  p->tile = rows <= 64 ? 64 : 128;
   p->target = nkv < PF_WGS ? PF_WGS / nkv : 1;
   // each prefix that a sequence has may end with a tile that is not full
   const long long tiles = rows / p->tile + (prefixes < seqs ? prefixes : seqs);
@@ -288,8 +274,8 @@ static bool prefix_work(int seqs, int nh, int nkv, int hd, long long cap, long l
                         bool tracked, PrefixWork* w) {
   if (!attn_plan(seqs, nh, nkv, hd, cap, rows, tracked, true, &w->own) ||
       !prefix_plan(seqs, nh, nkv, prefixes, far_cap, &w->far) ||
-      (long long)w->far.items * nkv + 1 + (long long)w->own.chunks * nkv * w->own.hgs > PG_MAX_GRID / 2)
-    return false;  // (workgroups of 512 threads)
+      (long long)w->far.items * nkv + 1 + (long long)w->own.chunks * nkv * w->own.hgs > PG_MAX_GRID)
+    return false;
   w->rows = (size_t)w->own.chunks * nh + w->far.rows;
   w->desc = (w->rows * (2 + hd) + 3) / 4 * 4;
   w->scores = w->desc + (size_t)seqs * 8;
@@ -315,13 +301,12 @@ extern "C" int ttsp_paged_attention_prefix_work_kib(int seqs, int nh, int nkv, i
 template <int FORM>
 static int prefix_launch(const AttnArgs& a, const PrefixWork& w, int hd, int dtype, hipStream_t stream) {
   const int items = w.far.items * a.c.nkv;
-  const dim3 grid((unsigned)(items + 1 + w.own.chunks * ((a.c.nkv * w.own.hgs + 1) / 2)));
+  const dim3 grid((unsigned)(items + 1 + w.own.chunks * a.c.nkv * w.own.hgs));
   const int gathers = w.own.chunks * a.c.nkv;
 #define TTSP_PFX(DTV, DV)                                                                                              \
   do {                                                                                                                 \
     if (w.far.tile == 64) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 2, FORM>), grid, dim3(TA_T), 0, stream, a, items);         \
-    else if (w.far.tile == 128) hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4, FORM>), grid, dim3(TA_T), 0, stream, a, items);   \
-    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 8, FORM>), grid, dim3(TA_T), 0, stream, a, items);                          \
+    else hipLaunchKernelGGL((paged_prefix_kernel<DTV, DV, 4, FORM>), grid, dim3(TA_T), 0, stream, a, items);            \
     if (FORM & PG_TRACK)                                                                                               \
       hipLaunchKernelGGL((paged_gather_kernel<DTV, DV, FORM>), dim3(gathers + a.seqs * a.nh), dim3(256), 0, stream, a,  \
                          gathers);                                                                                     \

@@ -2,19 +2,18 @@
 // such rows: sequences that share a prefix (paged_prefix.hip) and a prompt's rows
 // through a window (prefill_window.hip).
 //
-// A workgroup of eight waves takes 32 RG query rows of one kv head. Its keys come in
-// tiles through a ring in LDS, straight from memory (buffer loads to LDS, so that no
-// register holds what is on its way): RG waves take 32 rows each of the same 32 keys,
-// and 8 / RG such groups of waves every (8 / RG)-th run of 32 keys; the groups' sums
-// join in LDS at the end. The fewer the rows, the more keys are under way.
+// A workgroup of four waves takes 32 RG query rows of one kv head. Its keys come in
+// tiles of 64 through a ring of two in LDS, straight from memory (buffer loads to LDS,
+// so that no register holds what is on its way): RG waves take 32 rows each of the same
+// keys, and with two row groups (RG 2) the other two waves take the other half of a
+// tile's keys and join their sums through LDS at the end. Two workgroups fit a CU.
 //
 // A wave's 32 keys: S^T = K Q^T on the matrix cores (Q stays in registers), so that a
 // lane holds 16 keys of one query row; the exponentials subtract a reference that
 // moves only when a score outgrows it (pg_above), so the running maximum needs no
 // exchange between lanes but a vote; P^T goes back to the matrix cores from the
 // registers it is in, in PARTS of the cache's type: O^T += V^T P^T, V^T through the
-// transposing LDS read. Two waves a SIMD: one's exponentials run beside the other's
-// products.
+// transposing LDS read.
 //
 // K and V rows lie in LDS as in memory, their 16-byte pieces swizzled by row (ta_swz):
 // sixteen rows' same piece lies in sixteen different bank groups (K's reads), and the
@@ -31,13 +30,13 @@ namespace ttsp {
 
 typedef __attribute__((address_space(3))) void* ta_lds_ptr;
 
-constexpr int TA_WAVES = 8, TA_T = 64 * TA_WAVES;
+constexpr int TA_WAVES = 4, TA_T = 64 * TA_WAVES;
 
 template <int D, int RG>
 struct Tile {
-  static constexpr int KG = TA_WAVES / RG, SB = RG == 8 ? 2 : 1;  // key groups; runs of 32 keys a wave takes of a tile
-  static constexpr int KEYS = 32 * KG * SB, ROWB = D * 2, PPR = ROWB / 16;
-  static constexpr int HALF = KEYS * ROWB, STAGE = 2 * HALF, ST = RG == 2 ? 2 : 3;  // K, then V; stages of the ring
+  static constexpr int KG = TA_WAVES / RG, SB = 2 / KG;  // key groups; runs of 32 keys a wave takes of a tile
+  static constexpr int KEYS = 64, ROWB = D * 2, PPR = ROWB / 16;
+  static constexpr int HALF = KEYS * ROWB, STAGE = 2 * HALF;  // K, then V
   static constexpr int RPI = 1024 / ROWB, PER = KEYS / RPI / TA_WAVES;  // rows a load covers, loads of K (and of V) a wave
 };
 
@@ -89,35 +88,47 @@ struct TaWave {
     vb = row * (D * 2) + ((piece ^ ta_swz<D>(row)) << 4) + (li & 1) * 8;
   }
 
-  // 32 keys: K and V rows at k and v. masked (uniform): key j of the run is none where gone(j).
-  template <typename F>
+  // 32 NB keys, K and V rows at k and v. masked (uniform): key j of them is none where gone(j).
+  // (64 at once: the second's products run beside the first's exponentials.)
+  template <int NB, typename F>
   __device__ __forceinline__ void run(const uint8_t* k, const uint8_t* v, float scale2, bool masked, F gone) {
-    f32x16_v s;
+    f32x16_v s[NB];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) s = mfma32<DT>(*reinterpret_cast<const u32x4*>(k + (kb ^ (i << 5))), q[i], s);
+      for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        s[b] = mfma32<DT>(*reinterpret_cast<const u32x4*>(k + b * 32 * D * 2 + (kb ^ (i << 5))), q[i], s[b]);
+    }
     if (masked) {
       const int h4 = (threadIdx.x & 63) >> 5 << 2;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (gone(8 * (r / 4) + h4 + r % 4)) s[r] = -__builtin_inff();
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (gone(32 * b + 8 * (r / 4) + h4 + r % 4)) s[b][r] = -__builtin_inff();
     }
     // The weights with the reference as it is, and only where they come out too large
     // (sixteen of 2^8 and less sum up to no more than 4096) the maximum, a new reference and the
     // weights again. fp16 weights have no room for that: their maximum is looked at first.
-    float p[16], sum = 0.0f;
+    f32x16_v p[NB];
+    float sum[NB];
     auto weigh = [&]() {
-      sum = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -m));
+      for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += p[r];
+        for (int r = 0; r < 16; ++r) p[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], scale2, -m));
+        sum[b] = ((p[b][0] + p[b][1]) + (p[b][2] + p[b][3])) + ((p[b][4] + p[b][5]) + (p[b][6] + p[b][7])) +
+                 (((p[b][8] + p[b][9]) + (p[b][10] + p[b][11])) + ((p[b][12] + p[b][13]) + (p[b][14] + p[b][15])));
+      }
     };
     auto largest = [&]() {
-      float bm = s[0];
+      float bm = s[0][0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[b][r]);
       return bm * scale2;
     };
     auto move = [&](float bm) {
@@ -137,69 +148,63 @@ struct TaWave {
       weigh();
     } else {
       weigh();
-      if (__any(!(sum <= 4096.0f))) {
+      bool most = true;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) most = most && sum[b] <= 4096.0f;
+      if (__any(!most)) {
         move(largest());
         weigh();
       }
     }
-    l += sum;
-    u32x4 pf[2][PARTS];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int b = 0; b < NB; ++b) l += sum[b];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        uint32_t parts[PARTS];
-        ta_split<DT, PARTS>(p[8 * c + 2 * u], p[8 * c + 2 * u + 1], parts);
+    for (int b = 0; b < NB; ++b) {
+      u32x4 pf[2][PARTS];
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) pf[c][i][u] = parts[i];
-      }
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+        for (int u = 0; u < 4; ++u) {
+          uint32_t parts[PARTS];
+          ta_split<DT, PARTS>(p[b][8 * c + 2 * u], p[b][8 * c + 2 * u + 1], parts);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint2 lo = pg_ld_tr(v + 16 * c * (D * 2) + (vb ^ (d << 6)));
-        const uint2 hi = pg_ld_tr(v + (16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32));
-        const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
+          for (int i = 0; i < PARTS; ++i) pf[c][i][u] = parts[i];
+        }
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) o[d] = mfma32<DT>(vt, pf[c][i], o[d]);
-      }
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          const uint2 lo = pg_ld_tr(v + (32 * b + 16 * c) * (D * 2) + (vb ^ (d << 6)));
+          const uint2 hi = pg_ld_tr(v + (32 * b + 16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32));
+          const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) o[d] = mfma32<DT>(vt, pf[c][i], o[d]);
+        }
+    }
   }
 };
 
-// n tiles through the ring: load(t, ring) issues this wave's 2 PER loads of tile t (any
+// n tiles through a ring of two: load(t, ring) issues this wave's 2 PER loads of tile t (any
 // t: past the last it may load what it likes), landed(t, ring) may touch up the rows
 // that this wave loaded, compute(t, ring) reads tile t.
 template <typename C, typename F, typename G, typename H>
-__device__ __forceinline__ void ta_tiles(int n, uint8_t* ring0, uint8_t* ring1, uint8_t* ring2, F load, G landed, H compute) {
-  constexpr int L = 2 * C::PER;
+__device__ __forceinline__ void ta_tiles(int n, uint8_t* ring0, uint8_t* ring1, F load, G landed, H compute) {
   if (n <= 0) return;
   load(0, ring0);
-  if constexpr (C::ST > 2) load(1, ring1);
-  // step t: tile t has landed and every wave is past tile t - 1, whose place tile t + ST - 1 takes
+  // step t: tile t has landed and every wave is past tile t - 1, whose place tile t + 1 takes
   auto one = [&](int t, uint8_t* rd, uint8_t* dst) {
-    TTSP_WAIT_VM_LGKM0((C::ST - 2) * L);
+    TTSP_WAIT_VM_LGKM0(0);
     landed(t, rd);
     TTSP_WAIT_LGKM0();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    load(t + C::ST - 1, dst);
+    load(t + 1, dst);
     compute(t, rd);
   };
-  int t = 0;
-  if constexpr (C::ST == 2) {
-    for (; t + 2 <= n; t += 2) {
-      one(t, ring0, ring1);
-      one(t + 1, ring1, ring0);
-    }
-    if (t < n) one(t, ring0, ring1);
-  } else {
-    for (; t + 3 <= n; t += 3) {
-      one(t, ring0, ring2);
-      one(t + 1, ring1, ring0);
-      one(t + 2, ring2, ring1);
-    }
-    if (t < n) one(t, ring0, ring2);
+#pragma unroll 1
+  for (int t = 0; t < n; t += 2) {
+    one(t, ring0, ring1);
     if (t + 1 < n) one(t + 1, ring1, ring0);
   }
   TTSP_WAIT_VM_LGKM0(0);
@@ -209,28 +214,21 @@ __device__ __forceinline__ void ta_tiles(int n, uint8_t* ring0, uint8_t* ring1, 
 // The key groups' sums joined into the first group's waves (the ring is free). seen:
 // whether the wave has had a key; the first group's get the groups'.
 template <typename C, int DT, int D, int PARTS>
-__device__ __forceinline__ void ta_join(TaWave<DT, D, PARTS>& w, bool& seen, uint8_t* ring0, uint8_t* ring1, uint8_t* ring2, int rg,
-                                        int kg, int lane) {
-  constexpr int RG = TA_WAVES / C::KG;
+__device__ __forceinline__ void ta_join(TaWave<DT, D, PARTS>& w, bool& seen, uint8_t* ring0, uint8_t* ring1, int rg, int kg, int lane) {
   w.l += __shfl_xor(w.l, 32, 64);
-#pragma unroll
-  for (int st = C::KG / 2; st >= 1; st /= 2) {
-    const bool give = kg >= st && kg < 2 * st, take = kg < st;
-    const int slot = (give ? kg - st : kg) * RG + rg;
-    auto part = [&](int d) {  // 4 KB of the slot's O
-      const int at = (slot * (D / 32) + d) * 4096;
-      return reinterpret_cast<float*>(at < C::STAGE ? ring0 + at : ring1 + (at - C::STAGE)) + lane;
-    };
-    float* const ml = reinterpret_cast<float*>(C::ST > 2 ? ring2 : ring1) + slot * 192 + lane;
-    if (give) {
+  if constexpr (C::KG == 2) {
+    static_assert((TA_WAVES / 2) * (D / 32) * 4096 <= C::STAGE, "the givers' O in a stage");
+    float* const part = reinterpret_cast<float*>(ring0) + rg * (D / 32) * 1024 + lane;
+    float* const ml = reinterpret_cast<float*>(ring1) + rg * 192 + lane;
+    if (kg) {
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) part(d)[64 * r] = w.o[d][r];
+        for (int r = 0; r < 16; ++r) part[(16 * d + r) * 64] = w.o[d][r];
       ml[0] = w.m, ml[64] = w.l, ml[128] = seen ? 1.0f : 0.0f;
     }
     __syncthreads();
-    if (take) {
+    if (!kg) {
       const float m2 = ml[0], mm = fmaxf(w.m, m2);
       const float f1 = __builtin_amdgcn_exp2f(w.m - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
       w.l = w.l * f1 + ml[64] * f2;
@@ -239,9 +237,8 @@ __device__ __forceinline__ void ta_join(TaWave<DT, D, PARTS>& w, bool& seen, uin
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) w.o[d][r] = w.o[d][r] * f1 + part(d)[64 * r] * f2;
+        for (int r = 0; r < 16; ++r) w.o[d][r] = w.o[d][r] * f1 + part[(16 * d + r) * 64] * f2;
     }
-    __syncthreads();
   }
 }
 
