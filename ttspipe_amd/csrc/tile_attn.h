@@ -88,98 +88,112 @@ struct TaWave {
     vb = row * (D * 2) + ((piece ^ ta_swz<D>(row)) << 4) + (li & 1) * 8;
   }
 
+  // K's rows of 32 keys in the operand's layout
+  __device__ __forceinline__ void keys(const uint8_t* k, u32x4 (&kf)[D / 16]) const {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) kf[i] = *reinterpret_cast<const u32x4*>(k + (kb ^ (i << 5)));
+  }
+  __device__ __forceinline__ f32x16_v score(const u32x4 (&kf)[D / 16]) const {
+    f32x16_v s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma32<DT>(kf[i], q[i], s);
+    return s;
+  }
+  // Weights by the reference as it is; their sum.
+  __device__ __forceinline__ float weigh(const f32x16_v& s, float scale2, f32x16_v& p) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -m));
+    return (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+           (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+  }
+  // The reference above the scores: fp16 weights have no room for larger ones, so their
+  // maximum is looked at first; bf16 ones are weighed as the reference is, and only
+  // where they come out too large (sixteen of 2^8 and less sum up to no more than
+  // 4096) it moves, and they are weighed again.
+  __device__ __forceinline__ void move(const f32x16_v& s, float scale2) {
+    float bm = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+    bm *= scale2;
+    if (DT == DT_F16 && !__any(bm > m + pg_above<DT>)) return;
+    bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+    const float mnew = bm > m + pg_above<DT> ? bm - pg_below<DT> : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+    m = mnew;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+  }
+  // V^T of 16 keys at v, and O^T += V^T P^T of them
+  __device__ __forceinline__ void values(const uint8_t* v, u32x4 (&vt)[D / 32]) const {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const uint2 lo = pg_ld_tr(v + (vb ^ (d << 6))), hi = pg_ld_tr(v + 8 * (D * 2) + (vb ^ (d << 6) ^ 32));
+      vt[d] = u32x4{lo.x, lo.y, hi.x, hi.y};
+    }
+  }
+  __device__ __forceinline__ void split(const f32x16_v& p, int c, u32x4 (&pf)[PARTS]) const {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t parts[PARTS];
+      ta_split<DT, PARTS>(p[8 * c + 2 * u], p[8 * c + 2 * u + 1], parts);
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) pf[i][u] = parts[i];
+    }
+  }
+  __device__ __forceinline__ void add(const u32x4 (&vt)[D / 32], const u32x4 (&pf)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) o[d] = mfma32<DT>(vt[d], pf[i], o[d]);
+  }
+
   // 32 NB keys, K and V rows at k and v. masked (uniform): key j of them is none where gone(j).
-  // (64 at once: the second's products run beside the first's exponentials.)
   template <int NB, typename F>
   __device__ __forceinline__ void run(const uint8_t* k, const uint8_t* v, float scale2, bool masked, F gone) {
-    f32x16_v s[NB];
+    constexpr int RB = 32 * D * 2;  // bytes of 32 rows
+    const int h4 = (threadIdx.x & 63) >> 5 << 2;
+    auto mask = [&](int b, f32x16_v& s) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (gone(32 * b + 8 * (r / 4) + h4 + r % 4)) s[r] = -__builtin_inff();
+    };
+    u32x4 kf[NB][D / 16];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) keys(k + b * RB, kf[b]);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16_v s[NB], p;
+    s[0] = score(kf[0]);
+    if (masked) mask(0, s[0]);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        s[b] = mfma32<DT>(*reinterpret_cast<const u32x4*>(k + b * 32 * D * 2 + (kb ^ (i << 5))), q[i], s[b]);
-    }
-    if (masked) {
-      const int h4 = (threadIdx.x & 63) >> 5 << 2;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (gone(32 * b + 8 * (r / 4) + h4 + r % 4)) s[b][r] = -__builtin_inff();
-    }
-    // The weights with the reference as it is, and only where they come out too large
-    // (sixteen of 2^8 and less sum up to no more than 4096) the maximum, a new reference and the
-    // weights again. fp16 weights have no room for that: their maximum is looked at first.
-    f32x16_v p[NB];
-    float sum[NB];
-    auto weigh = [&]() {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], scale2, -m));
-        sum[b] = ((p[b][0] + p[b][1]) + (p[b][2] + p[b][3])) + ((p[b][4] + p[b][5]) + (p[b][6] + p[b][7])) +
-                 (((p[b][8] + p[b][9]) + (p[b][10] + p[b][11])) + ((p[b][12] + p[b][13]) + (p[b][14] + p[b][15])));
-      }
-    };
-    auto largest = [&]() {
-      float bm = s[0][0];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[b][r]);
-      return bm * scale2;
-    };
-    auto move = [&](float bm) {
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mnew = bm > m + pg_above<DT> ? bm - pg_below<DT> : m;
-      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-      m = mnew;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-    };
-    if constexpr (DT == DT_F16) {
-      const float bm = largest();
-      if (__any(bm > m + pg_above<DT>)) move(bm);
-      weigh();
-    } else {
-      weigh();
-      bool most = true;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) most = most && sum[b] <= 4096.0f;
-      if (__any(!most)) {
-        move(largest());
-        weigh();
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) l += sum[b];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      u32x4 pf[2][PARTS];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t parts[PARTS];
-          ta_split<DT, PARTS>(p[b][8 * c + 2 * u], p[b][8 * c + 2 * u + 1], parts);
-#pragma unroll
-          for (int i = 0; i < PARTS; ++i) pf[c][i][u] = parts[i];
+      // the weights of run b beside the scores of run b + 1 or the products of run b - 1
+      if constexpr (DT == DT_F16) move(s[b], scale2);
+      if (b + 1 < NB) s[b + 1] = score(kf[b + 1]);
+      float sum = weigh(s[b], scale2, p);
+      if (b + 1 < NB)
+        for (int i = 0; i < D / 16; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
         }
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          const uint2 lo = pg_ld_tr(v + (32 * b + 16 * c) * (D * 2) + (vb ^ (d << 6)));
-          const uint2 hi = pg_ld_tr(v + (32 * b + 16 * c + 8) * (D * 2) + (vb ^ (d << 6) ^ 32));
-          const u32x4 vt = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-          for (int i = 0; i < PARTS; ++i) o[d] = mfma32<DT>(vt, pf[c][i], o[d]);
+      if (b + 1 < NB && masked) mask(b + 1, s[b + 1]);
+      if constexpr (DT != DT_F16)
+        if (__any(!(sum <= 4096.0f))) {
+          move(s[b], scale2);
+          sum = weigh(s[b], scale2, p);
         }
+      l += sum;
+      u32x4 vt[2][D / 32], pf[2][PARTS];
+      values(v + b * RB, vt[0]);
+      values(v + b * RB + RB / 2, vt[1]);
+      split(p, 0, pf[0]);
+      add(vt[0], pf[0]);
+      split(p, 1, pf[1]);
+      add(vt[1], pf[1]);
     }
   }
 };
