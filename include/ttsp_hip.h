@@ -557,7 +557,7 @@ int ttsp_prefill_attention_window(const void* Q, long long q_seq_stride, long lo
 
 /* Key splits that ttsp_prefill_attention_window's workspace is for (host-only), as
  * ttsp_prefill_attention_splits. */
-int ttsp_prefill_attention_window_splits(int S, int nkv, int L, int window, int sinks);
+int ttsp_prefill_attention_window_splits(int S, int nh, int nkv, int L, int window, int sinks);
 
 /* out[d] = round(sum_{c < ntok} E[(c*vocab + tok[c]) * D + d]) (tok int32 on the
  * device, clamped into [0, vocab)). Replaces: the codebook-embedding lookup of

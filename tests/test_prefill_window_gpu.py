@@ -142,7 +142,7 @@ def test_infinities_and_nan_behind_the_window_are_not_seen():
 
 def test_strides_workspaces_and_out():
     q, k, v, pos = make(40, 3000, 32, 8, BF, seed=10, pad=72)
-    splits = fastpath.prefill_splits(40, 8, 3000, 2500, 4)
+    splits = fastpath.prefill_splits(40, 32, 8, 3000, 2500, 4)
     need = fastpath.prefill_work_floats(40, 32, splits)
     work, out = torch.full((max(need, 4),), math.nan, device="cuda"), torch.empty(1, 40, 4096, dtype=BF, device="cuda")
     y = run(q, k, v, pos, 2500, 4, out=out, work=work)
@@ -173,7 +173,7 @@ def test_refusals():
 def test_a_captured_call_follows_the_positions():
     q, k, v, pos = make(64, 1500, 8, 2, BF, seed=12)
     out = torch.empty(1, 64, 1024, dtype=BF, device="cuda")
-    splits = fastpath.prefill_splits(64, 2, 1500, 500, 4)
+    splits = fastpath.prefill_splits(64, 8, 2, 1500, 500, 4)
     work = torch.empty(max(4, fastpath.prefill_work_floats(64, 8, splits)), device="cuda")
     step = lambda: fastpath.prefill_attention(q, k, v, None, 8, 2, 128, positions=pos, window=500, sinks=4, out=out, work=work)  # noqa: E731
     step()

@@ -137,7 +137,7 @@ SIGNATURES: dict[str, list] = {
                                       _vp, _i, _vp],
     "ttsp_prefill_attention_window": [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _f,
                                       _i, _vp, _i, _vp],
-    "ttsp_prefill_attention_window_splits": [_i, _i, _i, _i, _i],
+    "ttsp_prefill_attention_window_splits": [_i, _i, _i, _i, _i, _i],
     "ttsp_sample_topk": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "ttsp_sample_max_top_k": [],
     "ttsp_sample_max_vocab": [],

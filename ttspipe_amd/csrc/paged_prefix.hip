@@ -14,7 +14,7 @@
 namespace ttsp {
 
 constexpr int PF_MAX = 256;   // prefixes of a call (one a thread)
-constexpr int PF_WGS = 256;   // workgroups the chunks are meant to make, two a CU
+constexpr int PF_WGS = 256;   // workgroups the chunks are meant to make
 constexpr int PF_PARTS = 2;
 
 // Item gx of the call: a chunk of a prefix and a tile of its query rows.

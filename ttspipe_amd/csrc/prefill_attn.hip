@@ -34,6 +34,7 @@
 // operands agree on is fine); accumulator r of lane l is
 // D[8*(r/4) + 4*(l/32) + r%4][l % 32].
 #include "attn_common.h"
+#include "prefill_window.h"
 
 namespace ttsp {
 
@@ -695,10 +696,14 @@ static int prefill_launch(const void* Q, long long q_seq_stride, long long q_hea
                 q_seq_stride, q_head_stride, (int)k_seq_stride, (int)k_head_stride, (int)v_seq_stride,
                 (int)v_head_stride, (int)mask_row_stride, S, nh, nkv, L, scale * PA_LOG2E,
                 splits > 1 ? work : nullptr, pos, window < L ? window : L, sinks < L ? sinks : L};
+  const int wide = window > 0 && splits == 1 ? prompt_window_tiles(S, nh, nkv) : 0;
   const int groups = nh / nkv;
   const dim3 grid(nkv, (S + PA_QB - 1) / PA_QB, splits);
   int rc;
-  if (window > 0 && dtype == DT_F16)
+  if (wide && (dtype == DT_F16 || dtype == DT_BF16))
+    rc = prompt_window_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride, v_head_stride,
+                              pos, Y, S, nh, nkv, L, a.window, a.sinks, scale, dtype, wide, stream);
+  else if (window > 0 && dtype == DT_F16)
     rc = prefill_dispatch<DT_F16, true, true>(groups, grid, splits, a, stream);
   else if (window > 0 && dtype == DT_BF16)
     rc = prefill_dispatch<DT_BF16, true, true>(groups, grid, splits, a, stream);
@@ -778,8 +783,9 @@ static int window_keys(int S, int L, int window, int sinks) {
   return n < L ? (int)n : L;
 }
 
-extern "C" int ttsp_prefill_attention_window_splits(int S, int nkv, int L, int window, int sinks) {
-  if (S <= 0 || nkv <= 0 || L <= 0 || window <= 0 || sinks < 0) return 1;
+extern "C" int ttsp_prefill_attention_window_splits(int S, int nh, int nkv, int L, int window, int sinks) {
+  if (S <= 0 || nkv <= 0 || nh < nkv || L <= 0 || window <= 0 || sinks < 0) return 1;
+  if (prompt_window_tiles(S, nh, nkv)) return 1;
   return prefill_splits(S, nkv, window_keys(S, L, window, sinks));
 }
 

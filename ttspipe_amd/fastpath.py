@@ -102,7 +102,7 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     lib = _lib.lib()
     if window is not None:
         window, sinks = min(int(window), L), min(int(sinks), L)
-    splits = prefill_splits(seqlen, n_local_heads, L, window, sinks)
+    splits = prefill_splits(seqlen, n_head, n_local_heads, L, window, sinks)
     need = prefill_work_floats(seqlen, n_head, splits)
     if splits > 1 and work is None:
         work = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -219,13 +219,13 @@ def causal_rows_attention_qkv(qkv, q_weight, k_weight, eps, freqs_cis, input_pos
     return y
 
 
-def prefill_splits(seqlen: int, n_local_heads: int, width: int, window: int | None = None, sinks: int = 0) -> int:
+def prefill_splits(seqlen: int, n_head: int, n_local_heads: int, width: int, window: int | None = None, sinks: int = 0) -> int:
     """Key splits of `prefill_attention` over `width` keys (its workspace: `prefill_work_floats`)."""
     from ttspipe_amd import _lib
 
     if window is None:
         return _lib.lib().ttsp_prefill_attention_splits(seqlen, n_local_heads, width)
-    return _lib.lib().ttsp_prefill_attention_window_splits(seqlen, n_local_heads, width, min(window, width),
+    return _lib.lib().ttsp_prefill_attention_window_splits(seqlen, n_head, n_local_heads, width, min(window, width),
                                                            min(sinks, width))
 
 
