@@ -212,8 +212,8 @@ __global__ __launch_bounds__(TA_T, 2) void paged_prefix_kernel(const AttnArgs a,
       }
     else
       seen = true;
-    w.template run<C::SB>(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, gone || r0 + 32 * C::SB > n,
-                          [&](int i) { return r0 + i >= n || (gone >> (i / 16) & 1); });
+    w.template run<C::SB>(ring + row * C::ROWB, ring + C::HALF + row * C::ROWB, scale2, gone || r0 + 32 * C::SB > n, n - 1 - r0, 0,
+                          0, gone);
   };
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" ::"v"(w.q[i]));  // (waited for here, not among the loop's loads)

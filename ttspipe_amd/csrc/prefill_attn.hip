@@ -34,7 +34,7 @@
 // operands agree on is fine); accumulator r of lane l is
 // D[8*(r/4) + 4*(l/32) + r%4][l % 32].
 #include "attn_common.h"
-#include "prefill_window.h"
+#include "prefill_merge.h"
 
 namespace ttsp {
 
@@ -131,7 +131,6 @@ struct PrefillArgs {
   float scale2;  // scale * log2(e): scores in log2 units
   float* WO;     // SPLIT: unnormalised O [z][i][head][128], then m, l [z][i][head]
   const long long* POS;  // CAUSAL: the S query rows' positions (M unused)
-  int window, sinks;     // WINDOW: at least 1 and 0, at most L
 };
 
 // LDS of one staged key block: K rows, V rows, mask tile (bytes)
@@ -150,13 +149,10 @@ constexpr int PA_BLK = PA_KT + PA_VT + PA_MT;
 // (and the first key some row may not see) from its own 32 position loads.
 // The same keys are masked and the same blocks flagged whole as with the
 // causal mask's bytes, so the results are those bits.
-// WINDOW (CAUSAL): a row at position p does not see keys from `sinks` to
-// p - window. The blocks that no row of the workgroup sees are left out: block b
-// is the b-th of those that hold a sink or a key of some row's window.
 // GW: the query heads a workgroup takes, of the G that share a kv head
 // (G / GW workgroups a kv head and query block, each staging the kv head's
 // keys for its own heads).
-template <int DT, int G, int NS, bool SPLIT, bool CAUSAL = false, int GW = G, bool WINDOW = false>
+template <int DT, int G, int NS, bool SPLIT, bool CAUSAL = false, int GW = G>
 __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const PrefillArgs a) {
   static_assert(G % GW == 0, "a kv head's query heads split evenly over its workgroups");
   static_assert((NS & (NS - 1)) == 0, "the key splits merge in halving rounds");
@@ -184,10 +180,6 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   const int L = a.L;
   const int z = blockIdx.z;
   int kb0 = 0;  // first key of this workgroup's run (SPLIT: set after the mask scan)
-  // WINDOW: blocks of sinks, and the blocks left out behind them (keys)
-  const int sink_keys = WINDOW ? (a.sinks + PA_KB - 1) / PA_KB * PA_KB : 0;
-  int gap = 0;
-  auto key_at = [&](int j) { return WINDOW && j >= sink_keys ? j + gap : j; };
   const __amdgpu_buffer_rsrc_t kr = pa_rsrc(a.K + (size_t)kh * a.k_sh, (uint32_t)((L - 1) * a.k_ss + HD) * 2);
   const __amdgpu_buffer_rsrc_t vr = pa_rsrc(a.V + (size_t)kh * a.v_sh, (uint32_t)((L - 1) * a.v_ss + HD) * 2);
   // the mask buffer ends with the 16-byte piece holding the last row's byte
@@ -229,13 +221,13 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
 #pragma unroll
     for (int n = 0; n < KPT; ++n) {
       const int p = min(tid + n * NT, NKP - 1), blk = p / (PA_KB * (HD / 8)), q = p % (PA_KB * (HD / 8));
-      const int j = min(key_at(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8)), L - 1), e = (q % (HD / 8)) * 8;
+      const int j = min(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8), L - 1), e = (q % (HD / 8)) * 8;
       r.k[n] = pa_ld16(kr, (uint32_t)(j * a.k_ss + e) * 2);
     }
 #pragma unroll
     for (int n = 0; n < VPT; ++n) {
       const int p = min(tid + n * NT, NVP - 1), blk = p / (PA_KB * (HD / 8)), q = p % (PA_KB * (HD / 8));
-      const int j = min(key_at(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8)), L - 1), e = (q % (HD / 8)) * 8;
+      const int j = min(kb0 + NS * t * PA_KB + blk * PA_KB + q / (HD / 8), L - 1), e = (q % (HD / 8)) * 8;
       r.v[n] = pa_ld16(vr, (uint32_t)(j * a.v_ss + e) * 2);
     }
     if constexpr (!CAUSAL) {
@@ -278,7 +270,7 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       }
     }
   };
-  if constexpr (!SPLIT && !WINDOW) {
+  if constexpr (!SPLIT) {
     load(rs[0], 0);
     __builtin_amdgcn_sched_barrier(0);
     load(rs[1], 1);
@@ -293,20 +285,6 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   // key over the workgroup's rows, below which every block is whole
   const int klast = CAUSAL ? (int)max(min(pos_i, (long long)L - 1), -1LL) : 0;
   int kwhole = 0;
-  // WINDOW: the first key of this lane's row's window, and the highest such key
-  // over the workgroup's rows, from which on no block is cut by one
-  const int klow = WINDOW ? (int)min(max(pos_i - a.window + 1, 0LL), (long long)L) : 0;
-  int low = 0;
-  if constexpr (WINDOW) {
-    int first = ql < nq ? klow : L;
-    low = ql < nq ? klow : 0;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      first = min(first, __shfl_xor(first, o, 64));
-      low = max(low, __shfl_xor(low, o, 64));
-    }
-    gap = max(first / PA_KB * PA_KB - sink_keys, 0);
-  }
   if constexpr (CAUSAL) {
     hit = klast;
     kwhole = ql < nq ? klast : L;
@@ -336,14 +314,12 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
   }
   // this workgroup's key blocks: all blocks holding keys 0 .. last, or split
   // z's run of them
-  const int live = max(last + PA_KB - gap, 0) / PA_KB;
+  const int live = (last + PA_KB) / PA_KB;
   int nkb = live;
   if constexpr (SPLIT) {
     const int bps = (live + (int)gridDim.z - 1) / (int)gridDim.z;
     kb0 = z * bps * PA_KB;
     nkb = max(0, min(live, (z + 1) * bps) - z * bps);
-  }
-  if constexpr (SPLIT || WINDOW) {
     load(rs[0], 0);
     __builtin_amdgcn_sched_barrier(0);
     load(rs[1], 1);
@@ -377,9 +353,7 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       // (CAUSAL: the group's blocks whole when its last key is below every row's
       // last key, as the causal mask's tiles are then all set)
       const int gend = kb0 + (NS * t + NS) * PA_KB - 1;
-      // (WINDOW: and none of them between the sinks and the last row's window)
-      const bool all = CAUSAL ? key_at(gend) <= kwhole && (!WINDOW || key_at(kb0 + NS * t * PA_KB) >= low || key_at(gend) < a.sinks)
-                              : __builtin_amdgcn_readfirstlane(full[t % 3]) != 0;
+      const bool all = CAUSAL ? gend <= kwhole : __builtin_amdgcn_readfirstlane(full[t % 3]) != 0;
       // S^T = K Q^T for keys 32 b .. 32 b + 31
       pa_f32x16 s;
 #pragma unroll
@@ -410,13 +384,12 @@ __global__ __launch_bounds__(64 * GW * NS) void prefill_attn_kernel(const Prefil
       // lane and lane ^ 32, in log2 units
       if (!all) {
         if constexpr (CAUSAL) {
-          const int k0 = key_at(kb0 + b * PA_KB) + 4 * h;  // key of s[0]
+          const int k0 = kb0 + b * PA_KB + 4 * h;  // key of s[0]
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (k0 + 8 * g + c > klast || (WINDOW && k0 + 8 * g + c >= a.sinks && k0 + 8 * g + c < klow))
-                s[4 * g + c] = -__builtin_inff();
+              if (k0 + 8 * g + c > klast) s[4 * g + c] = -__builtin_inff();
         } else {
           const uint8_t* mrow = ms + ql * PA_MROW + 4 * h;
 #pragma unroll
@@ -618,6 +591,29 @@ static int prefill_splits(int S, int nkv, int L) {
   return sp;
 }
 
+void prefill_merge(const float* work, int splits, int S, int nh, void* Y, int dtype, hipStream_t stream) {
+  const long long n = (long long)S * nh * (HD / 8);
+  const dim3 mg((unsigned)((n + 255) / 256));
+#define TTSP_PM(DTV, SPM) \
+  hipLaunchKernelGGL((prefill_merge_kernel<DTV, SPM>), mg, dim3(256), 0, stream, work, splits, S, nh, (uint16_t*)Y)
+#define TTSP_PM_SP(DTV)          \
+  if (splits <= 2)               \
+    TTSP_PM(DTV, 2);             \
+  else if (splits <= 4)          \
+    TTSP_PM(DTV, 4);             \
+  else if (splits <= 8)          \
+    TTSP_PM(DTV, 8);             \
+  else                           \
+    TTSP_PM(DTV, 16);
+  if (dtype == DT_F16) {
+    TTSP_PM_SP(DT_F16)
+  } else {
+    TTSP_PM_SP(DT_BF16)
+  }
+#undef TTSP_PM_SP
+#undef TTSP_PM
+}
+
 }  // namespace ttsp
 
 using namespace ttsp;
@@ -633,22 +629,22 @@ extern "C" int ttsp_prefill_max_groups() { return PA_MAX_GROUPS; }
 // half the serial key steps, for twice the key staging (512 causal rows,
 // 32 / 8 heads: 14.5 against 15.9 us; with fewer rows, or with key splits,
 // the staging costs more than it saves).
-template <int DT, bool CAUSAL, bool WINDOW = false>
+template <int DT, bool CAUSAL>
 static int prefill_dispatch(int groups, dim3 grid, int splits, const PrefillArgs& a, hipStream_t stream) {
   if constexpr (CAUSAL) {
     if (groups == 4 && splits == 1 && (long long)grid.x * grid.y >= 128) {
       grid.x *= 2;
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, 4, 4, false, true, 2, WINDOW>), grid, dim3(64 * 2 * 4), 0, stream, a);
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, 4, 4, false, true, 2>), grid, dim3(64 * 2 * 4), 0, stream, a);
       return 0;
     }
   }
 #define TTSP_PA_G(G)                                                                                         \
   case G:                                                                                                    \
     if (splits > 1)                                                                                          \
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), true, CAUSAL, G, WINDOW>), grid,                     \
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), true, CAUSAL>), grid,                     \
                          dim3(64 * G * PA_SPLITS(G)), 0, stream, a);                                         \
     else                                                                                                     \
-      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), false, CAUSAL, G, WINDOW>), grid,                    \
+      hipLaunchKernelGGL((prefill_attn_kernel<DT, G, PA_SPLITS(G), false, CAUSAL>), grid,                    \
                          dim3(64 * G * PA_SPLITS(G)), 0, stream, a);                                         \
     return 0;
   switch (groups) {
@@ -667,13 +663,12 @@ static int prefill_dispatch(int groups, dim3 grid, int splits, const PrefillArgs
 }
 
 // mask: bool rows (mask_row_stride bytes apart), or null with pos, the S
-// rows' positions, for the causal mask at those positions; window > 0: through a
-// window with sinks
+// rows' positions, for the causal mask at those positions
 static int prefill_launch(const void* Q, long long q_seq_stride, long long q_head_stride, const void* K,
                           long long k_seq_stride, long long k_head_stride, const void* V, long long v_seq_stride,
                           long long v_head_stride, const void* mask, long long mask_row_stride, const long long* pos,
                           void* Y, int S, int nh, int nkv, int L, float scale, int dtype, float* work, int splits,
-                          hipStream_t stream, int window = 0, int sinks = 0) {
+                          hipStream_t stream) {
   const bool causal = pos != nullptr;
   if (causal) mask = nullptr, mask_row_stride = 0;
   if (!Q || !K || !V || (!causal && !mask) || !Y || S <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || L <= 0 ||
@@ -695,19 +690,11 @@ static int prefill_launch(const void* Q, long long q_seq_stride, long long q_hea
   PrefillArgs a{(const uint16_t*)Q, (const uint16_t*)K, (const uint16_t*)V, (const uint8_t*)mask, (uint16_t*)Y,
                 q_seq_stride, q_head_stride, (int)k_seq_stride, (int)k_head_stride, (int)v_seq_stride,
                 (int)v_head_stride, (int)mask_row_stride, S, nh, nkv, L, scale * PA_LOG2E,
-                splits > 1 ? work : nullptr, pos, window < L ? window : L, sinks < L ? sinks : L};
-  const int wide = window > 0 && splits == 1 ? prompt_window_tiles(S, nh, nkv) : 0;
+                splits > 1 ? work : nullptr, pos};
   const int groups = nh / nkv;
   const dim3 grid(nkv, (S + PA_QB - 1) / PA_QB, splits);
   int rc;
-  if (wide && (dtype == DT_F16 || dtype == DT_BF16))
-    rc = prompt_window_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride, v_head_stride,
-                              pos, Y, S, nh, nkv, L, a.window, a.sinks, scale, dtype, wide, stream);
-  else if (window > 0 && dtype == DT_F16)
-    rc = prefill_dispatch<DT_F16, true, true>(groups, grid, splits, a, stream);
-  else if (window > 0 && dtype == DT_BF16)
-    rc = prefill_dispatch<DT_BF16, true, true>(groups, grid, splits, a, stream);
-  else if (dtype == DT_F16)
+  if (dtype == DT_F16)
     rc = causal ? prefill_dispatch<DT_F16, true>(groups, grid, splits, a, stream)
                 : prefill_dispatch<DT_F16, false>(groups, grid, splits, a, stream);
   else if (dtype == DT_BF16)
@@ -716,28 +703,7 @@ static int prefill_launch(const void* Q, long long q_seq_stride, long long q_hea
   else
     return (int)hipErrorInvalidValue;
   if (rc) return rc;
-  if (splits > 1) {
-    const long long n = (long long)S * nh * (HD / 8);
-    const dim3 mg((unsigned)((n + 255) / 256));
-#define TTSP_PM(DTV, SPM) \
-  hipLaunchKernelGGL((prefill_merge_kernel<DTV, SPM>), mg, dim3(256), 0, stream, work, splits, S, nh, (uint16_t*)Y)
-#define TTSP_PM_SP(DTV)          \
-  if (splits <= 2)               \
-    TTSP_PM(DTV, 2);             \
-  else if (splits <= 4)          \
-    TTSP_PM(DTV, 4);             \
-  else if (splits <= 8)          \
-    TTSP_PM(DTV, 8);             \
-  else                           \
-    TTSP_PM(DTV, 16);
-    if (dtype == DT_F16) {
-      TTSP_PM_SP(DT_F16)
-    } else {
-      TTSP_PM_SP(DT_BF16)
-    }
-#undef TTSP_PM_SP
-#undef TTSP_PM
-  }
+  if (splits > 1) prefill_merge(work, splits, S, nh, Y, dtype, stream);
   TTSP_RETURN_LAUNCH();
 }
 
@@ -775,28 +741,4 @@ extern "C" int ttsp_prefill_attention_causal(const void* Q, long long q_seq_stri
   if (!pos) return (int)hipErrorInvalidValue;
   return prefill_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride,
                         v_head_stride, nullptr, 0, pos, Y, S, nh, nkv, L, scale, dtype, work, splits, stream);
-}
-
-// Keys the rows of a workgroup see at most.
-static int window_keys(int S, int L, int window, int sinks) {
-  const long long n = (long long)window + sinks + S;
-  return n < L ? (int)n : L;
-}
-
-extern "C" int ttsp_prefill_attention_window_splits(int S, int nh, int nkv, int L, int window, int sinks) {
-  if (S <= 0 || nkv <= 0 || nh < nkv || L <= 0 || window <= 0 || sinks < 0) return 1;
-  if (prompt_window_tiles(S, nh, nkv)) return 1;
-  return prefill_splits(S, nkv, window_keys(S, L, window, sinks));
-}
-
-extern "C" int ttsp_prefill_attention_window(const void* Q, long long q_seq_stride, long long q_head_stride,
-                                             const void* K, long long k_seq_stride, long long k_head_stride,
-                                             const void* V, long long v_seq_stride, long long v_head_stride,
-                                             const long long* pos, void* Y, int S, int nh, int nkv, int L, int window,
-                                             int sinks, float scale, int dtype, float* work, int splits,
-                                             hipStream_t stream) {
-  if (!pos || window < 1 || sinks < 0) return (int)hipErrorInvalidValue;
-  return prefill_launch(Q, q_seq_stride, q_head_stride, K, k_seq_stride, k_head_stride, V, v_seq_stride,
-                        v_head_stride, nullptr, 0, pos, Y, S, nh, nkv, L, scale, dtype, work, splits, stream, window,
-                        sinks);
 }

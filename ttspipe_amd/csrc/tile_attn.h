@@ -152,15 +152,27 @@ struct TaWave {
       for (int d = 0; d < D / 32; ++d) o[d] = mfma32<DT>(vt[d], pf[i], o[d]);
   }
 
-  // 32 NB keys, K and V rows at k and v. masked (uniform): key j of them is none where gone(j).
-  template <int NB, typename F>
-  __device__ __forceinline__ void run(const uint8_t* k, const uint8_t* v, float scale2, bool masked, F gone) {
+  // 32 NB keys, K and V rows at k and v. masked (uniform): those behind key `after` of them
+  // are none, nor the `hidden` ones from key `from` on, nor 16-key run i where bit i of
+  // `gone` (uniform) is set.
+  template <int NB>
+  __device__ __forceinline__ void run(const uint8_t* k, const uint8_t* v, float scale2, bool masked, int after, int from,
+                                      uint32_t hidden, uint32_t gone) {
     constexpr int RB = 32 * D * 2;  // bytes of 32 rows
     const int h4 = (threadIdx.x & 63) >> 5 << 2;
     auto mask = [&](int b, f32x16_v& s) {
+      int last = after - (32 * b + h4), first = from - (32 * b + h4);
+      asm volatile("" : "+v"(last), "+v"(first));  // (what follows from them would be computed ahead, and spilled)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (gone(32 * b + 8 * (r / 4) + h4 + r % 4)) s[r] = -__builtin_inff();
+      for (int r = 0; r < 16; ++r) {
+        const int j = 8 * (r / 4) + r % 4;
+        if ((j > last) | ((uint32_t)(j - first) < hidden)) s[r] = -__builtin_inff();
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (gone >> (2 * b + i) & 1)
+#pragma unroll
+          for (int r = 0; r < 8; ++r) s[8 * i + r] = -__builtin_inff();
     };
     u32x4 kf[NB][D / 16];
 #pragma unroll
