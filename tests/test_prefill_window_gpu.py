@@ -75,7 +75,7 @@ def test_spans_and_windows(S, window, sinks):
         check(*a, window, sinks, run(*a, window, sinks), f"L {L}")
 
 
-@pytest.mark.parametrize("nh,nkv", [(1, 1), (2, 1), (3, 1), (32, 8), (5, 1), (12, 2), (7, 7), (14, 2), (8, 1), (16, 8)])
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (2, 1), (3, 1), (32, 8), (5, 1), (12, 2), (7, 7), (14, 2), (8, 1), (16, 8), (24, 1), (70, 1)])
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_other_heads(nh, nkv, dtype):
     for S, L, window, sinks in ((100, 100, 40, 3), (70, 1200, 300, 16), (40, 900, 800, 0)):
@@ -167,7 +167,13 @@ def test_refusals():
     for bad in (pos.int(), pos[:19], pos.cpu()):
         assert att(q, k, v, None, 8, 2, 128, positions=bad, window=5) is None
     assert att(q.float(), k.float(), v.float(), None, 8, 2, 128, positions=pos, window=5) is None
-    assert att(q.repeat(1, 3, 1, 1), k[:, :1], v[:, :1], None, 24, 1, 128, positions=pos, window=5) is None
+    assert att(q.repeat(1, 3, 1, 1), k[:, :1], v[:, :1], None, 24, 1, 64, positions=pos, window=5) is None
+    assert att(q[:, :7], k, v, None, 7, 2, 128, positions=pos, window=5) is None
+    for odd in (q[..., 4:], torch.randn(1, 8, 20, 132, dtype=BF, device="cuda")[..., :128]):
+        assert att(odd, k, v, None, 8, 2, 128, positions=pos, window=5) is None
+    for kw in (dict(out=torch.empty(1, 20, 1000, dtype=BF, device="cuda")), dict(out=torch.empty(1, 20, 1024, device="cuda"))):
+        with pytest.raises(ValueError):
+            att(q, k, v, None, 8, 2, 128, positions=pos, window=5, **kw)
 
 
 def test_a_captured_call_follows_the_positions():

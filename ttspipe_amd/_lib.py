@@ -247,15 +247,18 @@ def stream() -> int:
 
 def launch(what: str, dev: int, *args) -> None:
     """`what` of the library on the current stream of device `dev`."""
-    import torch
-
-    fn = getattr(lib(), what)
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(*args, stream())
+    fn = getattr(_lib if _lib is not None else load(), what)
+    if _raw_stream is None:
+        stream()  # (finds torch's getters)
+    if _raw_stream is not None and _raw_stream[1]() == dev:
+        rc = fn(*args, _raw_stream[0](dev))
     else:
+        import torch
+
         with torch.cuda.device(dev):
             rc = fn(*args, stream())
-    check(rc, what)
+    if rc:
+        raise RuntimeError(f"{what} failed: hipError_t {rc}")
 
 
 def check(rc: int, what: str) -> None:

@@ -19,6 +19,8 @@ attention kernels, row by row.
 
 from __future__ import annotations
 
+import functools
+
 GROUPED_MAX_QUERY = 64
 HEAD_DIM = 128
 CHUNK = 64  # cache positions per chunk of the decode attention (ttsp_attn_chunk)
@@ -82,7 +84,9 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     pairs), whose merge order rounds differently.
     `window` (with `positions`): row i sees keys j <= positions[i] with j < sinks
     or j > positions[i] - window only, and key blocks that no row of a workgroup
-    sees are not read (their workspace: `prefill_splits(...)`)."""
+    sees are not read. Any number of query heads a KV head is taken, and tensors
+    of another device than the current one; the workspace is of
+    `prefill_work_floats(S, n_head, prefill_splits(...))` elements."""
     import torch
 
     from ttspipe_amd import _lib
@@ -91,6 +95,8 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
         raise ValueError("a window goes by the rows' positions")
     if sinks < 0 or (window is None and sinks) or (window is not None and window < 1):
         raise ValueError("a window has at least one key, and its sinks are not negative")
+    if window is not None:
+        return _windowed(q, k, v, n_head, n_local_heads, head_dim, out, work, positions, int(window), int(sinks))
     if not _lib.gpu_present() or not _prefill_eligible(q, k, v, mask, n_head, n_local_heads, head_dim, positions):
         _stats["prefill_declined"] += 1
         return None
@@ -100,9 +106,7 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     elif out.shape != (1, seqlen, n_head * head_dim) or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous (1, S, n_head * head_dim) tensor of q's dtype")
     lib = _lib.lib()
-    if window is not None:
-        window, sinks = min(int(window), L), min(int(sinks), L)
-    splits = prefill_splits(seqlen, n_head, n_local_heads, L, window, sinks)
+    splits = lib.ttsp_prefill_attention_splits(seqlen, n_local_heads, L)
     need = prefill_work_floats(seqlen, n_head, splits)
     if splits > 1 and work is None:
         work = torch.empty(need, dtype=torch.float32, device=q.device)
@@ -110,12 +114,7 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
                          or work.data_ptr() % 16):
         raise ValueError(f"work must be a contiguous 16-byte aligned fp32 tensor of at least {need} elements")
     wp = work.data_ptr() if splits > 1 else None
-    if window is not None:
-        _lib.launch("ttsp_prefill_attention_window", q.get_device(), q.data_ptr(), q.stride(2), q.stride(1), k.data_ptr(),
-                    k.stride(2), k.stride(1), v.data_ptr(), v.stride(2), v.stride(1), positions.data_ptr(), out.data_ptr(),
-                    seqlen, n_head, n_local_heads, L, window, sinks, float(head_dim**-0.5), _lib.dtype_code(q.dtype), wp,
-                    splits)
-    elif positions is not None:
+    if positions is not None:
         rc = lib.ttsp_prefill_attention_causal(
             q.data_ptr(), q.stride(2), q.stride(1), k.data_ptr(), k.stride(2), k.stride(1), v.data_ptr(),
             v.stride(2), v.stride(1), positions.data_ptr(), out.data_ptr(), seqlen, n_head, n_local_heads, L,
@@ -129,6 +128,57 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
         _lib.check(rc, "ttsp_prefill_attention_split")
     _stats["prefill_attn"] += 1
     return out.view(1, seqlen, n_head, head_dim).transpose(1, 2)
+
+
+def _windowed(q, k, v, n_head, n_local_heads, head_dim, out, work, positions, window, sinks):
+    """`prefill_attention` through a window (its checks in one place: a short span's call is bound by them)."""
+    import torch
+
+    from ttspipe_amd import _lib
+
+    dtype, dev, qs, ks = q.dtype, q.get_device(), q.shape, k.shape
+    dt = _lib.dtype_code(dtype)
+    if (not _lib.gpu_present() or dev < 0 or dt not in (_lib.DT_F16, _lib.DT_BF16) or k.dtype is not dtype or v.dtype is not dtype
+            or len(qs) != 4 or len(ks) != 4 or v.shape != ks or k.get_device() != dev or v.get_device() != dev
+            or head_dim != HEAD_DIM or qs[0] != 1 or qs[1] != n_head or qs[3] != HEAD_DIM or ks[0] != 1 or ks[3] != HEAD_DIM
+            or ks[1] != n_local_heads or n_local_heads < 1 or n_head % n_local_heads or n_head > 65535 or not qs[2] or not ks[2]
+            or positions.dtype is not torch.int64 or positions.dim() != 1 or positions.shape[0] != qs[2]
+            or not positions.is_contiguous() or positions.get_device() != dev):
+        _stats["prefill_declined"] += 1
+        return None
+    (_, qh, qr, ql), (_, kh, kr, kl), (_, vh, vr, vl) = q.stride(), k.stride(), v.stride()
+    qp, kp, vp, S, L = q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[2], ks[2]
+    if (ql != 1 or kl != 1 or vl != 1 or qh % 8 or qr % 8 or kh % 8 or kr % 8 or vh % 8 or vr % 8 or qp % 16 or kp % 16 or vp % 16
+            or S > 1 << 20 or L >= 1 << 31 or max((L - 1) * kr + 128, (L - 1) * vr + 128) >= 1 << 30
+            or -(-S * (n_head // n_local_heads) // 64) * n_local_heads > 1 << 20):
+        _stats["prefill_declined"] += 1
+        return None
+    if out is None:
+        out = q.new_empty((1, S, n_head * HEAD_DIM))
+    elif (out.shape != (1, S, n_head * HEAD_DIM) or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != dev
+          or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous, 16-byte aligned (1, S, n_head * head_dim) tensor of q's dtype")
+    window, sinks = min(window, L), min(sinks, L)
+    splits, wp = _window_splits(S, n_head, n_local_heads, L, window, sinks), 0
+    if splits > 1:
+        need = prefill_work_floats(S, n_head, splits)
+        if work is None:
+            work = q.new_empty(need, dtype=torch.float32)
+        elif (work.dtype is not torch.float32 or work.numel() < need or not work.is_contiguous() or work.get_device() != dev
+              or work.data_ptr() % 16):
+            raise ValueError(f"work must be a contiguous 16-byte aligned fp32 tensor of at least {need} elements")
+        wp = work.data_ptr()
+    _lib.launch("ttsp_prefill_attention_window", dev, qp, qr, qh, kp, kr, kh, vp, vr, vh, positions.data_ptr(), out.data_ptr(), S,
+                n_head, n_local_heads, L, window, sinks, HEAD_DIM**-0.5, dt, wp, splits)
+    _stats["prefill_attn"] += 1
+    return out.view(1, S, n_head, HEAD_DIM).transpose(1, 2)
+
+
+@functools.lru_cache(maxsize=256)
+def _window_splits(seqlen, n_head, n_local_heads, width, window, sinks) -> int:
+    from ttspipe_amd import _lib
+
+    return _lib.lib().ttsp_prefill_attention_window_splits(seqlen, n_head, n_local_heads, width, window, sinks)
 
 
 #: Longest causal span `causal_rows_attention` serves (the grouped decode
@@ -225,8 +275,7 @@ def prefill_splits(seqlen: int, n_head: int, n_local_heads: int, width: int, win
 
     if window is None:
         return _lib.lib().ttsp_prefill_attention_splits(seqlen, n_local_heads, width)
-    return _lib.lib().ttsp_prefill_attention_window_splits(seqlen, n_head, n_local_heads, width, min(window, width),
-                                                           min(sinks, width))
+    return _window_splits(seqlen, n_head, n_local_heads, width, min(int(window), width), min(int(sinks), width))
 
 
 def prefill_work_floats(seqlen: int, n_head: int, splits: int) -> int:

@@ -23,6 +23,8 @@ from __future__ import annotations
 
 import struct
 
+import torch
+
 from ttspipe_amd import _lib
 
 #: Largest `top_k` the kernel takes; larger requests use the caller's sampler.
@@ -50,8 +52,6 @@ def sample(logits, temperature, top_p, top_k, uniform=None):
     one-element int64 tensor, all on the logits' device (so a captured graph
     can change them in place); `uniform` (optional) supplies the per-index
     uniform numbers (default: `torch.rand`)."""
-    import torch
-
     row = logits.reshape(-1)
     if row.numel() > MAX_VOCAB:
         return None
@@ -81,19 +81,30 @@ def pack_mask(allowed):
     """The words `penalize` takes as `mask` (int32, (..., ceil(V / 32))) from a
     boolean tensor (..., V): bit t % 32 of word t // 32 is allowed[..., t]. Torch
     operations, for programs whose grammar does not write the words itself."""
-    import torch
-
     v = allowed.shape[-1]
     bits = torch.nn.functional.pad(allowed.to(torch.int64), (0, -v % 32)).unflatten(-1, (-1, 32))
     words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
     return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
 
 
-def _rows_of(t, shapes, what):
-    """(address, row stride) of a tensor of one of `shapes` with a contiguous last axis."""
-    if t.shape not in shapes or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what} must have one of the shapes {[tuple(s) for s in shapes]} and a contiguous last axis")
-    return t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else 0
+def _rows_of(t, rows, width, dev, what):
+    """(address, row stride) of a tensor (rows, width), (1, width) or (width,) on `dev`. (On every call's host path, as the next.)"""
+    shape = t.shape
+    if len(shape) == 2:
+        n, step = shape[0], t.stride()
+        if shape[1] == width and (n == rows or n == 1) and (step[1] == 1 or width < 2) and t.get_device() == dev:
+            return t.data_ptr(), step[0] if n > 1 else 0
+    elif len(shape) == 1 and shape[0] == width and (width < 2 or t.stride()[0] == 1) and t.get_device() == dev:
+        return t.data_ptr(), 0
+    raise ValueError(f"{what} must be ({rows}, {width}) or ({width},) with a contiguous last axis, on the logits' device")
+
+
+def _vector(t, rows, dev, what):
+    """(address, 0: one value for all rows) of an fp32 tensor of one value a row, or of one."""
+    n = t.numel()
+    if t.dtype is torch.float32 and (n == rows or n == 1) and t.dim() < 2 and t.is_contiguous() and t.get_device() == dev:
+        return t.data_ptr(), int(n > 1)
+    raise ValueError(f"{what} must be a contiguous fp32 tensor of one value a row, or of one, on the logits' device")
 
 
 def penalize(logits, history=None, *, lengths=None, repetition=None, frequency=None, presence=None, bias=None,
@@ -120,63 +131,59 @@ def penalize(logits, history=None, *, lengths=None, repetition=None, frequency=N
     take the logits (no GPU, another type, a last axis that is not contiguous);
     ValueError for parts that do not fit them. Work is queued on the current
     stream of the logits' device; with `out` nothing is allocated."""
-    import torch
-
-    dt = _lib.dtype_code(logits.dtype)
-    if not _lib.gpu_present() or dt is None or logits.dim() not in (1, 2) or logits.get_device() < 0:
+    dtype, shape, dev = logits.dtype, logits.shape, logits.get_device()
+    dt, dims = _lib.dtype_code(dtype), len(shape)
+    if not _lib.gpu_present() or dt is None or dims not in (1, 2) or dev < 0:
         return None
-    dev, vocab = logits.get_device(), logits.shape[-1]
-    rows = logits.shape[0] if logits.dim() == 2 else 1
-    x_row = logits.stride(0) if logits.dim() == 2 and rows > 1 else vocab
-    if vocab > 1 << 30 or rows > 1 << 24 or rows * -(-vocab // 1024) > 0xffffff or (vocab > 1 and logits.stride(-1) != 1):
+    step, vocab = logits.stride(), shape[-1]
+    rows, x_row = (shape[0], step[0]) if dims == 2 and shape[0] != 1 else (1, vocab)
+    if vocab > 1 << 30 or rows > 1 << 24 or rows * -(-vocab // 2048) > 0x3fffff or (vocab > 1 and step[-1] != 1):
         return None
-    for t in (history, lengths, repetition, frequency, presence, bias, mask):
-        if t is not None and t.get_device() != dev:
-            raise ValueError("every part must be on the logits' device")
-    hist = hp = hs = h64 = lp = l64 = 0
+    hist = hp = hs = h64 = lp = l64 = rp = rr = fp = fr = pp = pr = bp = bs = mp = ms = 0
+    bias_dt = dt
     if history is not None:
-        if history.dtype not in (torch.int32, torch.int64) or history.dim() not in (1, 2):
-            raise ValueError("history must be an int32 or int64 tensor (rows, H) or (H,)")
-        hist, h64 = history.shape[-1], int(history.dtype is torch.int64)
-        hp, hs = _rows_of(history, ((rows, hist), (1, hist), (hist,)), "history")
-        if hist >= 1 << 31:
-            raise ValueError("a history holds at most 2^31 - 1 tokens")
+        h64 = history.dtype is torch.int64
+        hist = history.shape[-1] if history.dim() else 0
+        if (not h64 and history.dtype is not torch.int32) or not history.dim() or hist >= 1 << 31:
+            raise ValueError("history must be an int32 or int64 tensor of at most 2^31 - 1 tokens a row")
+        hp, hs = _rows_of(history, rows, hist, dev, "history")
     if lengths is not None:
-        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (rows,) or not lengths.is_contiguous():
-            raise ValueError("lengths must be a contiguous int32 or int64 tensor (rows,)")
-        lp, l64 = lengths.data_ptr(), int(lengths.dtype is torch.int64)
-    scalars = []
-    for t, what in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
-        if t is None:
-            scalars.append((0, 0))
-            continue
-        if t.dtype is not torch.float32 or t.dim() > 1 or t.numel() not in (rows, 1) or not t.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous fp32 tensor of one value a row, or of one")
-        scalars.append((t.data_ptr(), int(t.numel() > 1)))
-    bp = bs = mp = ms = 0
+        l64 = lengths.dtype is torch.int64
+        if ((not l64 and lengths.dtype is not torch.int32) or lengths.shape != (rows,) or not lengths.is_contiguous()
+                or lengths.get_device() != dev):
+            raise ValueError("lengths must be a contiguous int32 or int64 tensor (rows,) on the logits' device")
+        lp = lengths.data_ptr()
+    if repetition is not None:
+        rp, rr = _vector(repetition, rows, dev, "repetition")
+    if frequency is not None:
+        fp, fr = _vector(frequency, rows, dev, "frequency")
+    if presence is not None:
+        pp, pr = _vector(presence, rows, dev, "presence")
     if bias is not None:
-        if bias.dtype not in (torch.float32, logits.dtype):
+        if bias.dtype is torch.float32:
+            bias_dt = _lib.DT_F32
+        elif bias.dtype is not dtype:
             raise ValueError("bias must be fp32 or of the logits' type")
-        bp, bs = _rows_of(bias, ((rows, vocab), (1, vocab), (vocab,)), "bias")
+        bp, bs = _rows_of(bias, rows, vocab, dev, "bias")
     if mask is not None:
-        words = -(-vocab // 32)
         if mask.dtype is not torch.int32:
             raise ValueError("mask must hold int32 words")
-        mp, ms = _rows_of(mask, ((rows, words), (1, words), (words,)), "mask")
+        mp, ms = _rows_of(mask, rows, -(-vocab // 32), dev, "mask")
+    xp = logits.data_ptr()
     if out is None:
-        out = logits.new_empty(logits.shape)
-    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (vocab > 1 and out.stride(-1) != 1):
-        raise ValueError("out must have the logits' shape, type and device, and a contiguous last axis")
-    y_row = out.stride(0) if logits.dim() == 2 and rows > 1 else vocab
-    if not rows or not vocab:
-        return out
-    if rows > 1 and y_row < vocab:
-        raise ValueError("out's rows must not overlap")
-    xp, yp, size = logits.data_ptr(), out.data_ptr(), logits.element_size()
-    if (xp != yp or x_row != y_row) and xp < yp + ((rows - 1) * y_row + vocab) * size and yp < xp + ((rows - 1) * x_row + vocab) * size:
-        raise ValueError("out must be the logits themselves or not overlap them")
-    (rp, rr), (fp, fr), (pp, pr) = scalars
-    block = _PENALTIES.pack(hp, lp, rp, fp, pp, bp, mp, hs, bs, ms, hist, h64, l64, rr, fr, pr,
-                            dt if bias is None else _lib.dtype_code(bias.dtype))
-    _lib.launch("ttsp_penalize", dev, block, xp, x_row, yp, y_row, rows, vocab, dt)
+        out = logits.new_empty(shape)
+        yp, y_row = out.data_ptr(), vocab
+    else:
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or (vocab > 1 and out.stride()[-1] != 1):
+            raise ValueError("out must have the logits' shape, type and device, and a contiguous last axis")
+        yp, y_row = out.data_ptr(), out.stride()[0] if rows > 1 else vocab
+        if rows > 1 and vocab and y_row < vocab:
+            raise ValueError("out's rows must not overlap")
+        size = out.element_size()
+        if ((xp != yp or x_row != y_row) and rows and vocab and xp < yp + ((rows - 1) * y_row + vocab) * size
+                and yp < xp + ((rows - 1) * x_row + vocab) * size):
+            raise ValueError("out must be the logits themselves or not overlap them")
+    if rows and vocab:
+        block = _PENALTIES.pack(hp, lp, rp, fp, pp, bp, mp, hs, bs, ms, hist, h64, l64, rr, fr, pr, bias_dt)
+        _lib.launch("ttsp_penalize", dev, block, xp, x_row, yp, y_row, rows, vocab, dt)
     return out
