@@ -130,6 +130,15 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     return out.view(1, seqlen, n_head, head_dim).transpose(1, 2)
 
 
+def window_mask(positions, width: int, window: int, sinks: int = 0):
+    """The boolean mask (1, 1, S, width) of a sliding window with sinks, for `decode_attention`: row i
+    allows keys j <= positions[i] with j < sinks or j > positions[i] - window."""
+    import torch
+
+    key, pos = torch.arange(width, device=positions.device), positions[:, None]
+    return ((key <= pos) & ((key < sinks) | (key > pos - window)))[None, None]
+
+
 def _windowed(q, k, v, n_head, n_local_heads, head_dim, out, work, positions, window, sinks):
     """`prefill_attention` through a window (its checks in one place: a short span's call is bound by them)."""
     import torch

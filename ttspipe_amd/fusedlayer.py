@@ -342,15 +342,15 @@ def _attend_in_parts(q, kc, vc, input_pos, nh, nkv, parts):
     return out.view(1, n, nh, HEAD_DIM).transpose(1, 2)
 
 
-def prefill_block(block, x, freqs_cis, mask, input_pos):
+def prefill_block(block, x, freqs_cis, mask, input_pos, *, window=None, sinks=0):
     """`TransformerBlock.forward` for several positions (B = 1, S > 1), or None.
     The block of `prefill_block_chain` without a carried norm."""
-    r = prefill_block_chain(block, x, freqs_cis, mask, input_pos)
+    r = prefill_block_chain(block, x, freqs_cis, mask, input_pos, window=window, sinks=sinks)
     return None if r is None else r[0]
 
 
 def prefill_block_chain(block, x, freqs_cis, mask, input_pos, *, xn=None, next_norm=None, causal=False,
-                        attend=None):
+                        attend=None, window=None, sinks=0):
     """`(out, out_n)`: the block's output for several positions (B = 1, S > 1)
     and, with `next_norm` (an RMSNorm module), `next_norm(out)` for the next
     block (else None, and None for a span of up to `nf4gemv.FUSED_MAX_ROWS`
@@ -368,6 +368,9 @@ def prefill_block_chain(block, x, freqs_cis, mask, input_pos, *, xn=None, next_n
     `attend` (with `causal`): `(first row, end row, window)` of each attention
     launch, in order and covering the rows, each over the first `window` cache
     positions; default one launch over the mask's width.
+    `window`, `sinks`: each row sees keys j <= its position with j < sinks or
+    j > position - window, and the mask's width alone counts (of the block's other
+    arguments `causal` and `attend` go with no window).
 
     The fork's block in its own order with the prefill kernels: RMSNorm,
     wqkv GEMM, q/k head norms + rotary + KV-cache write for every row in one
@@ -385,6 +388,10 @@ def prefill_block_chain(block, x, freqs_cis, mask, input_pos, *, xn=None, next_n
     from ttspipe_amd import fastpath, fusedops, nf4gemv
     from ttspipe_amd.llama import apply_rotary_emb
 
+    if window is not None and (causal or attend is not None):
+        raise ValueError("a window goes without causal and attend")
+    if (window is None and sinks) or (window is not None and (window < 1 or sinks < 0)):
+        raise ValueError("a window has at least one key, and its sinks are not negative")
     if not _lib.gpu_present() or not _prefill_eligible(block, x, mask, input_pos):
         return None
     a, ff = block.attention, block.feed_forward
@@ -467,6 +474,10 @@ def prefill_block_chain(block, x, freqs_cis, mask, input_pos, *, xn=None, next_n
             k, v = k[:, :, : mask.shape[-1]], v[:, :, : mask.shape[-1]]
         if causal and rows_ok and attend is not None:
             y = _attend_in_parts(q, kc, vc, input_pos, nh, nkv, attend)
+        if window is not None:
+            y = fastpath.prefill_attention(q, k, v, None, nh, nkv, hd, positions=input_pos, window=window, sinks=sinks)
+            if y is None:
+                y = fastpath.decode_attention(q, k, v, fastpath.window_mask(input_pos, k.shape[2], window, sinks), nh, nkv, hd)
         # a causal span's mask follows from its positions: computed in the kernel, not read
         if y is None:
             y = fastpath.prefill_attention(q, k, v, mask, nh, nkv, hd, positions=input_pos if causal else None)

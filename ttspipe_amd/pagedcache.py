@@ -19,8 +19,9 @@ it needs and gives them back. For D-wide heads (64 or 128) and 16-bit caches:
   gathered and the position its row came from; a head's slots contiguous, any
   strides that keep the heads apart.
 
-`qk_rope_kv` and `store` write rows, `attention` reads them, `evict` cuts a
-sequence down to a budget. `PageTable` hands the pages out and keeps the device
+`qk_rope_kv` and `store` write rows, `attention` reads them (all of a sequence's,
+or those a sliding window leaves, and those of a prefix that sequences share),
+`evict` cuts a sequence down to a budget. `PageTable` hands the pages out and keeps the device
 tensors above; `PagedKVCache` is one layer's pools with the four calls as
 methods; `fusedlayer.decode_batch` runs a transformer block on them.
 
@@ -415,14 +416,22 @@ class PageTable:
     drops them. Running out of pages raises MemoryError and changes nothing; so does,
     with ValueError, a row past `max_len` rows or past `max_position` positions
     (the rotary table's rows: a sequence that is evicted from runs on while its
-    rows stay few; None: not checked here)."""
+    rows stay few; None: not checked here).
+
+    With `prefixes`, up to so many prefixes of up to `max_prefix` rows (default:
+    `max_len`) are held beside the sequences, in pages of the same pools:
+    `admit_prefix` takes one in, `admit(rows, prefix=p)` starts a sequence behind it
+    (its own slots count from 0, its positions from the prefix's end), and `prefix`
+    is what `attention` takes. `slide` gives pages back that a window has left."""
 
     def __init__(self, seqs: int, max_len: int, pages: int, page_size: int = 64, device="cuda",
-                 max_position: int | None = None):
+                 max_position: int | None = None, prefixes: int = 0, max_prefix: int | None = None):
         if not MIN_PAGE <= page_size <= MAX_PAGE or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from {MIN_PAGE} to {MAX_PAGE}")
         if seqs < 1 or pages < 1 or max_len < 1 or (max_position is not None and max_position < 1):
             raise ValueError("seqs, max_len, pages and max_position must be positive")
+        if not 0 <= prefixes <= _lib.PAGED_MAX_PREFIXES or (max_prefix is not None and max_prefix < 1):
+            raise ValueError(f"a table has 0 to {_lib.PAGED_MAX_PREFIXES} prefixes, of at least one row")
         self.page_size, self.pages, self.max_len, self.max_position = page_size, pages, max_len, max_position
         columns = -(-max_len // page_size)
         self.block_table = torch.full((seqs, columns), -1, dtype=torch.int32, device=device)
@@ -430,8 +439,18 @@ class PageTable:
         self.positions = torch.full((seqs,), -1, dtype=torch.int64, device=device)
         self._active = torch.zeros(seqs, dtype=torch.int64, device=device)
         self._free = list(range(pages - 1, -1, -1))
-        self._held: list[list[int]] = [[] for _ in range(seqs)]
+        self._held: list[list[int | None]] = [[] for _ in range(seqs)]  # (None: given back by `slide`)
         self._rows, self._next = [0] * seqs, [0] * seqs  # rows held, the next position
+        self.max_prefix = max_len if max_prefix is None else max_prefix
+        self._prefix: list[int | None] = [None] * seqs
+        self._prefix_held: list[list[int]] = [[] for _ in range(prefixes)]
+        self._prefix_rows = [0] * prefixes
+        self.prefix = None
+        if prefixes:
+            self.prefix = Prefix(
+                torch.full((prefixes, -(-self.max_prefix // page_size)), -1, dtype=torch.int32, device=device),
+                torch.full((prefixes,), -1, dtype=torch.int64, device=device),
+                torch.full((seqs,), -1, dtype=torch.int32, device=device))
 
     @property
     def free_pages(self) -> int:
@@ -443,8 +462,17 @@ class PageTable:
         return max(self._next)
 
     def rows(self, seq: int) -> int:
-        """Rows sequence `seq` holds."""
+        """Rows sequence `seq` holds (its own, behind its prefix's)."""
         return self._rows[seq]
+
+    def prefix_rows(self, prefix: int) -> int:
+        """Rows prefix `prefix` holds."""
+        return self._prefix_rows[prefix]
+
+    def first_position(self, seq: int) -> int:
+        """The position of sequence `seq`'s first own row: its prefix's rows."""
+        p = self._prefix[seq]
+        return 0 if p is None else self._prefix_rows[p]
 
     def _missing(self, seq: int, rows: int) -> int:
         return max(0, -(-rows // self.page_size) - len(self._held[seq]))
@@ -457,22 +485,64 @@ class PageTable:
             for _ in range(self._missing(seq, rows)):
                 new.append((seq, len(held), self._free.pop()))
                 held.append(new[-1][2])
-        if not new:
-            return
-        dev = self.block_table.device
-        up = torch.tensor(list(zip(*new)), dtype=torch.int64, pin_memory=dev.type == "cuda").to(dev, non_blocking=True)
-        self.block_table[up[0], up[1]] = up[2].to(torch.int32)
+        self._write(self.block_table, new)
 
-    def _place(self, seq: int, newest: int, active: int) -> None:
+    @staticmethod
+    def _write(table, entries) -> None:
+        """`entries`, (row, column, page) triples, into a table, in one upload that nothing waits for."""
+        if not entries:
+            return
+        dev = table.device
+        up = torch.tensor(list(zip(*entries)), dtype=torch.int64, pin_memory=dev.type == "cuda").to(dev, non_blocking=True)
+        table[up[0], up[1]] = up[2].to(torch.int32)
+
+    def _place(self, seq: int, newest: int, position: int, active: int) -> None:
         # (fill_: a number assigned to one element is uploaded, and waited for)
         self.slots[seq].fill_(newest)
-        self.positions[seq].fill_(newest)
+        self.positions[seq].fill_(position)
         self._active[seq].fill_(active)
+        if self.prefix is not None:
+            p = self._prefix[seq]
+            self.prefix.of[seq].fill_(-1 if p is None else p)
 
-    def admit(self, rows: int):
+    def admit_prefix(self, rows: int):
+        """A free prefix with pages for `rows` rows (at positions 0 .. rows - 1; `PagedKVCache.store_prefix`
+        writes them): its index, or None when every prefix is taken."""
+        if self.prefix is None:
+            raise ValueError("this table has no prefixes")
+        if not 1 <= rows <= self.max_prefix or rows > (self.max_position or rows):
+            raise ValueError(f"a prefix holds 1 to {self.max_prefix} rows, at positions below {self.max_position}")
+        p = next((i for i, n in enumerate(self._prefix_rows) if n == 0), None)
+        if p is None:
+            return None
+        need = -(-rows // self.page_size)
+        if need > len(self._free):
+            raise MemoryError(f"{need} pages needed, {len(self._free)} free")
+        held = self._prefix_held[p] = [self._free.pop() for _ in range(need)]
+        self._write(self.prefix.table, [(p, c, page) for c, page in enumerate(held)])
+        self._prefix_rows[p] = rows
+        self.prefix.slots[p].fill_(rows - 1)
+        return p
+
+    def release_prefix(self, prefix: int) -> None:
+        """Prefix `prefix` ends (ValueError while a sequence has it): its pages go back to the pool."""
+        if not 0 <= prefix < len(self._prefix_rows):
+            raise ValueError(f"there is no prefix {prefix}")
+        if prefix in self._prefix:
+            raise ValueError(f"sequence {self._prefix.index(prefix)} has prefix {prefix}")
+        self._free += self._prefix_held[prefix][::-1]
+        self._prefix_held[prefix], self._prefix_rows[prefix] = [], 0
+        self.prefix.table[prefix].fill_(-1)
+        self.prefix.slots[prefix].fill_(-1)
+
+    def admit(self, rows: int, prefix: int | None = None):
         """A free sequence with pages for `rows` rows (a prompt's, at positions
-        0 .. rows - 1): its index, or None when every sequence is taken."""
-        if not 1 <= rows <= self.max_len or rows > (self.max_position or rows):
+        0 .. rows - 1, or from the end of `prefix` on): its index, or None when every
+        sequence is taken."""
+        if prefix is not None and not (0 <= prefix < len(self._prefix_rows) and self._prefix_rows[prefix]):
+            raise ValueError(f"there is no prefix {prefix}")
+        first = 0 if prefix is None else self._prefix_rows[prefix]
+        if not 1 <= rows <= self.max_len or first + rows > (self.max_position or first + rows):
             raise ValueError(f"a sequence holds 1 to {self.max_len} rows, at positions below {self.max_position}")
         seq = next((i for i, n in enumerate(self._rows) if n == 0), None)
         if seq is None:
@@ -480,8 +550,8 @@ class PageTable:
         if self._missing(seq, rows) > len(self._free):
             raise MemoryError(f"{self._missing(seq, rows)} pages needed, {len(self._free)} free")
         self._grow([(seq, rows)])
-        self._rows[seq] = self._next[seq] = rows
-        self._place(seq, rows - 1, 1)
+        self._rows[seq], self._next[seq], self._prefix[seq] = rows, first + rows, prefix
+        self._place(seq, rows - 1, first + rows - 1, 1)
         return seq
 
     def step(self) -> None:
@@ -513,29 +583,48 @@ class PageTable:
             if n > budget:
                 self._rows[seq] = budget
                 held = self._held[seq]
-                self._free += held[keep:][::-1]
+                self._free += [page for page in held[keep:][::-1] if page is not None]
                 del held[keep:]
         if len(self._free) > free:  # (no sequence holds more than `keep` pages now)
             self.block_table[:, keep:].fill_(-1)
+
+    def slide(self, window: int, sinks: int = 0) -> None:
+        """Pages of which `attention` with this window reads no row, at this step or
+        a later one, go back to the pool. With several layers the window is the
+        widest one, and with layers that have none there is nothing to give back."""
+        if window < 1 or sinks < 0:
+            raise ValueError("a window has at least one row, and its sinks are not negative")
+        first, gone = -(-sinks // self.page_size), []
+        for seq, n in enumerate(self._rows):
+            held = self._held[seq]
+            for c in range(first, max(n - window, 0) // self.page_size):
+                if held[c] is not None:
+                    gone.append((seq, c, -1))
+                    self._free.append(held[c])
+                    held[c] = None
+        self._write(self.block_table, gone)
 
     def release(self, seq: int) -> None:
         """Sequence `seq` ends: its pages go back to the pool."""
         if not 0 <= seq < len(self._rows):
             raise ValueError(f"there is no sequence {seq}")
-        self._free += self._held[seq][::-1]
-        self._held[seq], self._rows[seq], self._next[seq] = [], 0, 0
+        self._free += [page for page in self._held[seq][::-1] if page is not None]
+        self._held[seq], self._rows[seq], self._next[seq], self._prefix[seq] = [], 0, 0, None
         self.block_table[seq].fill_(-1)
-        self._place(seq, -1, 0)
+        self._place(seq, -1, -1, 0)
 
 
 class PagedKVCache(nn.Module):
     """One layer's pools on a `PageTable`. `tracked`: with the scores and slot
-    positions that `evict` needs."""
+    positions that `evict` needs. `window`, `sinks`: `attention` goes through that
+    window (and `evict` is refused: it takes the slots out of order)."""
 
-    def __init__(self, table: PageTable, n_heads: int, head_dim: int = 128, dtype=torch.bfloat16, tracked: bool = False):
+    def __init__(self, table: PageTable, n_heads: int, head_dim: int = 128, dtype=torch.bfloat16, tracked: bool = False,
+                 window: int | None = None, sinks: int = 0):
         super().__init__()
+        _window(window, sinks)
         dev = table.block_table.device
-        self.table = table
+        self.table, self.window, self.sinks = table, window, sinks
         shape = (table.pages, n_heads, table.page_size, head_dim)
         self.register_buffer("k_pages", torch.zeros(shape, dtype=dtype, device=dev))
         self.register_buffer("v_pages", torch.zeros(shape, dtype=dtype, device=dev))
@@ -564,24 +653,38 @@ class PagedKVCache(nn.Module):
 
     def store(self, seq: int, k, v, start: int = 0):
         """Rows start .. start + rows - 1 of sequence `seq` from k, v (rows, n_heads,
-        head_dim), their slots also their positions."""
+        head_dim), their slots, from the sequence's first position on, also their positions."""
         t, rows = self.table, k.shape[0]
         if not 0 <= seq < t.slots.shape[0] or start < 0 or start + rows > t.rows(seq):
             raise ValueError(f"sequence {seq} has no rows {start} to {start + rows - 1}")
         slots = torch.arange(start, start + rows, dtype=torch.int64, device=t.slots.device)
         seqs = torch.full((rows,), seq, dtype=torch.int32, device=t.slots.device)
-        return store(k, v, self.k_pages, self.v_pages, t.block_table, slots, positions=slots, seqs=seqs,
-                     scores=self.scores, slot_pos=self.slot_pos)
+        first = t.first_position(seq)
+        return store(k, v, self.k_pages, self.v_pages, t.block_table, slots, positions=slots + first if first else slots,
+                     seqs=seqs, scores=self.scores, slot_pos=self.slot_pos)
+
+    def store_prefix(self, prefix: int, k, v, start: int = 0):
+        """Rows start .. start + rows - 1 of prefix `prefix`, as `store`."""
+        t, rows = self.table, k.shape[0]
+        if t.prefix is None or not 0 <= prefix < t.prefix.slots.shape[0] or start < 0 or start + rows > t.prefix_rows(prefix):
+            raise ValueError(f"prefix {prefix} has no rows {start} to {start + rows - 1}")
+        slots = torch.arange(start, start + rows, dtype=torch.int64, device=t.slots.device)
+        seqs = torch.full((rows,), prefix, dtype=torch.int32, device=t.slots.device)
+        return store(k, v, self.k_pages, self.v_pages, t.prefix.table, slots, seqs=seqs)
 
     def attention(self, q, *, out=None, work=None):
-        """`attention` of each sequence's newest token; a tracked cache gathers its weights."""
+        """`attention` of each sequence's newest token, over its prefix where the table
+        has any, through the cache's window; a tracked cache gathers its weights."""
         t = self.table
-        return attention(q, self.k_pages, self.v_pages, t.block_table, t.slots, scores=self.scores, out=out, work=work)
+        return attention(q, self.k_pages, self.v_pages, t.block_table, t.slots, scores=self.scores, out=out, work=work,
+                         window=self.window, sinks=self.sinks, prefix=t.prefix)
 
     def evict(self, budget: int, *, sinks: int = 0, recent: int = 0, work=None):
         """`evict` on this layer (then, once for all layers, `PageTable.evicted`)."""
         if self.scores is None:
             raise ValueError("only a tracked cache is evicted from")
+        if self.window is not None:
+            raise ValueError("a cache with a window keeps its rows in order")
         t = self.table
         return evict(self.k_pages, self.v_pages, t.block_table, t.slots, self.scores, self.slot_pos, t.positions, budget,
                      sinks=sinks, recent=recent, work=work)
