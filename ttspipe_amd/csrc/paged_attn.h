@@ -69,12 +69,15 @@ constexpr int PG_STEP = PG_WAVES * PG_KEYS;    // chunk lengths are multiples of
 // 42.5 us; 64 of 2048 to 5119 167 / 166 / 165; one of 130995 90 / 96 / 96 (32 query
 // and 8 kv heads of 128, bf16; 512 of them, one round: 49 / 200 / 88).
 constexpr int PG_WGS = 1024;
+// One round where a window makes the sequences about as long (32 of 200 to 8000 rows,
+// window 1024: 35.3 us in two rounds, 33.2 in one; 64, window 4093: 183 and 174) and
+// beside a prefix's workgroups (24 behind five prefixes 45 and 38).
+constexpr int PG_ROUND = 512;
 // Caches of up to this many slots: a sequence is one chunk, and there is no
 // joining launch (300 rows, alone: 8.3 us; in three chunks and joined: 10.2).
 constexpr int PG_SHORT = 512;
 constexpr int PG_HEADS = 16;                   // query heads a workgroup takes
 // Rows a prefix's chunk has at most (their runs' places are held in LDS), and so its most chunks.
-constexpr int PF_OWN = 512;
 constexpr int PF_CHUNK = 8192, PF_CHUNKS = TTSP_PAGED_MAX_SLOTS / PF_CHUNK;
 constexpr float PG_NONE = -3.0e38f;            // the reference before any score
 // A moved reference lies `pg_below` under the largest score and moves again when a
@@ -769,7 +772,7 @@ inline bool attn_plan(int seqs, int nh, int nkv, int hd, long long cap, long lon
   const int group = nh / nkv;
   p->hgs = (group + PG_HEADS - 1) / PG_HEADS;
   const long long wide = (long long)nkv * p->hgs;
-  const int wgs = joined ? PF_OWN : PG_WGS;
+  const int wgs = joined || rows < cap ? PG_ROUND : PG_WGS;
   p->target = (int)(wide < wgs ? wgs / wide : 1);
   p->parts = p->scores = 0;
   if ((long long)seqs * ((rows + PG_STEP - 1) / PG_STEP) > 0x3fffffff) return false;  // (more rows than any memory holds)
