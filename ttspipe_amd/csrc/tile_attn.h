@@ -6,7 +6,10 @@
 // tiles of 64 through a ring of two in LDS, straight from memory (buffer loads to LDS,
 // so that no register holds what is on its way): RG waves take 32 rows each of the same
 // keys, and with two row groups (RG 2) the other two waves take the other half of a
-// tile's keys and join their sums through LDS at the end. Two workgroups fit a CU.
+// tile's keys and join their sums through LDS at the end. Two workgroups fit a CU: one
+// waits at its barrier while the other computes (eight waves in one workgroup: 64
+// sequences behind 32763 rows 111 us, so 100). A ring of four tiles is slower for few
+// tiles: twice the code to be fetched before it has run once (2 to 5 us).
 //
 // A wave's 32 keys: S^T = K Q^T on the matrix cores (Q stays in registers), so that a
 // lane holds 16 keys of one query row; the exponentials subtract a reference that
@@ -27,8 +30,6 @@
 #include "paged_attn.h"
 
 namespace ttsp {
-
-typedef __attribute__((address_space(3))) void* ta_lds_ptr;
 
 constexpr int TA_WAVES = 4, TA_T = 64 * TA_WAVES;
 
@@ -275,7 +276,7 @@ __device__ __forceinline__ void ta_join(TaWave<DT, D, PARTS>& w, bool& seen, uin
 // One load of 1024 bytes of rows from base into LDS at dst, lane l's 16 bytes from byte voff.
 __device__ __forceinline__ void ta_load(const void* base, uint32_t voff, uint8_t* dst) {
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, -1, 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ta_lds_ptr)dst, 16, voff, 0, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voff, 0, 0, 0);
 }
 
 }  // namespace ttsp

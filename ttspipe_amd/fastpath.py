@@ -84,7 +84,10 @@ def prefill_attention(q, k, v, mask, n_head, n_local_heads, head_dim, out=None, 
     pairs), whose merge order rounds differently.
     `window` (with `positions`): row i sees keys j <= positions[i] with j < sinks
     or j > positions[i] - window only, and key blocks that no row of a workgroup
-    sees are not read. Any number of query heads a KV head is taken, and tensors
+    sees are not read. A value that is not finite shows in the rows that see it, and
+    may in their neighbours (as a weight of 0 times it does); keys that are not
+    finite show in the rows that see them only. Any number of query heads a KV head
+    is taken, and tensors
     of another device than the current one; the workspace is of
     `prefill_work_floats(S, n_head, prefill_splits(...))` elements."""
     import torch
