@@ -284,14 +284,16 @@ def _workspace(work, need, dtype, like):
 def _prefix_block(prefix, seqs, page, dev):
     """The C-ABI's argument block of a `Prefix`, or None where the kernels do not take it."""
     table, slots, of = prefix
-    if (table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != dev
-            or not _vector(slots, torch.int64, table.shape[0], dev) or not _vector(of, torch.int32, seqs, dev)):
+    shape, step = table.shape, table.stride()
+    if len(shape) != 2:
         return None
-    (count, cols), (t0, t1) = table.shape, table.stride()
-    if (not 1 <= count <= _lib.PAGED_MAX_PREFIXES or not 1 <= cols <= _lib.PAGED_MAX_SLOTS // page or (t1 != 1 and cols > 1)
-            or (count > 1 and t0 < cols)):
+    (count, cols), (t0, t1) = shape, step
+    if (table.dtype is not torch.int32 or table.get_device() != dev or slots.dtype is not torch.int64 or slots.shape != (count,)
+            or not slots.is_contiguous() or slots.get_device() != dev or of.dtype is not torch.int32 or of.shape != (seqs,)
+            or not of.is_contiguous() or of.get_device() != dev or not 1 <= count <= _lib.PAGED_MAX_PREFIXES
+            or not 1 <= cols <= _lib.PAGED_MAX_SLOTS // page or (t1 != 1 and cols > 1) or (count > 1 and t0 < cols)):
         return None
-    return _PREFIX.pack(table.data_ptr(), slots.data_ptr(), of.data_ptr(), max(t0, cols), count, cols)
+    return _PREFIX.pack(table.data_ptr(), slots.data_ptr(), of.data_ptr(), t0 if t0 > cols else cols, count, cols)
 
 
 def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = None, scores=None, out=None,
@@ -341,7 +343,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
         far = _prefix_block(prefix, seqs, page, dev)
         if far is None:
             return _declined()
-        kib = _prefix_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks, *prefix.table.shape)
+        kib = _prefix_kib(seqs, nh, nkv, hd, cols, page, scores is not None, window, sinks,
+                          *prefix.table.shape)
     if kib < 0:
         return _declined()
     if out is None:
