@@ -160,6 +160,23 @@ def test_a_mask_that_allows_nothing_leaves_minus_infinity():
     assert torch.equal(call(*a), torch.full((2, 300), -math.inf, dtype=FP, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_a_grammar_of_few_tokens_is_what_is_drawn_from(dtype):
+    """Fewer tokens allowed than the sampler's top-k takes: none of the others is drawn."""
+    g = torch.Generator().manual_seed(21)
+    logits = (torch.randn(24, 4096, generator=g) * 4).to(dtype).cuda()
+    allowed = torch.zeros(24, 4096, dtype=torch.bool)
+    for r in range(24):
+        allowed[r, torch.randperm(4096, generator=g)[: 1 + r % 6]] = True
+    y = fusedsample.penalize(logits, mask=fusedsample.pack_mask(allowed).cuda())
+    temp, topp = torch.full((1,), 0.9, dtype=dtype, device="cuda"), torch.full((1,), 0.95, dtype=dtype, device="cuda")
+    for top_k in (1, 30, 64):
+        uniform = (torch.rand(24, 4096, generator=g) * 0.998 + 0.001).cuda()
+        for r in range(24):
+            t = fusedsample.sample(y[r], temp, topp, torch.tensor([top_k], device="cuda"), uniform=uniform[r])
+            assert allowed[r, int(t)], (r, top_k, int(t))
+
+
 def test_one_row_and_shared_parts():
     """(V,) logits; a bias, a mask and a history of one row for all; a bias of the logits' type."""
     g = torch.Generator().manual_seed(3)
