@@ -443,6 +443,8 @@ class PageTable:
         self._active = torch.zeros(seqs, dtype=torch.int64, device=device)
         self._free = list(range(pages - 1, -1, -1))
         self._held: list[list[int | None]] = [[] for _ in range(seqs)]  # (None: given back by `slide`)
+        # `slide` has given back all that a sequence held from column _slid_from to before its _slid
+        self._slid_from, self._slid = 0, [0] * seqs
         self._rows, self._next = [0] * seqs, [0] * seqs  # rows held, the next position
         self.max_prefix = max_len if max_prefix is None else max_prefix
         self._prefix: list[int | None] = [None] * seqs
@@ -588,6 +590,7 @@ class PageTable:
                 held = self._held[seq]
                 self._free += [page for page in held[keep:][::-1] if page is not None]
                 del held[keep:]
+                self._slid[seq] = min(self._slid[seq], keep)
         if len(self._free) > free:  # (no sequence holds more than `keep` pages now)
             self.block_table[:, keep:].fill_(-1)
 
@@ -598,13 +601,16 @@ class PageTable:
         if window < 1 or sinks < 0:
             raise ValueError("a window has at least one row, and its sinks are not negative")
         first, gone = -(-sinks // self.page_size), []
+        if first != self._slid_from:
+            self._slid_from, self._slid = first, [first] * len(self._rows)
         for seq, n in enumerate(self._rows):
-            held = self._held[seq]
-            for c in range(first, max(n - window, 0) // self.page_size):
+            held, end = self._held[seq], max(n - window, 0) // self.page_size
+            for c in range(max(first, self._slid[seq]), end):
                 if held[c] is not None:
                     gone.append((seq, c, -1))
                     self._free.append(held[c])
                     held[c] = None
+            self._slid[seq] = max(self._slid[seq], end)
         self._write(self.block_table, gone)
 
     def release(self, seq: int) -> None:
@@ -613,6 +619,7 @@ class PageTable:
             raise ValueError(f"there is no sequence {seq}")
         self._free += [page for page in self._held[seq][::-1] if page is not None]
         self._held[seq], self._rows[seq], self._next[seq], self._prefix[seq] = [], 0, 0, None
+        self._slid[seq] = 0
         self.block_table[seq].fill_(-1)
         self._place(seq, -1, -1, 0)
 
