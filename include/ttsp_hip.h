@@ -737,6 +737,12 @@ int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_size, int bu
 int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS, int budget,
                      int sinks, int recent, int* work, void* stream);
 
+/* ttsp_paged_evict of sequences whose rows start at position FIRST[b] (int64,
+ * those behind a prefix; NULL: 0): rows with slot_pos < FIRST[b] + sinks are kept
+ * first. Replaces: nothing. */
+int ttsp_paged_evict_from(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS,
+                          const long long* FIRST, int budget, int sinks, int recent, int* work, void* stream);
+
 #endif /* TTSP_HIP_TYPES_ONLY */
 
 #ifdef __cplusplus

@@ -165,6 +165,7 @@ SIGNATURES: dict[str, list] = {
     "ttsp_paged_attention_prefix": [_vp, _vp, _vp, _ll, _vp, _vp, _i, _f, _i, _i, _vp, _vp],
     "ttsp_paged_evict_work_kib": [_i, _i, _i, _i, _i],
     "ttsp_paged_evict": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
+    "ttsp_paged_evict_from": [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp],
 }
 
 

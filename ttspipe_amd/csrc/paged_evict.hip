@@ -1,6 +1,6 @@
 // Eviction from a paged cache by gathered attention weight. For each
 // (sequence, kv head) of n > budget rows, the rows are ranked by
-//   key = +inf where slot_pos < sinks or slot_pos > position - recent,
+//   key = +inf where slot_pos < first + sinks or slot_pos > position - recent,
 //         else the score (NaN counts as -inf; a score of +inf is as good as protected),
 // ties to the lowest slot; the first `budget` are kept. Attention does not
 // care about the order of the slots, so a kept row below `budget` stays where
@@ -51,6 +51,7 @@ struct EvictArgs {
   Paged c;
   const long long* SLOT;
   const long long* POS;
+  const long long* FIRST;  // the position of each sequence's first row (null: 0)
   int budget, sinks, recent, max_moves;
   int* work;  // per (sequence, kv head), list_ints: the count, then max_moves sources and max_moves destinations
   // long caches: parts of `part` slots; behind the lists, per (sequence, kv
@@ -63,6 +64,10 @@ struct EvictArgs {
   int* hists;
   uint2* cands;
   __host__ __device__ size_t list_ints() const { return 1 + 2 * (size_t)max_moves; }
+  // Sequence b's positions below this are its sinks.
+  __device__ __forceinline__ int sinks_of(int b) const {
+    return FIRST ? (int)min(max(FIRST[b], 0LL) + sinks, 0x7fffffffLL) : sinks;
+  }
 };
 
 constexpr int EV_BINS = 2048, EV_COPIES = 8;
@@ -204,6 +209,7 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
   float* const sc = a.c.scores + b * a.c.score_seq + h * a.c.score_head;
   int* const sp = a.c.slot_pos + b * a.c.pos_seq + h * a.c.pos_head;
   const long long newest = a.POS[b] - a.recent;
+  const int sinks = a.sinks_of(b);
   const bool few = INLINE && n - a.budget <= EV_FEW;
   constexpr int LH = D / 8;
   // few: group g of LH lanes holds the row of slot budget + g
@@ -226,7 +232,7 @@ __global__ __launch_bounds__(T) void paged_evict_select_kernel(const EvictArgs a
       f[i] = sc[j], p[i] = sp[j];
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) held[i] = evict_key(f[i], p[i], a.sinks, newest);
+    for (int i = 0; i < R; ++i) held[i] = evict_key(f[i], p[i], sinks, newest);
   }
   if constexpr (INLINE) {
     if (few) {
@@ -355,6 +361,7 @@ struct Part {
   const float* sc;
   const int* sp;
   long long newest;
+  int sinks;
 };
 __device__ __forceinline__ bool part_of(const EvictArgs& a, Part* q) {
   q->p = blockIdx.x, q->h = blockIdx.y, q->b = blockIdx.z;
@@ -365,6 +372,7 @@ __device__ __forceinline__ bool part_of(const EvictArgs& a, Part* q) {
   q->sc = a.c.scores + q->b * a.c.score_seq + q->h * a.c.score_head;
   q->sp = a.c.slot_pos + q->b * a.c.pos_seq + q->h * a.c.pos_head;
   q->newest = a.POS[q->b] - a.recent;
+  q->sinks = a.sinks_of(q->b);
   return q->n > a.budget && q->j0 < q->n;
 }
 
@@ -384,7 +392,7 @@ __device__ __forceinline__ void part_rows(const EvictArgs& a, const Part& q, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int j = first + 64 * (i0 + i);
-      if (i0 + i < steps) f(j, evict_key(sc[i], sp[i], a.sinks, q.newest), j < q.j1);
+      if (i0 + i < steps) f(j, evict_key(sc[i], sp[i], q.sinks, q.newest), j < q.j1);
     }
   }
 }
@@ -636,16 +644,18 @@ extern "C" int ttsp_paged_evict_work_kib(int seqs, int nkv, int cols, int page_s
   return kib > 0x7fffffffu ? -1 : (int)kib;
 }
 
-extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS,
-                                int budget, int sinks, int recent, int* work, hipStream_t stream) {
+extern "C" int ttsp_paged_evict_from(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS,
+                                     const long long* FIRST, int budget, int sinks, int recent, int* work,
+                                     hipStream_t stream) {
   EvictArgs a{};
   if (!paged_args(cache, &a.c) || !a.c.scores || !a.c.slot_pos || !SLOT || !POS || budget < 1 || sinks < 0 ||
-      recent < 0 || sinks > budget - recent)
+      recent < 0 || sinks > budget - recent || (uintptr_t)FIRST % 8)
     return (int)hipErrorInvalidValue;
   const long long cap = a.c.cap();
   if (cap <= budget) return 0;  // no table row holds more than the budget
   a.SLOT = SLOT;
   a.POS = POS;
+  a.FIRST = FIRST;
   a.budget = budget;
   a.sinks = sinks;
   a.recent = recent;
@@ -662,4 +672,9 @@ extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* 
   if (cache->head_dim == 128) launch_evict<128>(a, p, stream);
   else launch_evict<64>(a, p, stream);
   TTSP_RETURN_LAUNCH();
+}
+
+extern "C" int ttsp_paged_evict(const ttsp_paged_cache* cache, const long long* SLOT, const long long* POS,
+                                int budget, int sinks, int recent, int* work, hipStream_t stream) {
+  return ttsp_paged_evict_from(cache, SLOT, POS, nullptr, budget, sinks, recent, work, stream);
 }

@@ -373,9 +373,10 @@ def evict_work(seqs: int, n_local_heads: int, columns: int, page_size: int, budg
 
 
 def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, budget: int, *, sinks: int = 0,
-          recent: int = 0, work=None):
+          recent: int = 0, work=None, first=None):
     """Cut every sequence of more than `budget` rows down to it, in place and in
-    each KV head by itself: kept are rows of the first `sinks` positions and of
+    each KV head by itself: kept are rows of the first `sinks` positions (from
+    `first[b]` on, int64 (sequences,), where given: sequences behind a prefix) and of
     the last `recent` ones (up to `positions[b]`, int64, the newest), then those
     of the largest scores (+inf is as good as protected, NaN counts as -inf), ties
     to the lowest slot. Rows that no step has attended to yet, a prompt's after
@@ -398,12 +399,13 @@ def evict(k_pages, v_pages, block_table, slots, scores, slot_pos, positions, bud
     if c is None:
         return _declined()
     block, nkv, page, _, seqs, cols, _, dev = c
-    if not _vector(slots, torch.int64, seqs, dev) or not _vector(positions, torch.int64, seqs, dev):
+    if (not _vector(slots, torch.int64, seqs, dev) or not _vector(positions, torch.int64, seqs, dev)
+            or (first is not None and not _vector(first, torch.int64, seqs, dev))):
         return _declined()
     if cols * page > budget:  # else no sequence can be longer
         work = _workspace(work, evict_work(seqs, nkv, cols, page, budget), torch.int32, k_pages)
-        _lib.launch("ttsp_paged_evict", dev, block, slots.data_ptr(), positions.data_ptr(), budget, sinks, recent,
-                0 if work is None else work.data_ptr())
+        _lib.launch("ttsp_paged_evict_from", dev, block, slots.data_ptr(), positions.data_ptr(),
+                    0 if first is None else first.data_ptr(), budget, sinks, recent, 0 if work is None else work.data_ptr())
     _stats["evict"] += 1
     return True
 
@@ -424,8 +426,8 @@ class PageTable:
     With `prefixes`, up to so many prefixes of up to `max_prefix` rows (default:
     `max_len`) are held beside the sequences, in pages of the same pools:
     `admit_prefix` takes one in, `admit(rows, prefix=p)` starts a sequence behind it
-    (its own slots count from 0, its positions from the prefix's end), and `prefix`
-    is what `attention` takes. `slide` gives pages back that a window has left."""
+    (its own slots count from 0, its positions from the prefix's end, `starts` on the
+    device), and `prefix` is what `attention` takes. `slide` gives pages back that a window has left."""
 
     def __init__(self, seqs: int, max_len: int, pages: int, page_size: int = 64, device="cuda",
                  max_position: int | None = None, prefixes: int = 0, max_prefix: int | None = None):
@@ -450,8 +452,9 @@ class PageTable:
         self._prefix: list[int | None] = [None] * seqs
         self._prefix_held: list[list[int]] = [[] for _ in range(prefixes)]
         self._prefix_rows = [0] * prefixes
-        self.prefix = None
+        self.prefix = self.starts = None
         if prefixes:
+            self.starts = torch.zeros(seqs, dtype=torch.int64, device=device)
             self.prefix = Prefix(
                 torch.full((prefixes, -(-self.max_prefix // page_size)), -1, dtype=torch.int32, device=device),
                 torch.full((prefixes,), -1, dtype=torch.int64, device=device),
@@ -509,6 +512,7 @@ class PageTable:
         if self.prefix is not None:
             p = self._prefix[seq]
             self.prefix.of[seq].fill_(-1 if p is None else p)
+            self.starts[seq].fill_(self.first_position(seq))
 
     def admit_prefix(self, rows: int):
         """A free prefix with pages for `rows` rows (at positions 0 .. rows - 1; `PagedKVCache.store_prefix`
@@ -690,11 +694,12 @@ class PagedKVCache(nn.Module):
                          window=self.window, sinks=self.sinks, prefix=t.prefix)
 
     def evict(self, budget: int, *, sinks: int = 0, recent: int = 0, work=None):
-        """`evict` on this layer (then, once for all layers, `PageTable.evicted`)."""
+        """`evict` on this layer (then, once for all layers, `PageTable.evicted`): the sinks
+        are a sequence's own first rows, also behind a prefix (all of whose rows stay)."""
         if self.scores is None:
             raise ValueError("only a tracked cache is evicted from")
         if self.window is not None:
             raise ValueError("a cache with a window keeps its rows in order")
         t = self.table
         return evict(self.k_pages, self.v_pages, t.block_table, t.slots, self.scores, self.slot_pos, t.positions, budget,
-                     sinks=sinks, recent=recent, work=work)
+                     sinks=sinks, recent=recent, work=work, first=t.starts)
