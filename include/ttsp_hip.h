@@ -691,8 +691,9 @@ int ttsp_paged_attention(const ttsp_paged_cache* cache, const void* Q, long long
                          const long long* SLOT, void* Y, int nh, float scale, float* work, void* stream);
 
 /* ttsp_paged_attention through a sliding window: of the rows of sequence b the
- * keys are those in slots j < sinks and j > SLOT[b] - window (window >= 1,
- * sinks >= 0), and only they and their pages' table entries are read. Replaces:
+ * keys are those in slots j < sinks and j > s - window (window >= 1, sinks >= 0),
+ * s being SLOT[b] or, where that lies past it, the table's last slot; only they and
+ * their pages' table entries are read. Replaces:
  * nothing (the reference's attention sees the whole cache). */
 int ttsp_paged_attention_window(const ttsp_paged_cache* cache, const void* Q, long long q_seq_stride,
                                 const long long* SLOT, void* Y, int nh, float scale, int window, int sinks,

@@ -308,7 +308,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
     count as infinite.
 
     With a `window`, a sequence's token sees only slots j with j < sinks or
-    j > slots[b] - window: the first rows stay visible, the others slide out. Only
+    j > slots[b] - window (slots[b] cut to the table's last slot, as above): the first
+    rows stay visible, the others slide out. Only
     those rows and their pages' table entries are read, so the pages in between
     may have been given back (`PageTable.slide`). Slots have to be in the order of
     their positions: a cache that `evict` has moved rows in has no window.
