@@ -370,7 +370,10 @@ def prefill_block_chain(block, x, freqs_cis, mask, input_pos, *, xn=None, next_n
     positions; default one launch over the mask's width.
     `window`, `sinks`: each row sees keys j <= its position with j < sinks or
     j > position - window, and the mask's width alone counts (of the block's other
-    arguments `causal` and `attend` go with no window).
+    arguments `causal` and `attend` go with no window). Positions are the cache's:
+    rows behind a shared prefix of n rows see what a `pagedcache.PagedKVCache` with
+    this window and s sinks lets later tokens see where `sinks` is n + s.
+    `decode_block` has no window; such a cache and `decode_batch` have.
 
     The fork's block in its own order with the prefill kernels: RMSNorm,
     wqkv GEMM, q/k head norms + rotary + KV-cache write for every row in one
