@@ -225,7 +225,8 @@ extern "C" int ttsp_prefill_attention_window(const void* Q, long long q_seq_stri
     return (int)hipErrorInvalidValue;
   // a tile's rows are addressed with 32-bit byte offsets from its first one
   const long long lim = (1LL << 31) - 1;
-  if (((L - 1) * k_seq_stride + 128) * 2 > lim || ((L - 1) * v_seq_stride + 128) * 2 > lim)
+  if (L > lim - 127 ||  // (tiles are counted to the one behind the last, in keys)
+      (L > 1 && (k_seq_stride > lim || v_seq_stride > lim)) || ((L - 1) * k_seq_stride + 128) * 2 > lim || ((L - 1) * v_seq_stride + 128) * 2 > lim)
     return (int)hipErrorInvalidValue;
   window = window < L ? window : L, sinks = sinks < L ? sinks : L;
   const PromptPlan p = prompt_plan(S, nh, nkv, L, window, sinks);

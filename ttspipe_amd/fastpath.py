@@ -161,7 +161,7 @@ def _windowed(q, k, v, n_head, n_local_heads, head_dim, out, work, positions, wi
     (_, qh, qr, ql), (_, kh, kr, kl), (_, vh, vr, vl) = q.stride(), k.stride(), v.stride()
     qp, kp, vp, S, L = q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[2], ks[2]
     if (ql != 1 or kl != 1 or vl != 1 or qh % 8 or qr % 8 or kh % 8 or kr % 8 or vh % 8 or vr % 8 or qp % 16 or kp % 16 or vp % 16
-            or S > 1 << 20 or L >= 1 << 31 or max((L - 1) * kr + 128, (L - 1) * vr + 128) >= 1 << 30
+            or S > 1 << 20 or L > (1 << 31) - 128 or max((L - 1) * kr + 128, (L - 1) * vr + 128) >= 1 << 30
             or -(-S * (n_head // n_local_heads) // 64) * n_local_heads > 1 << 20):
         _stats["prefill_declined"] += 1
         return None
