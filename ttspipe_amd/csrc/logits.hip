@@ -8,7 +8,7 @@
 // into the slice in LDS (integer adds, so their order does not matter) while the
 // slice's logits are on their way, and applies the counts as it writes. So there
 // is no count array in memory and no second pass. 256 rows of 131001 logits in fp32
-// after up to 4096 tokens: 59 us, 4.7 TB/s, where a copy of as many bytes runs at 5.1;
+// after up to 4096 tokens: 63 us, 4.4 TB/s, where a copy of as many bytes runs at 5.1;
 // a row of 4096 after 16 tokens 3.5 us, a launch and two reads one after the other.
 #define TTSP_HIP_TYPES_ONLY
 #include "../../include/ttsp_hip.h"
@@ -182,7 +182,8 @@ extern "C" int ttsp_penalize(const ttsp_penalties* p, const void* X, long long x
                 p->mask_row_stride};
   // Every workgroup reads its row's history, so long ones (of enough rows to fill the GPU
   // all the same) go with large slices: 256 rows of 131001 in fp32 after 4096 tokens
-  // 89 us in slices of 2048 and 59 in those of 16384, after 50 tokens 46 and 52.
+  // 66 us in slices of 2048 and 56 in those of 16384, 1500 tokens 53 and 53, 50 tokens 47
+  // and 52 (the same inputs again and again, which the caches then hold in part).
   constexpr int WIDE = 16384, SMALL = 2048;
   const bool wide = p->hist > 1024 && (long long)rows * ((vocab + WIDE - 1) / WIDE) >= LG_FULL;
   const int slice = wide ? WIDE : SMALL;

@@ -10,14 +10,20 @@
 // sequence by itself has group rows for a key). The chunks are cut on the device from
 // the prefixes' lengths and the number of sequences that have each.
 //
-// The weights go to the matrix cores in two parts (bf16 within 2^-16, fp16 2^-22), so
-// that an output is off by its own rounding only, as without a prefix: the products
-// with V are two then, of three in all. 1000 rows for 256 query rows of each of 8 kv
-// heads take 1.36 us more, 1.16 PFLOP/s of the matrix cores' work. 64 sequences behind
-// 32763 rows (32 and 8 heads of 128, bf16; own rows through a window of 512): 75 us and 9
-// for the joining launch. Few query rows are bound by latency: 32 sequences behind 2011
-// rows, own 20 to 900: 24 and 6 us, 2.9 TB/s. The own rows' workgroups are in the same
-// launch (in one of their own before it 36 us a call in place of 30).
+// The weights go to the matrix cores in two parts (bf16 within 2^-16, fp16 2^-22); the
+// products with V are two then, of three in all. In bf16 that takes 3.6 outputs in a
+// thousand a step off the nearest one (32 sequences behind 2011 rows), where three parts,
+// which the own rows' weights have, take 0.4, as without a prefix; the error's norm is
+// 0.00166 of the output's either way, the output's own rounding. The third part would
+// cost 0.3 us there, and 98 in place of 87 us for 64 sequences behind 32763 rows.
+// 1000 rows for 256 query rows of each of 8 kv heads take 1.36 us more, 1.16 PFLOP/s of
+// the matrix cores' work. 64 sequences behind 32763 rows (32 and 8 heads of 128, bf16;
+// own rows through a window of 512): 75 us and 9 for the joining launch, the matrix cores
+// busy 37 % of the time: a SIMD has 1.6 waves on average, since the own rows'
+// workgroups end first, and they wait 39 % of theirs. Few query rows are bound by
+// latency: 32 sequences behind 2011 rows, own 20 to 900: 24 and 6 us, 2.9 TB/s. The own
+// rows' workgroups are in the same launch (in one of their own before it 36 us a call in
+// place of 30).
 #include "tile_attn.h"
 
 namespace ttsp {

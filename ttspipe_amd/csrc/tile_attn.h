@@ -7,8 +7,8 @@
 // so that no register holds what is on its way): RG waves take 32 rows each of the same
 // keys, and with two row groups (RG 2) the other two waves take the other half of a
 // tile's keys and join their sums through LDS at the end. Two workgroups fit a CU: one
-// waits at its barrier while the other computes (eight waves in one workgroup: 64
-// sequences behind 32763 rows 111 us, so 100). A ring of four tiles is slower for few
+// waits at its barrier while the other computes (64 sequences behind 32763 rows: 111 us
+// with eight waves in one workgroup, 100 so, and 84 since a prefix's chunks are longer). A ring of four tiles is slower for few
 // tiles: twice the code to be fetched before it has run once (2 to 5 us).
 //
 // A wave's 32 keys: S^T = K Q^T on the matrix cores (Q stays in registers), so that a
@@ -114,7 +114,7 @@ struct TaWave {
   // first. The others are weighed as the reference is, and only where they come out too
   // large (sixteen of 2^8 and less sum up to no more than 4096) it moves, and they are
   // weighed again; fp16's largest is 2^4 then, which keeps those down to 2^-28 of it
-  // (a prompt of 8111 rows in fp16: 295 us with the maximum of every run, 276 so).
+  // (a prompt of 8111 rows in fp16: 295 us with the maximum of every run, 261 so).
   static constexpr bool FIRST = DT == DT_F16 && PARTS > 1;
   static constexpr float above = FIRST ? pg_above<DT> : 8.0f, below = FIRST ? pg_below<DT> : DT == DT_F16 ? 4.0f : 0.0f;
   __device__ __forceinline__ void move(const f32x16_v& s, float scale2) {

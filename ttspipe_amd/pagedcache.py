@@ -316,7 +316,8 @@ def attention(q, k_pages, v_pages, block_table, slots, *, scale: float | None = 
 
     With a `prefix`, sequence b also sees all rows of prefix `prefix.of[b]`, whose
     pages are read once for all sequences that have it. The window and the scores
-    are those of its own rows.
+    are those of its own rows. (In bf16 a prefix row's weight counts within 2^-16 of
+    itself, where an own row's counts whole.)
 
     With `scores`, each slot's weight, summed over the query heads of its KV
     head, is added to it (what `evict` ranks by). `work`: an fp32 workspace of
@@ -632,7 +633,8 @@ class PageTable:
 class PagedKVCache(nn.Module):
     """One layer's pools on a `PageTable`. `tracked`: with the scores and slot
     positions that `evict` needs. `window`, `sinks`: `attention` goes through that
-    window (and `evict` is refused: it takes the slots out of order)."""
+    window (and `evict` is refused: it takes the slots out of order; what a tracked
+    one gathers is in `scores` for its caller)."""
 
     def __init__(self, table: PageTable, n_heads: int, head_dim: int = 128, dtype=torch.bfloat16, tracked: bool = False,
                  window: int | None = None, sinks: int = 0):
